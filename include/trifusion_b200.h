@@ -512,6 +512,43 @@ int tf_ragged_copy_fwd(void* packed, void* const* dense, const int64_t* groups, 
                        const int64_t* step_bytes, int ntensors, const int64_t* lengths, int batch,
                        int to_dense, void* stream);
 
+/* ========================================================================
+ * Streaming operators (no counterpart in the reference, which sees whole clips):
+ * rotary positions at any position, and a linear recurrence with a carried state.
+ * ======================================================================== */
+
+/* Rotary positions of q [B,T,Hq,D] and k [B,T,Hk,D] (Hk may be 0), FP32 or BF16:
+ * theta = positions[b,t] * inv_freq[i] for i < R/2 (FP64 angles), pair (x1, x2) ->
+ * amplitude * (x1 cos - x2 sin, x2 cos + x1 sin) in FP32 with one rounding; pairs are
+ * (i, i + R/2), or (2i, 2i + 1) with `interleaved`; elements R..D-1 are copied.
+ * q_out/k_out may be q/k themselves. `strides` holds 14 int64 element strides: q, k,
+ * q_out, k_out (batch, time, head each; innermost stride 1), positions (batch, time).
+ * R/2 <= 512, D * (Hq + Hk) <= 65535 and B * T < 2^31 (else TF_ERR_SIZE). */
+int tf_rotary_positions_fwd(const void* q, const void* k, void* q_out, void* k_out, int dtype,
+                            const int64_t* positions, const double* inv_freq, float amplitude, int interleaved,
+                            const int64_t* strides, int batch, int seqlen, int q_heads, int k_heads, int head_dim,
+                            int rotary_dim, void* stream);
+
+/* Linear attention with a decay for each head:
+ *   S_t = e^decay[b,h,t] S_(t-1) + k_t v_t^T (key_dim x value_dim, FP32),
+ *   out_t = scale * q_t S_t,
+ * q, k [B,T,Hq,N], v and out [B,T,H,P] (FP32 or BF16), decay [B,H,T] FP32, N and P
+ * multiples of 8 up to 256. `state` (nullable) [state_slots,H,N,P] FP32, 16-byte
+ * aligned: row b starts from entry slots[b] (or b) and leaves its last state there;
+ * with `fresh` it starts from zero instead. A negative slot: zero outputs, no state
+ * changes; a slot >= state_slots or one that an earlier row has: NaN outputs, no
+ * state changes. Tokens at or past lengths[b] (nullable int64 [B]) are not read and
+ * their outputs are zero. seqlen 1 is the single-token form.
+ * `strides` holds 17 int64 element strides: q, k, v (batch, time, head), decay (batch,
+ * head, time), out (batch, time, head), state (slot, head); innermost strides are 1
+ * and the state is contiguous over [N,P]. `workspace` holds
+ * tf_linear_attention_workspace_size bytes (256-byte aligned, contents irrelevant). */
+int64_t tf_linear_attention_workspace_size(int batch, int seqlen, int heads, int key_dim, int value_dim, int dtype);
+int tf_linear_attention_fwd(const void* q, const void* k, const void* v, int dtype, const float* decay, float* state,
+                            int64_t state_slots, int fresh, const int64_t* slots, const int64_t* lengths, void* out,
+                            const int64_t* strides, int batch, int seqlen, int heads, int groups, int key_dim,
+                            int value_dim, float scale, void* workspace, int64_t workspace_bytes, void* stream);
+
 #ifdef __cplusplus
 }
 #endif

@@ -1,0 +1,185 @@
+// Linear attention with a decay for each head, and a carried state:
+//
+//   S_t = e^{g_t} S_{t-1} + k_t v_t^T      (N x P, FP32)
+//   o_t = scale * q_t S_t
+//
+// q and k heads are shared by H / Hq heads of v. This file holds the recurrent
+// form (one token after another, the state in registers).
+#include "../../include/trifusion_b200.h"
+#include "linear_attention.cuh"
+#include "tf_common.cuh"
+#include "tf_host.cuh"
+
+namespace tf {
+namespace {
+
+__device__ __forceinline__ float ld_f(const float* p) { return __ldg(p); }
+__device__ __forceinline__ float ld_f(const bf16* p) { return bf2f(__ldg(p)); }
+__device__ __forceinline__ void st_f(float* p, float x) { *p = x; }
+__device__ __forceinline__ void st_f(bf16* p, float x) { *p = __float2bfloat16_rn(x); }
+
+// e^g for a log decay g. -inf (a reset) gives exactly 0; NaN stays NaN.
+__device__ __forceinline__ float decay_factor(float g) { return ex2_approx(g * kLog2e); }
+
+// ---- recurrent form ------------------------------------------------------------
+// One block: one row, one head, 32 columns of its state. Thread (warp w, lane l)
+// holds columns 4 (l % 8) .. +3 of state rows w * 4 + l / 8 + 32 i, so a warp reads
+// four 128-byte row segments at a time, and the sum over rows for the output is
+// two shuffles and eight partial sums in shared memory. A single token is bound by
+// the state's bytes (read once, written once); a block has 16 KB of them in flight
+// at N = 128.
+constexpr int kScanThreads = 256;
+
+template <typename T, int NR>
+__global__ void __launch_bounds__(kScanThreads) linear_scan_kernel(const __grid_constant__ LinearParams p) {
+  __shared__ float4 partial[2][8][8];
+  const int slices = (p.P + 31) / 32;
+  const int slice = blockIdx.x % slices;
+  const int row = blockIdx.x / slices;
+  const int h = row % p.H, b = row / p.H;
+  const int w = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const int col = slice * 32 + 4 * (lane & 7);
+  const int r0 = w * 4 + (lane >> 3);
+  const bool on = col < p.P;
+
+  const int64_t slot = p.slots ? p.slots[b] : b;
+  const bool in_pool = p.state && slot >= 0 && slot < p.nslots;
+  float* st = p.state + (in_pool ? slot * p.ss[0] + h * p.ss[1] : 0);
+  float4 s[NR];
+#pragma unroll
+  for (int i = 0; i < NR; ++i) {
+    const int n = r0 + 32 * i;
+    s[i] = in_pool && !p.fresh && on && n < p.N ? *reinterpret_cast<const float4*>(st + static_cast<int64_t>(n) * p.P + col)
+                                                : make_float4(0.f, 0.f, 0.f, 0.f);
+  }
+  bool taken = false;  // an earlier row has this slot
+  if (p.slots) {
+    if (in_pool)
+      for (int i = threadIdx.x; i < b; i += kScanThreads) taken |= p.slots[i] == slot;
+    taken = __syncthreads_or(taken);
+  }
+  int64_t len = p.T;
+  if (p.lengths) len = min(max(p.lengths[b], static_cast<int64_t>(0)), len);
+  T* out = static_cast<T*>(p.out) + b * p.so[0] + h * p.so[2];
+  if (p.state && (!in_pool || taken)) {
+    // No state of its own: zeros for a row that is padding, NaN for one that names a wrong slot.
+    if (w == 0) {
+      const float fill = slot < 0 ? 0.f : __int_as_float(0x7fc00000);
+      const int c = slice * 32 + lane;
+      if (c < p.P)
+        for (int64_t t = 0; t < p.T; ++t) st_f(out + t * p.so[1] + c, t < len ? fill : 0.f);
+    }
+    return;
+  }
+  const int hq = h / (p.H / p.Hq);
+  const T* q = static_cast<const T*>(p.q) + b * p.sq[0] + hq * p.sq[2];
+  const T* k = static_cast<const T*>(p.k) + b * p.sk[0] + hq * p.sk[2];
+  const T* v = static_cast<const T*>(p.v) + b * p.sv[0] + h * p.sv[2];
+  const float* g = p.decay + b * p.sg[0] + h * p.sg[1];
+  for (int64_t t = 0; t < len; ++t) {
+    const float a = decay_factor(g[t * p.sg[2]]);
+    float vv[4];
+#pragma unroll
+    for (int j = 0; j < 4; ++j) vv[j] = on ? ld_f(v + t * p.sv[1] + col + j) : 0.f;
+    float4 o = make_float4(0.f, 0.f, 0.f, 0.f);
+#pragma unroll
+    for (int i = 0; i < NR; ++i) {
+      const int n = r0 + 32 * i;
+      const float kn = n < p.N ? ld_f(k + t * p.sk[1] + n) : 0.f;
+      const float qn = n < p.N ? ld_f(q + t * p.sq[1] + n) : 0.f;
+      s[i].x = fmaf(kn, vv[0], a * s[i].x);
+      s[i].y = fmaf(kn, vv[1], a * s[i].y);
+      s[i].z = fmaf(kn, vv[2], a * s[i].z);
+      s[i].w = fmaf(kn, vv[3], a * s[i].w);
+      o.x = fmaf(qn, s[i].x, o.x);
+      o.y = fmaf(qn, s[i].y, o.y);
+      o.z = fmaf(qn, s[i].z, o.z);
+      o.w = fmaf(qn, s[i].w, o.w);
+    }
+#pragma unroll
+    for (int d = 8; d < 32; d <<= 1) {
+      o.x += __shfl_xor_sync(0xffffffffu, o.x, d);
+      o.y += __shfl_xor_sync(0xffffffffu, o.y, d);
+      o.z += __shfl_xor_sync(0xffffffffu, o.z, d);
+      o.w += __shfl_xor_sync(0xffffffffu, o.w, d);
+    }
+    if (lane < 8) partial[t & 1][w][lane] = o;
+    __syncthreads();
+    if (w == 0) {
+      const float* f = reinterpret_cast<const float*>(&partial[t & 1][0][0]);
+      float sum = 0.f;
+#pragma unroll
+      for (int i = 0; i < 8; ++i) sum += f[32 * i + lane];
+      const int c = slice * 32 + lane;
+      if (c < p.P) st_f(out + t * p.so[1] + c, sum * p.scale);
+    }
+  }
+  if (w == 0 && slice * 32 + lane < p.P)
+    for (int64_t t = len; t < p.T; ++t) st_f(out + t * p.so[1] + slice * 32 + lane, 0.f);
+  if (p.state && on && (len > 0 || p.fresh))
+#pragma unroll
+    for (int i = 0; i < NR; ++i) {
+      const int n = r0 + 32 * i;
+      if (n < p.N) *reinterpret_cast<float4*>(st + static_cast<int64_t>(n) * p.P + col) = s[i];
+    }
+}
+
+template <typename T>
+void launch_scan(const LinearParams& p, cudaStream_t stream) {
+  const unsigned grid = static_cast<unsigned>(static_cast<int64_t>(p.B) * p.H * ((p.P + 31) / 32));
+  if (p.N <= 32) linear_scan_kernel<T, 1><<<grid, kScanThreads, 0, stream>>>(p);
+  else if (p.N <= 64) linear_scan_kernel<T, 2><<<grid, kScanThreads, 0, stream>>>(p);
+  else if (p.N <= 128) linear_scan_kernel<T, 4><<<grid, kScanThreads, 0, stream>>>(p);
+  else linear_scan_kernel<T, 8><<<grid, kScanThreads, 0, stream>>>(p);
+}
+
+}  // namespace
+}  // namespace tf
+
+extern "C" {
+
+int64_t tf_linear_attention_workspace_size(int batch, int seqlen, int heads, int key_dim, int value_dim, int dtype) {
+  (void)dtype;
+  if (batch <= 0 || seqlen <= 0 || heads <= 0 || key_dim <= 0 || value_dim <= 0) return 0;
+  return 0;
+}
+
+int tf_linear_attention_fwd(const void* q, const void* k, const void* v, int dtype, const float* decay, float* state,
+                            int64_t state_slots, int fresh, const int64_t* slots, const int64_t* lengths, void* out,
+                            const int64_t* strides, int batch, int seqlen, int heads, int groups, int key_dim,
+                            int value_dim, float scale, void* workspace, int64_t workspace_bytes, void* stream) {
+  using namespace tf;
+  if (dtype != TF_F32 && dtype != TF_BF16) return TF_ERR_ARG;
+  if (!strides || batch < 0 || seqlen < 0 || heads < 0 || groups < 1 || heads % groups || state_slots < 0)
+    return TF_ERR_ARG;
+  if (key_dim < 8 || value_dim < 8 || key_dim % 8 || value_dim % 8 || key_dim > 256 || value_dim > 256)
+    return TF_ERR_ARG;
+  if (slots && !state) return TF_ERR_ARG;
+  if (!slots && state && state_slots < batch) return TF_ERR_ARG;
+  if (batch == 0 || heads == 0 || (seqlen == 0 && !(state && fresh))) return TF_OK;
+  if (seqlen > 0 && (!q || !k || !v || !decay || !out)) return TF_ERR_ARG;
+  LinearParams p{};
+  p.q = q, p.k = k, p.v = v, p.out = out;
+  p.decay = decay;
+  p.state = state;
+  p.nslots = state_slots;
+  p.fresh = fresh != 0;
+  p.slots = slots;
+  p.lengths = lengths;
+  const int64_t* s = strides;
+  for (int i = 0; i < 3; ++i) p.sq[i] = s[i], p.sk[i] = s[3 + i], p.sv[i] = s[6 + i], p.sg[i] = s[9 + i], p.so[i] = s[12 + i];
+  p.ss[0] = s[15], p.ss[1] = s[16];
+  if (state && (reinterpret_cast<uintptr_t>(state) % 16 || (state_slots > 1 && p.ss[0] % 4) || (heads > 1 && p.ss[1] % 4)))
+    return TF_ERR_LAYOUT;
+  p.B = batch, p.T = seqlen, p.H = heads, p.Hq = groups, p.N = key_dim, p.P = value_dim;
+  p.scale = scale;
+  if (static_cast<int64_t>(batch) * heads * ((value_dim + 31) / 32) > 0x7fffffffll) return TF_ERR_SIZE;
+  (void)workspace, (void)workspace_bytes;
+  const int st = check_device();
+  if (st != TF_OK) return st;
+  if (dtype == TF_F32) launch_scan<float>(p, static_cast<cudaStream_t>(stream));
+  else launch_scan<bf16>(p, static_cast<cudaStream_t>(stream));
+  return launch_status();
+}
+
+}  // extern "C"

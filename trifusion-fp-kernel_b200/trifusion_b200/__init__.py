@@ -17,6 +17,10 @@ _EXPORTS = {
     "fused_mamba": (".mamba_fused", "fused_mamba"),
     "fused_recurrence": (".mamba_fused", "fused_recurrence"),
     "check_device_error": ("._lib", "check_device_error"),
+    "rotary_frequencies": (".rotary", "rotary_frequencies"),
+    "apply_rotary": (".rotary", "apply_rotary"),
+    "linear_attention": (".linear_attention", "linear_attention"),
+    "linear_attention_step": (".linear_attention", "linear_attention_step"),
 }
 
 

@@ -83,12 +83,18 @@ SIGNATURES = {
     "tf_local_topk_fwd": [_p, _q, _p, _q, _p, _p, _p, _i, _i, _p],
     "tf_decoder_heads_scratch_bytes": [_i],
     "tf_decoder_heads_fwd": [_p] * 18 + [_q, _p, _i, _p],
+    # Streaming operators.
+    "tf_rotary_positions_fwd": [_p, _p, _p, _p, _i, _p, _p, _f, _i, _p, _i, _i, _i, _i, _i, _i, _p],
+    "tf_linear_attention_workspace_size": [_i, _i, _i, _i, _i, _i],
+    "tf_linear_attention_fwd": [_p, _p, _p, _i, _p, _p, _q, _i, _p, _p, _p, _p, _i, _i, _i, _i, _i, _i, _f, _p, _q,
+                                _p],
 }
 _RESTYPES = {"tf_status_string": ctypes.c_char_p, "tf_last_cuda_error": ctypes.c_char_p,
              "tf_recurrence_workspace_size": ctypes.c_size_t,
              "tf_recurrence_workspace_size_multi": ctypes.c_size_t,
              "tf_query_read_state_floats": ctypes.c_int64,
-             "tf_decoder_heads_scratch_bytes": ctypes.c_int64}
+             "tf_decoder_heads_scratch_bytes": ctypes.c_int64,
+             "tf_linear_attention_workspace_size": ctypes.c_int64}
 
 
 class RecurrenceIO(ctypes.Structure):
@@ -189,6 +195,14 @@ def require_cuda(op, *tensors):
     if dev.type != "cuda" or any(t.device != dev for t in tensors):
         raise RuntimeError(f"{op}: all tensors must be CUDA tensors on one device")
     return dev
+
+
+def no_gradient(op, *tensors):
+    """Refuse operands that autograd would expect a gradient for (there is no backward pass)."""
+    import torch
+
+    if torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in tensors):
+        raise RuntimeError(f"{op}: no backward pass; detach the operands or call it under torch.no_grad()")
 
 
 def launch(fn, device, *args):
