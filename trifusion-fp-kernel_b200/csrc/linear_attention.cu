@@ -4,7 +4,8 @@
 //   o_t = scale * q_t S_t
 //
 // q and k heads are shared by H / Hq heads of v. This file holds the recurrent
-// form (one token after another, the state in registers).
+// form (one token after another, the state in registers); linear_chunks.cu the
+// chunked form on the tensor cores.
 #include "../../include/trifusion_b200.h"
 #include "linear_attention.cuh"
 #include "tf_common.cuh"
@@ -138,10 +139,11 @@ void launch_scan(const LinearParams& p, cudaStream_t stream) {
 
 extern "C" {
 
-int64_t tf_linear_attention_workspace_size(int batch, int seqlen, int heads, int key_dim, int value_dim, int dtype) {
-  (void)dtype;
-  if (batch <= 0 || seqlen <= 0 || heads <= 0 || key_dim <= 0 || value_dim <= 0) return 0;
-  return 0;
+int64_t tf_linear_attention_workspace_size(int batch, int seqlen, int heads, int groups, int key_dim, int value_dim,
+                                           int dtype) {
+  if (batch <= 0 || seqlen <= 0 || heads <= 0 || groups <= 0 || heads % groups || key_dim <= 0 || value_dim <= 0)
+    return 0;
+  return tf::linear_chunk_workspace(batch, seqlen, heads, groups, key_dim, value_dim, dtype);
 }
 
 int tf_linear_attention_fwd(const void* q, const void* k, const void* v, int dtype, const float* decay, float* state,
@@ -174,9 +176,12 @@ int tf_linear_attention_fwd(const void* q, const void* k, const void* v, int dty
   p.B = batch, p.T = seqlen, p.H = heads, p.Hq = groups, p.N = key_dim, p.P = value_dim;
   p.scale = scale;
   if (static_cast<int64_t>(batch) * heads * ((value_dim + 31) / 32) > 0x7fffffffll) return TF_ERR_SIZE;
-  (void)workspace, (void)workspace_bytes;
-  const int st = check_device();
+  int st = check_device();
   if (st != TF_OK) return st;
+  if (linear_chunk_workspace(batch, seqlen, heads, groups, key_dim, value_dim, dtype) > 0) {
+    st = launch_linear_chunks(p, dtype, workspace, workspace_bytes, static_cast<cudaStream_t>(stream));
+    if (st >= 0) return st;
+  }
   if (dtype == TF_F32) launch_scan<float>(p, static_cast<cudaStream_t>(stream));
   else launch_scan<bf16>(p, static_cast<cudaStream_t>(stream));
   return launch_status();

@@ -1,6 +1,7 @@
 // Parameters of the linear-attention launches (linear_attention.cu).
 #pragma once
 
+#include <cuda_runtime.h>
 #include <stdint.h>
 
 namespace tf {
@@ -20,5 +21,13 @@ struct LinearParams {
   int fresh;                // the state is written but not read: it starts at zero
   float scale;
 };
+
+// The chunked form (linear_chunks.cu): bytes of workspace it takes, 0 where it does not
+// apply; a launch of it, or -1 where a tensor's layout does not allow it.
+int64_t linear_chunk_workspace(int B, int T, int H, int Hq, int N, int P, int dtype);
+int launch_linear_chunks(const LinearParams& l, int dtype, void* workspace, int64_t workspace_bytes,
+                         cudaStream_t stream);
+int read_linear_error(int reset);
+int* host_error_word();
 
 }  // namespace tf

@@ -1,0 +1,731 @@
+// Linear attention with a decay for each head: the chunked form for prompts.
+//
+// Chunk of C = 64 tokens, state S (N x P) before it, c_i = g_1 + .. + g_i within it:
+//
+//   o_i   = scale * ( e^{c_i} q_i S  +  sum_{j <= i} e^{c_i - c_j} (q_i . k_j) v_j )
+//   S'    = e^{c_C} S + sum_j k_j (e^{c_C - c_j} v_j)^T
+//
+// Everything with a token pair or a state element in it is a 64-token matrix
+// product on the tensor cores (tcgen05, BF16 operands, FP32 accumulators in TMEM),
+// with the value dimension on the 128 accumulator lanes:
+//
+//   D [i, j]     = q k^T                       M 64   N 64   K N
+//   dS^T [p, n]  = (w v)^T k, w_j = e^{c_C-c_j}  M 128  N N    K 64, three times
+//   OI^T [p, i]  = S^T q^T                     M 128  N 64   K N
+//   OP^T [p, i]  = v^T P^T, P = D e^{c_i-c_j}  M 128  N 64   K 64, once a head
+//
+// The 128 lanes are two blocks of 64 value columns: the two halves of one wide head
+// (P > 64), or two heads (P <= 64) that share a k head, so that their D is formed
+// once and their state updates are one product.
+//
+// Precision. q, k and v enter the products as they are (BF16). w v is split into
+// three BF16 parts whose sum holds its 24 bits, so the state and its FP32 update are
+// as exact as an FP32 product; S lives in FP32 registers. Two roundings to BF16 are
+// made on the way to the output: P (after the decay) and S as the operand of q S.
+// Each is half a step of a term, like the output's own rounding. The sums of decays
+// of the state's weights run from the chunk's end (exact where they matter), the
+// ones of e^{c_i} from its start.
+//
+// Long rows on few heads: the time axis is cut into segments. One launch forms every
+// segment's own state from zero, one joins them (S_in of each segment), and the main
+// launch runs all segments side by side.
+#include <cuda.h>
+#include <cudaTypedefs.h>
+
+#include <atomic>
+
+#include "../../include/trifusion_b200.h"
+#include "linear_attention.cuh"
+#include "sm100.cuh"
+#include "tf_host.cuh"
+
+namespace tf {
+namespace {
+using namespace sm100;
+
+constexpr int kC = 64;                // tokens of a chunk
+constexpr int kBox = 8192;            // bytes of a 64 x 64 BF16 tile
+constexpr int kEpiWarps = 8, kPrepWarps = 4;
+constexpr int kThreads = 32 * (kEpiWarps + kPrepWarps + 1);
+constexpr float kMinLog2 = -256.f;    // a decay below it is zero in FP32 against any state
+
+__device__ int g_linear_error = 0;    // 1: a bounded wait gave up
+
+struct ChunkParams {
+  CUtensorMap tm_q, tm_k, tm_v;
+  LinearParams l;
+  int pairs;       // CTAs of a k head: pairs of its heads (P <= 64), or its heads
+  int chunks;      // of T
+  int segs;        // segments of the time axis
+  int seg_chunks;  // chunks of a segment
+  float* seg_state;   // [B*H][segs][N][P]: the state before each segment
+  float* seg_decay;   // [B*H][segs]: log2 decay over the segment
+  int* err_host;
+};
+
+// Shared memory, in bytes from a 1024-byte boundary. The values of stage 1 and 0 lie
+// around one zero tile: a block's tile and the zero tile are the two 64-column blocks
+// of the operand of its head's OP product.
+template <int NK>
+struct Layout {
+  static constexpr int q = 0;                          // [stage][NK]
+  static constexpr int k = q + 2 * NK * kBox;          // [stage][NK]
+  static constexpr int v = k + 2 * NK * kBox;          // a1 a0 zero b0 b1
+  static constexpr int wv = v + 5 * kBox;              // [part][block]
+  static constexpr int s = wv + 6 * kBox;              // [NK] of 128 rows
+  static constexpr int p = s + 2 * NK * kBox;          // [block]
+  static constexpr int misc = p + 2 * kBox;
+  static __device__ __forceinline__ uint32_t va(int stage) { return v + (stage ? 0 : 1) * kBox; }
+  static __device__ __forceinline__ uint32_t vb(int stage) { return v + (stage ? 4 : 3) * kBox; }
+};
+struct alignas(16) Misc {
+  uint64_t full[2], empty[2], d_full[2], ds_full[2], o_full;
+  uint32_t tmem;
+  alignas(16) float cs[2][2][kC];  // [stage][head] log2 decays summed from the chunk's start
+  float ecs[2][2][kC];   // 2^cs
+  float w[2][2][kC];     // 2^(sum after the token), 0 past the length
+  float total[2][2];     // 2^(sum of the chunk)
+};
+template <int NK>
+constexpr int smem_bytes() {
+  return Layout<NK>::misc + static_cast<int>(sizeof(Misc)) + 1024;
+}
+
+// TMEM columns.
+constexpr uint32_t kColD = 0, kColOI = 128, kColOP = 192, kColDS = 256;
+
+constexpr uint32_t idesc_bf16(int m, int n, bool a_mn, bool b_mn) {
+  return idesc_f16_f32(m, n, a_mn, b_mn) | (1u << 7) | (1u << 10);
+}
+
+__device__ __forceinline__ bool bar_or(int id, int n, bool x) {
+  uint32_t r;
+  asm volatile(
+      "{\n .reg .pred p, q;\n setp.ne.b32 p, %1, 0;\n barrier.cta.red.or.pred q, %2, %3, p;\n"
+      " selp.u32 %0, 1, 0, q;\n}\n"
+      : "=r"(r)
+      : "r"(static_cast<uint32_t>(x)), "r"(id), "r"(n)
+      : "memory");
+  return r != 0;
+}
+__device__ __forceinline__ void mbar_arrive(uint64_t* bar) {
+  asm volatile("{\n .reg .b64 st;\n mbarrier.arrive.shared::cta.b64 st, [%0];\n}\n" ::"r"(smem_u32(bar)) : "memory");
+}
+__device__ __forceinline__ uint4 lds16(uint32_t a) {
+  uint4 v;
+  asm volatile("ld.shared.v4.b32 {%0,%1,%2,%3}, [%4];" : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w) : "r"(a));
+  return v;
+}
+__device__ __forceinline__ void sts16(uint32_t a, uint4 v) {
+  asm volatile("st.shared.v4.b32 [%0], {%1,%2,%3,%4};" ::"r"(a), "r"(v.x), "r"(v.y), "r"(v.z), "r"(v.w) : "memory");
+}
+__device__ __forceinline__ void sts4(uint32_t a, uint32_t v) {
+  asm volatile("st.shared.b32 [%0], %1;" ::"r"(a), "r"(v) : "memory");
+}
+// 16 TMEM lanes x 32 columns as m16n8 fragments: thread t gets lanes t/4 and t/4 + 8,
+// columns 8 x + 2 (t % 4) + {0, 1}, as r[4 x + 0..1] and r[4 x + 2..3].
+__device__ __forceinline__ void tmem_ld_frag(uint32_t taddr, float (&r)[16]) {
+  uint32_t* u = reinterpret_cast<uint32_t*>(r);
+  asm volatile(
+      "tcgen05.ld.sync.aligned.16x256b.x4.b32 {%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15}, [%16];"
+      : "=r"(u[0]), "=r"(u[1]), "=r"(u[2]), "=r"(u[3]), "=r"(u[4]), "=r"(u[5]), "=r"(u[6]), "=r"(u[7]),
+        "=r"(u[8]), "=r"(u[9]), "=r"(u[10]), "=r"(u[11]), "=r"(u[12]), "=r"(u[13]), "=r"(u[14]), "=r"(u[15])
+      : "r"(taddr)
+      : "memory");
+}
+// x as BF16 pairs hi, and what is left of it.
+__device__ __forceinline__ uint32_t take_bf16(float& a, float& b) {
+  const uint32_t h = pack_bf16x2(a, b);
+  const float2 f = unpack_bf16x2(h);
+  a -= f.x;
+  b -= f.y;
+  return h;
+}
+
+// What a CTA works on.
+struct Unit {
+  int b, hk, seg;     // row, k head, segment
+  int head0, nheads;  // v heads: one (wide, or without a partner) or two
+  int64_t len;        // the row's length
+  int first, last;    // its chunks with live tokens
+};
+template <bool WIDE>
+__device__ __forceinline__ Unit unit_of(const ChunkParams& p, int x) {
+  Unit u;
+  const LinearParams& l = p.l;
+  u.seg = x % p.segs;
+  x /= p.segs;
+  const int pr = x % p.pairs;
+  x /= p.pairs;
+  u.hk = x % l.Hq;
+  u.b = x / l.Hq;
+  const int share = l.H / l.Hq;
+  u.head0 = u.hk * share + (WIDE ? pr : 2 * pr);
+  u.nheads = WIDE || 2 * pr + 1 >= share ? 1 : 2;
+  u.len = l.T;
+  if (l.lengths) u.len = min(max(l.lengths[u.b], static_cast<int64_t>(0)), static_cast<int64_t>(l.T));
+  const int live = static_cast<int>((u.len + kC - 1) / kC);
+  u.first = u.seg * p.seg_chunks;
+  u.last = min(live, u.first + p.seg_chunks);
+  return u;
+}
+
+// FULL: the outputs and the final state; otherwise a segment's own state from zero.
+template <int NK, bool WIDE, bool FULL>
+__global__ void __launch_bounds__(kThreads, 1) linear_chunk_kernel(const __grid_constant__ ChunkParams p) {
+  using L = Layout<NK>;
+  extern __shared__ unsigned char smem_raw[];
+  const uint32_t sb = (smem_u32(smem_raw) + 1023u) & ~1023u;
+  Misc& m = *reinterpret_cast<Misc*>(smem_raw + (sb - smem_u32(smem_raw)) + L::misc);
+  const LinearParams& l = p.l;
+  const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
+  const Unit u = unit_of<WIDE>(p, blockIdx.x);
+  const int live_chunks = static_cast<int>((u.len + kC - 1) / kC);
+
+  int64_t slot = 0;
+  bool in_pool = false;
+  if (FULL) {
+    slot = l.slots ? l.slots[u.b] : u.b;
+    in_pool = l.state && slot >= 0 && slot < l.nslots;
+    bool taken = false;  // an earlier row has this slot
+    if (l.slots) {
+      for (int i = tid; i < u.b; i += kThreads) taken |= l.slots[i] == slot;
+      taken = __syncthreads_or(taken);
+    }
+    const bool dead = l.state && (!in_pool || taken);
+    // Rows without a state of their own, and chunks past the length: zeros, or NaN for a wrong slot.
+    const int64_t t0 = dead ? static_cast<int64_t>(u.first) * kC
+                            : max(min(static_cast<int64_t>(live_chunks), static_cast<int64_t>(u.first + p.seg_chunks)),
+                                  static_cast<int64_t>(u.first)) * kC;
+    const int64_t t1 = min(static_cast<int64_t>(l.T), static_cast<int64_t>(u.first + p.seg_chunks) * kC);
+    const int width = u.nheads * l.P;
+    for (int64_t i = tid; i < (t1 - t0) * width; i += kThreads) {
+      const int64_t t = t0 + i / width;
+      const int c = static_cast<int>(i % width);
+      static_cast<bf16*>(l.out)[u.b * l.so[0] + t * l.so[1] + (u.head0 + c / l.P) * l.so[2] + c % l.P] =
+          __float2bfloat16_rn(dead && slot >= 0 && t < u.len ? __int_as_float(0x7fc00000) : 0.f);
+    }
+    if (dead) return;
+    if (live_chunks == 0 && u.seg == 0 && l.fresh)
+      for (int i = tid; i < u.nheads * l.N * l.P; i += kThreads)
+        l.state[slot * l.ss[0] + (u.head0 + i / (l.N * l.P)) * l.ss[1] + i % (l.N * l.P)] = 0.f;
+    if (u.first >= u.last) return;
+  } else if (u.first + p.seg_chunks >= live_chunks) {
+    return;  // nothing reads this segment's state
+  }
+
+  // ---- set-up ------------------------------------------------------------------
+  const bool two = WIDE || u.nheads == 2;  // the second block of value columns is there
+  if (warp == kEpiWarps + kPrepWarps) {
+    tmem_alloc(&m.tmem, 512);
+    tmem_relinquish();
+  }
+  if (tid == 0) {
+    for (int i = 0; i < 2; ++i) {
+      mbar_init(&m.full[i], 1);
+      mbar_init(&m.empty[i], kEpiWarps);
+      mbar_init(&m.d_full[i], 2);   // the product's commit, and the thread that issued it (for the decay sums)
+      mbar_init(&m.ds_full[i], 2);
+    }
+    mbar_init(&m.o_full, 1);
+    fence_mbar_init();
+  }
+  // The zero tile, and the second block's tiles where there is none.
+  for (int i = tid; i < kBox / 16; i += kThreads) {
+    const uint4 z = make_uint4(0, 0, 0, 0);
+    sts16(sb + L::v + 2 * kBox + 16 * i, z);
+    if (!two) {
+      sts16(sb + L::vb(0) + 16 * i, z);
+      sts16(sb + L::vb(1) + 16 * i, z);
+      for (int part = 0; part < 3; ++part) sts16(sb + L::wv + (2 * part + 1) * kBox + 16 * i, z);
+    }
+  }
+  fence_async_smem();
+  tc_fence_before();
+  __syncthreads();
+  tc_fence_after();
+  const uint32_t tm = m.tmem;
+  bool bad = false;  // a bounded wait gave up
+
+  if (warp == kEpiWarps + kPrepWarps) {
+    // ---- loads ------------------------------------------------------------------
+    if (lane == 0) {
+      const int boxes = (FULL ? 2 : 1) * NK + (two ? 2 : 1);
+      int issued = 0;
+      for (int c = u.first; c < u.last; ++c) {
+        const int it = c - u.first, st = it & 1;
+        if (it >= 2 && !mbar_wait(&m.empty[st], ((it >> 1) - 1) & 1)) {
+          bad = true;
+          break;
+        }
+        mbar_arrive_expect_tx(&m.full[st], boxes * kBox);
+        for (int x = 0; x < NK; ++x) {
+          if (FULL) tma_load_4d(sb + L::q + (st * NK + x) * kBox, &p.tm_q, &m.full[st], 64 * x, u.hk, c * kC, u.b);
+          tma_load_4d(sb + L::k + (st * NK + x) * kBox, &p.tm_k, &m.full[st], 64 * x, u.hk, c * kC, u.b);
+        }
+        tma_load_4d(sb + L::va(st), &p.tm_v, &m.full[st], 0, u.head0, c * kC, u.b);
+        if (two)
+          tma_load_4d(sb + L::vb(st), &p.tm_v, &m.full[st], WIDE ? 64 : 0, WIDE ? u.head0 : u.head0 + 1, c * kC, u.b);
+        ++issued;
+      }
+      // No copy of this CTA may be in flight when it ends (also after a wait that gave up).
+      for (int i = max(0, issued - 2); i < issued; ++i) bad |= !mbar_wait(&m.full[i & 1], (i >> 1) & 1);
+    }
+    __syncwarp();
+  } else if (warp >= kEpiWarps) {
+    // ---- decays, weighted values, scores and state products ------------------------
+    const int pt = tid - 32 * kEpiWarps, pw = warp - kEpiWarps;
+    const bool scan = pw < u.nheads;  // this warp sums head pw's decays
+    const float* g = l.decay + u.b * l.sg[0] + (u.head0 + pw) * l.sg[1];
+    float g0 = 0.f, g1 = 0.f, seg_total = 0.f;
+    auto load_decays = [&](int c) {
+      const int64_t t = static_cast<int64_t>(c) * kC + 2 * lane;
+      g0 = t < u.len ? g[t * l.sg[2]] * kLog2e : 0.f;
+      g1 = t + 1 < u.len ? g[(t + 1) * l.sg[2]] * kLog2e : 0.f;
+    };
+    if (scan) load_decays(u.first);
+    for (int c = u.first; c < u.last; ++c) {
+      const int it = c - u.first, st = it & 1;
+      bad |= !mbar_wait(&m.full[st], (it >> 1) & 1);
+      const int live = static_cast<int>(min(u.len - static_cast<int64_t>(c) * kC, static_cast<int64_t>(kC)));
+      if (scan) {
+        const float x0 = g0 < kMinLog2 ? kMinLog2 : g0, x1 = g1 < kMinLog2 ? kMinLog2 : g1;  // NaN stays
+        if (c + 1 < u.last) load_decays(c + 1);
+        float f = x0 + x1, r = f;
+#pragma unroll
+        for (int o = 1; o < 32; o <<= 1) {
+          const float a = __shfl_up_sync(0xffffffffu, f, o), b = __shfl_down_sync(0xffffffffu, r, o);
+          if (lane >= o) f += a;
+          if (lane + o < 32) r += b;
+        }
+        // Before / after this pair, without subtracting large sums.
+        float before = __shfl_up_sync(0xffffffffu, f, 1), after = __shfl_down_sync(0xffffffffu, r, 1);
+        if (lane == 0) before = 0.f;
+        if (lane == 31) after = 0.f;
+        const float c0 = before + x0, c1 = c0 + x1;
+        m.cs[st][pw][2 * lane] = c0;
+        m.cs[st][pw][2 * lane + 1] = c1;
+        m.ecs[st][pw][2 * lane] = ex2_approx(c0);
+        m.ecs[st][pw][2 * lane + 1] = ex2_approx(c1);
+        m.w[st][pw][2 * lane] = 2 * lane < live ? ex2_approx(after + x1) : 0.f;
+        m.w[st][pw][2 * lane + 1] = 2 * lane + 1 < live ? ex2_approx(after) : 0.f;
+        if (lane == 0) m.total[st][pw] = ex2_approx(r);
+        seg_total += r;
+      }
+      if (live < kC) {
+        // Rows past the length hold anything: as operands they must be zero.
+        const int bytes = (kC - live) * 128;
+        const uint4 z = make_uint4(0, 0, 0, 0);
+        for (int i = pt; i < (NK + 2) * bytes / 16; i += 32 * kPrepWarps) {
+          const int box = i / (bytes / 16), at = i % (bytes / 16);
+          const uint32_t base = box < NK ? L::k + (st * NK + box) * kBox : box == NK ? L::va(st) : L::vb(st);
+          sts16(sb + base + live * 128 + 16 * at, z);
+        }
+        fence_async_smem();
+      }
+      // The weighted-value tiles are free once the previous chunk's state product has read them.
+      if (it > 0) bad |= !mbar_wait(&m.ds_full[(it - 1) & 1], ((it - 1) >> 1) & 1);
+      bad = bar_or(2, 32 * kPrepWarps, bad);
+      if (bad) break;
+      if (FULL && pt == 0) {
+        tc_fence_after();
+        const uint32_t qs = sb + L::q + st * NK * kBox, ks = sb + L::k + st * NK * kBox;
+#pragma unroll
+        for (int kk = 0; kk < 4 * NK; ++kk) {
+          const uint32_t off = (kk >> 2) * kBox + (kk & 3) * 32u;
+          umma_f16(tm + kColD + 64 * st, desc_sw128(qs + off, 0, 1024), desc_sw128(ks + off, 0, 1024),
+                   idesc_bf16(64, 64, false, false), kk > 0);
+        }
+        umma_commit(&m.d_full[st]);
+        mbar_arrive(&m.d_full[st]);
+      }
+      // Weighted values: each thread 16-byte vectors of one column group, rows pt / 8 + 16 i.
+      const int blocks = two ? 2 : 1;
+      for (int blk = 0; blk < blocks; ++blk) {
+        const uint32_t src = sb + (blk ? L::vb(st) : L::va(st));
+        const float* w = m.w[st][WIDE ? 0 : blk];
+#pragma unroll
+        for (int i = 0; i < kC / 16; ++i) {
+          const int row = (pt >> 3) + 16 * i;
+          const uint32_t off = row * 128u + ((pt & 7u) << 4);  // any vector of the row: same place in and out
+          const float wj = w[row];
+          const uint4 x = lds16(src + off);
+          const uint32_t in[4] = {x.x, x.y, x.z, x.w};
+          uint32_t hi[4], mid[4], lo[4];
+#pragma unroll
+          for (int j = 0; j < 4; ++j) {
+            const float2 f = unpack_bf16x2(in[j]);
+            float a = f.x * wj, b = f.y * wj;
+            hi[j] = take_bf16(a, b);
+            mid[j] = take_bf16(a, b);
+            lo[j] = pack_bf16x2(a, b);
+          }
+          const uint32_t dst = sb + L::wv + blk * kBox + off;
+          sts16(dst, make_uint4(hi[0], hi[1], hi[2], hi[3]));
+          sts16(dst + 2 * kBox, make_uint4(mid[0], mid[1], mid[2], mid[3]));
+          sts16(dst + 4 * kBox, make_uint4(lo[0], lo[1], lo[2], lo[3]));
+        }
+      }
+      fence_async_smem();
+      bar_or(2, 32 * kPrepWarps, false);
+      if (pt == 0) {
+        tc_fence_after();
+        const uint32_t ks = sb + L::k + st * NK * kBox;
+#pragma unroll
+        for (int part = 2; part >= 0; --part)  // the small parts first
+#pragma unroll
+          for (int kk = 0; kk < 4; ++kk)
+            umma_f16(tm + kColDS + 128 * st, desc_sw128(sb + L::wv + 2 * part * kBox + kk * 2048u, kBox, 1024),
+                     desc_sw128(ks + kk * 2048u, kBox, 1024), idesc_bf16(128, 64 * NK, true, true),
+                     part < 2 || kk > 0);
+        umma_commit(&m.ds_full[st]);
+        mbar_arrive(&m.ds_full[st]);
+      }
+    }
+    if (!FULL && scan && lane == 0 && !bad)
+      p.seg_decay[(static_cast<int64_t>(u.b) * l.H + u.head0 + pw) * p.segs + u.seg] = seg_total;
+  } else {
+    // ---- scores to weights, outputs, state --------------------------------------------
+    const int q4 = warp & 3, half = warp >> 2;
+    const int row = 32 * q4 + lane;              // accumulator lane
+    const int blk = row >> 6;                    // block of value columns
+    const int hd = WIDE ? 0 : blk;               // head of the CTA
+    const int col = WIDE ? row : row & 63;       // value column in the head
+    const bool on = col < l.P && (WIDE || blk < u.nheads);
+    const int head = u.head0 + hd;
+    constexpr int kNS = 32 * NK;                 // state values of a thread: columns half * kNS ..
+    const int64_t srow = static_cast<int64_t>(u.b) * l.H + head;
+    const uint32_t tl = (32u * q4) << 16;
+    float s[kNS];
+#pragma unroll
+    for (int i = 0; i < kNS; ++i) s[i] = 0.f;
+    if (FULL) {
+      const float* from = nullptr;
+      if (p.segs > 1)
+        from = p.seg_state + (srow * p.segs + u.seg) * l.N * l.P;
+      else if (l.state && !l.fresh)
+        from = l.state + slot * l.ss[0] + head * l.ss[1];
+      if (from && on) {
+#pragma unroll
+        for (int i = 0; i < kNS; ++i) {
+          const int n = half * kNS + i;
+          if (n < l.N) s[i] = from[n * l.P + col];
+        }
+      }
+    }
+    // The state as the BF16 operand of q S: row p, 64 columns n a tile.
+    auto put_state = [&]() {
+#pragma unroll
+      for (int i = 0; i < kNS; i += 8) {
+        const int n = half * kNS + i;
+        sts16(sb + L::s + (n >> 6) * 2 * kBox + sw128_offset(row, n & 63),
+              make_uint4(pack_bf16x2(s[i], s[i + 1]), pack_bf16x2(s[i + 2], s[i + 3]),
+                         pack_bf16x2(s[i + 4], s[i + 5]), pack_bf16x2(s[i + 6], s[i + 7])));
+      }
+      fence_async_smem();
+    };
+    if (FULL) {
+      put_state();
+      bar_or(1, 32 * kEpiWarps, false);
+    }
+    for (int c = u.first; c < u.last; ++c) {
+      const int it = c - u.first, st = it & 1, ph = (it >> 1) & 1;
+      const int live = static_cast<int>(min(u.len - static_cast<int64_t>(c) * kC, static_cast<int64_t>(kC)));
+      if (FULL) {
+        const uint32_t qs = sb + L::q + st * NK * kBox;
+        if (tid == 0) {
+          bad |= !mbar_wait(&m.full[st], ph);
+          tc_fence_after();
+          if (!bad)
+#pragma unroll
+            for (int kk = 0; kk < 4 * NK; ++kk)
+              umma_f16(tm + kColOI, desc_sw128(sb + L::s + (kk >> 2) * 2 * kBox + (kk & 3) * 32u, 0, 1024),
+                       desc_sw128(qs + (kk >> 2) * kBox + (kk & 3) * 32u, 0, 1024), idesc_bf16(128, 64, false, false),
+                       kk > 0);
+        }
+        __syncwarp();
+        bad |= !mbar_wait(&m.d_full[st], ph);
+        tc_fence_after();
+        {
+          // P = D e^{c_i - c_j} for j <= i: rows 16 q4 + lane / 4 (+ 8), columns 32 half + ...
+          float d[16];
+          tmem_ld_frag(tm + kColD + 64 * st + 32 * half + tl, d);
+          tmem_wait_ld();
+          const int i0 = 16 * q4 + (lane >> 2);
+          const int heads = WIDE ? 1 : u.nheads;
+          for (int x = 0; x < heads; ++x) {
+            const float r0 = m.cs[st][x][i0], r1 = m.cs[st][x][i0 + 8];
+#pragma unroll
+            for (int y = 0; y < 4; ++y) {
+              const int j = 32 * half + 8 * y + 2 * (lane & 3);
+              const float2 cj = *reinterpret_cast<const float2*>(&m.cs[st][x][j]);
+              const float e00 = j <= i0 ? d[4 * y] * ex2_approx(r0 - cj.x) : 0.f;
+              const float e01 = j + 1 <= i0 ? d[4 * y + 1] * ex2_approx(r0 - cj.y) : 0.f;
+              const float e10 = j <= i0 + 8 ? d[4 * y + 2] * ex2_approx(r1 - cj.x) : 0.f;
+              const float e11 = j + 1 <= i0 + 8 ? d[4 * y + 3] * ex2_approx(r1 - cj.y) : 0.f;
+              sts4(sb + L::p + x * kBox + sw128_offset(i0, j), pack_bf16x2(e00, e01));
+              sts4(sb + L::p + x * kBox + sw128_offset(i0 + 8, j), pack_bf16x2(e10, e11));
+            }
+          }
+        }
+        fence_async_smem();
+        tc_fence_before();
+        bad = bar_or(1, 32 * kEpiWarps, bad);
+        if (bad) break;
+        if (tid == 0) {
+          tc_fence_after();
+          const int heads = WIDE ? 1 : u.nheads;
+          for (int x = 0; x < heads; ++x) {
+            // Wide: both tiles of v. Head x of a pair: its tile and the zero tile, in the order of the blocks.
+            const uint32_t base = sb + (WIDE || x == 0 ? L::va(st) : L::v + 2 * kBox);
+            const uint32_t step = WIDE ? L::vb(st) - L::va(st) : (st ? 2 * kBox : kBox);
+#pragma unroll
+            for (int kk = 0; kk < 4; ++kk)
+              umma_f16(tm + kColOP, desc_sw128(base + kk * 2048u, step, 1024),
+                       desc_sw128(sb + L::p + x * kBox + kk * 32u, 0, 1024), idesc_bf16(128, 64, true, false),
+                       x > 0 || kk > 0);
+          }
+          umma_commit(&m.o_full);
+        }
+        __syncwarp();
+      }
+      // State after the chunk: S = e^{c_C} S + dS.
+      bad |= !mbar_wait(&m.ds_full[st], ph);
+      tc_fence_after();
+      const float a = m.total[st][hd];
+#pragma unroll
+      for (int i = 0; i < kNS; i += 16) {
+        float d[16];
+        tmem_ld16(tm + kColDS + 128 * st + half * kNS + i + tl, d);
+        tmem_wait_ld();
+#pragma unroll
+        for (int j = 0; j < 16; ++j) s[i + j] = fmaf(a, s[i + j], d[j]);
+      }
+      if (FULL) {
+        bad |= !mbar_wait(&m.o_full, it & 1);
+        tc_fence_after();
+        if (c + 1 < u.last) put_state();
+        bf16* o = static_cast<bf16*>(l.out) + u.b * l.so[0] + head * l.so[2] + col;
+#pragma unroll
+        for (int i = 0; i < 32; i += 16) {
+          float oi[16], op[16];
+          tmem_ld16(tm + kColOI + 32 * half + i + tl, oi);
+          tmem_ld16(tm + kColOP + 32 * half + i + tl, op);
+          tmem_wait_ld();
+#pragma unroll
+          for (int j = 0; j < 16; ++j) {
+            const int tt = 32 * half + i + j;
+            const int64_t t = static_cast<int64_t>(c) * kC + tt;
+            const float y = tt < live ? l.scale * fmaf(oi[j], m.ecs[st][hd][tt], op[j]) : 0.f;
+            if (on && t < l.T) o[t * l.so[1]] = __float2bfloat16_rn(y);
+          }
+        }
+        tc_fence_before();
+        bad = bar_or(1, 32 * kEpiWarps, bad);
+        if (bad) break;
+      } else {
+        tc_fence_before();
+        __syncwarp();
+        if (__any_sync(0xffffffffu, bad)) {
+          bad = true;
+          break;
+        }
+      }
+      if (lane == 0) mbar_arrive(&m.empty[st]);
+    }
+    if (on && !bad) {
+      float* to = nullptr;
+      if (!FULL)
+        to = p.seg_state + (srow * p.segs + u.seg + 1) * l.N * l.P;
+      else if (u.last == live_chunks && l.state)
+        to = l.state + slot * l.ss[0] + head * l.ss[1];
+      if (to)
+#pragma unroll
+        for (int i = 0; i < kNS; ++i) {
+          const int n = half * kNS + i;
+          if (n < l.N) to[n * l.P + col] = s[i];
+        }
+    }
+  }
+  tc_fence_before();
+  const bool any = __syncthreads_or(bad);
+  if (any && tid == 0) {
+    atomicExch(&g_linear_error, 1);
+    if (p.err_host) {
+      *reinterpret_cast<volatile int*>(p.err_host) = 1;
+      __threadfence_system();
+    }
+  }
+  if (warp == kEpiWarps + kPrepWarps) {
+    tc_fence_after();
+    tmem_dealloc(tm, 512);
+  }
+}
+
+// The state before every segment, from the segments' own states: S_in(0) = the carried
+// state, S_in(i + 1) = 2^decay(i) S_in(i) + own(i). Thread: four neighbouring values of
+// one head; own(i) lies where S_in(i + 1) goes.
+__global__ void __launch_bounds__(256) linear_join_kernel(const __grid_constant__ ChunkParams p) {
+  const LinearParams& l = p.l;
+  const int quads = l.N * l.P / 4;
+  const int64_t i = static_cast<int64_t>(blockIdx.x) * 256 + threadIdx.x;
+  if (i >= static_cast<int64_t>(l.B) * l.H * quads) return;
+  const int64_t row = i / quads;
+  const int e = static_cast<int>(i % quads) * 4;
+  const int b = static_cast<int>(row / l.H), h = static_cast<int>(row % l.H);
+  int64_t len = l.T;
+  if (l.lengths) len = min(max(l.lengths[b], static_cast<int64_t>(0)), len);
+  const int live = static_cast<int>((len + kC - 1) / kC);
+  const int segs = (live + p.seg_chunks - 1) / p.seg_chunks;
+  if (segs == 0) return;
+  float* own = p.seg_state + row * p.segs * l.N * l.P + e;
+  const int64_t step = static_cast<int64_t>(l.N) * l.P;
+  float4 s = make_float4(0.f, 0.f, 0.f, 0.f);
+  const int64_t slot = l.slots ? l.slots[b] : b;
+  if (!l.fresh && l.state && slot >= 0 && slot < l.nslots)
+    s = *reinterpret_cast<const float4*>(l.state + slot * l.ss[0] + h * l.ss[1] + e);
+  *reinterpret_cast<float4*>(own) = s;
+  for (int g = 1; g < segs; ++g) {
+    const float a = ex2_approx(p.seg_decay[row * p.segs + g - 1]);
+    const float4 d = *reinterpret_cast<const float4*>(own + g * step);
+    s.x = fmaf(a, s.x, d.x);
+    s.y = fmaf(a, s.y, d.y);
+    s.z = fmaf(a, s.z, d.z);
+    s.w = fmaf(a, s.w, d.w);
+    *reinterpret_cast<float4*>(own + g * step) = s;
+  }
+}
+
+// ---- host side ---------------------------------------------------------------------
+PFN_cuTensorMapEncodeTiled_v12000 g_encode = nullptr;
+int g_encode_looked = 0;
+
+bool encode_available() {
+  if (!g_encode_looked) {
+    void* fn = nullptr;
+    cudaDriverEntryPointQueryResult q{};
+    if (cudaGetDriverEntryPoint("cuTensorMapEncodeTiled", &fn, cudaEnableDefault, &q) == cudaSuccess &&
+        q == cudaDriverEntryPointSuccess)
+      g_encode = reinterpret_cast<PFN_cuTensorMapEncodeTiled_v12000>(fn);
+    else
+      (void)cudaGetLastError();
+    g_encode_looked = 1;
+  }
+  return g_encode != nullptr;
+}
+
+// [B, T, heads, width] BF16 rows as a map with boxes of 64 tokens x 64 columns of one head,
+// 128-byte swizzled; columns past the width and tokens past T read as zero.
+bool encode(CUtensorMap* map, const void* base, int width, int heads, int T, int B, const int64_t* s) {
+  const int64_t st[3] = {s[2], s[1], s[0]};
+  const int ext[3] = {heads, T, B};
+  const cuuint64_t dims[4] = {static_cast<cuuint64_t>(width), static_cast<cuuint64_t>(heads), static_cast<cuuint64_t>(T),
+                              static_cast<cuuint64_t>(B)};
+  cuuint64_t strides[3];
+  if (reinterpret_cast<uintptr_t>(base) % 16) return false;
+  for (int i = 0; i < 3; ++i) {
+    const int64_t bytes = ext[i] == 1 ? (width * 2 + 15) / 16 * 16 : st[i] * 2;  // a lone entry's stride is never used
+    if (bytes <= 0 || bytes % 16 || bytes >= (1ll << 40)) return false;
+    strides[i] = static_cast<cuuint64_t>(bytes);
+  }
+  const cuuint32_t box[4] = {64, 1, kC, 1}, one[4] = {1, 1, 1, 1};
+  return g_encode(map, CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, 4, const_cast<void*>(base), dims, strides, box, one,
+                  CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
+                  CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
+}
+
+struct Plan {
+  int pairs, chunks, segs, seg_chunks;
+  int64_t rows, state_bytes, bytes;
+};
+
+// A prompt shorter than this runs token by token.
+constexpr int kMinTokens = 32;
+
+bool plan_of(int B, int T, int H, int Hq, int N, int P, int dtype, Plan& x) {
+  if (dtype != TF_BF16 || N > 128 || P > 128 || T < kMinTokens) return false;
+  const int share = H / Hq;
+  x.pairs = P > 64 ? share : (share + 1) / 2;
+  x.chunks = (T + kC - 1) / kC;
+  x.rows = static_cast<int64_t>(B) * Hq * x.pairs;
+  x.segs = 1;
+  const int sms = sm_count();
+  if (x.rows * 2 <= sms) {
+    const int64_t most = sms / x.rows;
+    x.segs = static_cast<int>(min(most, static_cast<int64_t>((x.chunks + 3) / 4)));
+  }
+  x.seg_chunks = (x.chunks + x.segs - 1) / x.segs;
+  x.segs = (x.chunks + x.seg_chunks - 1) / x.seg_chunks;
+  x.state_bytes = x.segs > 1 ? static_cast<int64_t>(B) * H * x.segs * N * P * 4 : 0;
+  x.bytes = 256 + x.state_bytes + (x.segs > 1 ? static_cast<int64_t>(B) * H * x.segs * 4 : 0);
+  return true;
+}
+
+template <int NK, bool WIDE, bool FULL>
+void launch_chunks(const ChunkParams& p, unsigned grid, cudaStream_t stream) {
+  auto kernel = linear_chunk_kernel<NK, WIDE, FULL>;
+  constexpr int bytes = smem_bytes<NK>();
+  static std::atomic<uint64_t> ready{0};  // devices on which the kernel has its shared memory size
+  int dev = 0;
+  cudaGetDevice(&dev);
+  if (!(ready.load() >> dev & 1)) {
+    cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, bytes);
+    ready.fetch_or(1ull << dev);
+  }
+  kernel<<<grid, kThreads, bytes, stream>>>(p);
+}
+template <bool FULL>
+void launch_any(const ChunkParams& p, unsigned grid, cudaStream_t stream) {
+  if (p.l.N > 64) {
+    if (p.l.P > 64) launch_chunks<2, true, FULL>(p, grid, stream);
+    else launch_chunks<2, false, FULL>(p, grid, stream);
+  } else {
+    if (p.l.P > 64) launch_chunks<1, true, FULL>(p, grid, stream);
+    else launch_chunks<1, false, FULL>(p, grid, stream);
+  }
+}
+
+}  // namespace
+
+int64_t linear_chunk_workspace(int B, int T, int H, int Hq, int N, int P, int dtype) {
+  Plan x;
+  return plan_of(B, T, H, Hq, N, P, dtype, x) ? x.bytes : 0;
+}
+
+int launch_linear_chunks(const LinearParams& l, int dtype, void* workspace, int64_t workspace_bytes,
+                         cudaStream_t stream) {
+  Plan x;
+  if (!plan_of(l.B, l.T, l.H, l.Hq, l.N, l.P, dtype, x) || !encode_available()) return -1;
+  ChunkParams p{};
+  if (!encode(&p.tm_q, l.q, l.N, l.Hq, l.T, l.B, l.sq) || !encode(&p.tm_k, l.k, l.N, l.Hq, l.T, l.B, l.sk) ||
+      !encode(&p.tm_v, l.v, l.P, l.H, l.T, l.B, l.sv))
+    return -1;
+  if (x.rows * x.segs > 0x7fffffffll) return TF_ERR_SIZE;
+  if (!workspace || reinterpret_cast<uintptr_t>(workspace) % 256) return TF_ERR_ARG;
+  if (workspace_bytes < x.bytes) return TF_ERR_SIZE;
+  p.l = l;
+  p.pairs = x.pairs, p.chunks = x.chunks, p.segs = x.segs, p.seg_chunks = x.seg_chunks;
+  p.seg_state = static_cast<float*>(workspace);
+  p.seg_decay = reinterpret_cast<float*>(static_cast<char*>(workspace) + x.state_bytes);
+  p.err_host = host_error_word();
+  const unsigned grid = static_cast<unsigned>(x.rows * x.segs);
+  if (x.segs > 1) {
+    launch_any<false>(p, grid, stream);
+    const int64_t quads = static_cast<int64_t>(l.B) * l.H * l.N * l.P / 4;
+    linear_join_kernel<<<static_cast<unsigned>((quads + 255) / 256), 256, 0, stream>>>(p);
+  }
+  launch_any<true>(p, grid, stream);
+  return launch_status();
+}
+
+int read_linear_error(int reset) {
+  int v = 0;
+  cudaMemcpyFromSymbol(&v, g_linear_error, sizeof(int));
+  if (reset) {
+    const int zero = 0;
+    cudaMemcpyToSymbol(g_linear_error, &zero, sizeof(int));
+  }
+  return v;
+}
+
+}  // namespace tf

@@ -8,6 +8,7 @@
 #include <mutex>
 
 #include "../../include/trifusion_b200.h"
+#include "linear_attention.cuh"
 #include "recurrence.cuh"
 #include "tf_host.cuh"
 
@@ -256,7 +257,10 @@ int tf_version(void) { return 100; }
 
 const char* tf_last_cuda_error(void) { return tf::g_last_error; }
 
-int tf_device_error(int reset) { return tf::read_device_error(reset); }
+int tf_device_error(int reset) {
+  const int recurrence = tf::read_device_error(reset), linear = tf::read_linear_error(reset);
+  return recurrence ? recurrence : linear;
+}
 
 int tf_error_watch_init(void) {
   static std::mutex m;

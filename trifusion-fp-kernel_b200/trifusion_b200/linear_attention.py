@@ -61,6 +61,10 @@ def _check_state(op, state, slots, b, h, n, p):
         raise ValueError(f"{op}: slots must be int64 [B]")
 
 
+def _aligned(x):
+    return x.data_ptr() % 16 == 0 and all(e == 1 or (s > 0 and s % 8 == 0) for e, s in zip(x.shape[:3], x.stride()))
+
+
 def linear_attention(q, k, v, decay, state=None, *, slots=None, lengths=None, scale=None, out=None):
     """A piece of T tokens for each row: returns ``(out, state)``.
 
@@ -111,8 +115,13 @@ def linear_attention(q, k, v, decay, state=None, *, slots=None, lengths=None, sc
     fresh = state is None
     if fresh:
         state = torch.empty((b, h, n, p), dtype=torch.float32, device=dev)
-    nbytes = _lib.lib().tf_linear_attention_workspace_size(b, t, h, n, p, dtype)
-    work = torch.empty(nbytes, dtype=torch.uint8, device=dev) if nbytes else None
+    _lib.error_watch()
+    _lib.check_device_error()
+    nbytes = _lib.lib().tf_linear_attention_workspace_size(b, t, h, hq, n, p, dtype)
+    work = None
+    if nbytes:  # the chunked form, whose tile loads need 16-byte rows
+        q, k, v = (x if _aligned(x) else x.clone(memory_format=torch.contiguous_format) for x in (q, k, v))
+        work = torch.empty(nbytes, dtype=torch.uint8, device=dev)
     strides = _lib.int64_array((*q.stride()[:3], *k.stride()[:3], *v.stride()[:3], *decay.stride(),
                                 *out.stride()[:3], *state.stride()[:2]))
     _lib.launch("tf_linear_attention_fwd", dev, q.data_ptr(), k.data_ptr(), v.data_ptr(), dtype, decay.data_ptr(),
