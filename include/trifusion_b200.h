@@ -543,7 +543,7 @@ int tf_rotary_positions_fwd(const void* q, const void* k, void* q_out, void* k_o
  * head, time), out (batch, time, head), state (slot, head); innermost strides are 1
  * and the state is contiguous over [N,P]. `workspace` holds
  * tf_linear_attention_workspace_size bytes (256-byte aligned, contents irrelevant);
- * where that is not 0 the tokens run in chunks on the tensor cores if q, k and v lie on
+ * where that is not 0 the tokens run in chunks on the tensor cores if q, k, v and out lie on
  * 16-byte boundaries with strides that are multiples of 16 bytes, one by one otherwise. */
 int64_t tf_linear_attention_workspace_size(int batch, int seqlen, int heads, int groups, int key_dim, int value_dim,
                                            int dtype);

@@ -46,13 +46,15 @@ using namespace sm100;
 constexpr int kC = 64;                // tokens of a chunk
 constexpr int kBox = 8192;            // bytes of a 64 x 64 BF16 tile
 constexpr int kEpiWarps = 8, kPrepWarps = 4;
-constexpr int kThreads = 32 * (kEpiWarps + kPrepWarps + 1);
+constexpr int kLoadWarp = kEpiWarps + kPrepWarps, kMmaWarp = kLoadWarp + 1;
+constexpr int kThreads = 32 * (kMmaWarp + 1);
+constexpr int kSums = 4;              // chunks whose decay sums are kept
 constexpr float kMinLog2 = -256.f;    // a decay below it is zero in FP32 against any state
 
 __device__ int g_linear_error = 0;    // 1: a bounded wait gave up
 
 struct ChunkParams {
-  CUtensorMap tm_q, tm_k, tm_v;
+  CUtensorMap tm_q, tm_k, tm_v, tm_o;
   LinearParams l;
   int pairs;       // CTAs of a k head: pairs of its heads (P <= 64), or its heads
   int chunks;      // of T
@@ -74,25 +76,30 @@ struct Layout {
   static constexpr int wv = v + 5 * kBox;              // [part][block]
   static constexpr int s = wv + 6 * kBox;              // [NK] of 128 rows
   static constexpr int p = s + 2 * NK * kBox;          // [block]
-  static constexpr int misc = p + 2 * kBox;
+  static constexpr int o = p + 2 * kBox;               // [warp] 32 tokens x 32 columns
+  static constexpr int misc = o + kEpiWarps * 2048;
   static __device__ __forceinline__ uint32_t va(int stage) { return v + (stage ? 0 : 1) * kBox; }
   static __device__ __forceinline__ uint32_t vb(int stage) { return v + (stage ? 4 : 3) * kBox; }
 };
 struct alignas(16) Misc {
-  uint64_t full[2], empty[2], d_full[2], ds_full[2], o_full;
+  // Tiles loaded / free again; decay sums of a chunk there; scores there.
+  uint64_t full[2], empty[2], sums[2], d_full[2];
+  // Weighted values written, state product there, read; state operand written, P
+  // written, both output products there.
+  uint64_t wv_ready, ds_full, ds_free, s_ready, p_ready, o_full;
   uint32_t tmem;
-  alignas(16) float cs[2][2][kC];  // [stage][head] log2 decays summed from the chunk's start
-  float ecs[2][2][kC];   // 2^cs
-  float w[2][2][kC];     // 2^(sum after the token), 0 past the length
-  float total[2][2];     // 2^(sum of the chunk)
+  alignas(16) float cs[kSums][2][kC];  // [chunk][head] log2 decays summed from the chunk's start
+  float ecs[kSums][2][kC];   // 2^cs
+  float w[kSums][2][kC];     // 2^(sum after the token), 0 past the length
+  float total[kSums][2];     // 2^(sum of the chunk)
 };
 template <int NK>
 constexpr int smem_bytes() {
   return Layout<NK>::misc + static_cast<int>(sizeof(Misc)) + 1024;
 }
 
-// TMEM columns.
-constexpr uint32_t kColD = 0, kColOI = 128, kColOP = 192, kColDS = 256;
+// TMEM columns: D and the outputs twice, so that the next chunk's start before this one's are read.
+constexpr uint32_t kColD = 0, kColDS = 128, kColOI = 256, kColOP = 384;
 
 constexpr uint32_t idesc_bf16(int m, int n, bool a_mn, bool b_mn) {
   return idesc_f16_f32(m, n, a_mn, b_mn) | (1u << 7) | (1u << 10);
@@ -122,6 +129,20 @@ __device__ __forceinline__ void sts16(uint32_t a, uint4 v) {
 __device__ __forceinline__ void sts4(uint32_t a, uint32_t v) {
   asm volatile("st.shared.b32 [%0], %1;" ::"r"(a), "r"(v) : "memory");
 }
+// Four 8 x 8 fragments stored transposed: lane l gives the address of row l % 8 of matrix l / 8.
+__device__ __forceinline__ void stsm_x4_t(uint32_t a, uint32_t r0, uint32_t r1, uint32_t r2, uint32_t r3) {
+  asm volatile("stmatrix.sync.aligned.m8n8.x4.trans.shared.b16 [%0], {%1,%2,%3,%4};" ::"r"(a), "r"(r0), "r"(r1),
+               "r"(r2), "r"(r3)
+               : "memory");
+}
+__device__ __forceinline__ void tma_store_4d(const void* tmap, uint32_t src, int c0, int c1, int c2, int c3) {
+  asm volatile("cp.async.bulk.tensor.4d.global.shared::cta.tile.bulk_group [%0, {%1, %2, %3, %4}], [%5];" ::"l"(
+                   reinterpret_cast<uint64_t>(tmap)),
+               "r"(c0), "r"(c1), "r"(c2), "r"(c3), "r"(src)
+               : "memory");
+  asm volatile("cp.async.bulk.commit_group;" ::: "memory");
+}
+__device__ __forceinline__ void tma_store_wait_read() { asm volatile("cp.async.bulk.wait_group.read 0;" ::: "memory"); }
 // 16 TMEM lanes x 32 columns as m16n8 fragments: thread t gets lanes t/4 and t/4 + 8,
 // columns 8 x + 2 (t % 4) + {0, 1}, as r[4 x + 0..1] and r[4 x + 2..3].
 __device__ __forceinline__ void tmem_ld_frag(uint32_t taddr, float (&r)[16]) {
@@ -133,13 +154,13 @@ __device__ __forceinline__ void tmem_ld_frag(uint32_t taddr, float (&r)[16]) {
       : "r"(taddr)
       : "memory");
 }
-// x as BF16 pairs hi, and what is left of it.
+// The upper halves of a and b as a BF16 pair (their first 8 significant bits), taken off
+// both. Twice, then what is left has 8 bits or fewer: three pairs hold 24 bits exactly.
 __device__ __forceinline__ uint32_t take_bf16(float& a, float& b) {
-  const uint32_t h = pack_bf16x2(a, b);
-  const float2 f = unpack_bf16x2(h);
-  a -= f.x;
-  b -= f.y;
-  return h;
+  const uint32_t x = __float_as_uint(a), y = __float_as_uint(b);
+  a -= __uint_as_float(x & 0xffff0000u);
+  b -= __uint_as_float(y & 0xffff0000u);
+  return __byte_perm(x, y, 0x7632);
 }
 
 // What a CTA works on.
@@ -216,7 +237,7 @@ __global__ void __launch_bounds__(kThreads, 1) linear_chunk_kernel(const __grid_
 
   // ---- set-up ------------------------------------------------------------------
   const bool two = WIDE || u.nheads == 2;  // the second block of value columns is there
-  if (warp == kEpiWarps + kPrepWarps) {
+  if (warp == kLoadWarp) {
     tmem_alloc(&m.tmem, 512);
     tmem_relinquish();
   }
@@ -224,9 +245,14 @@ __global__ void __launch_bounds__(kThreads, 1) linear_chunk_kernel(const __grid_
     for (int i = 0; i < 2; ++i) {
       mbar_init(&m.full[i], 1);
       mbar_init(&m.empty[i], kEpiWarps);
-      mbar_init(&m.d_full[i], 2);   // the product's commit, and the thread that issued it (for the decay sums)
-      mbar_init(&m.ds_full[i], 2);
+      mbar_init(&m.sums[i], u.nheads);
+      mbar_init(&m.d_full[i], 1);
     }
+    mbar_init(&m.wv_ready, kPrepWarps);
+    mbar_init(&m.ds_full, 1);
+    mbar_init(&m.ds_free, kEpiWarps);
+    mbar_init(&m.s_ready, kEpiWarps);
+    mbar_init(&m.p_ready, kEpiWarps);
     mbar_init(&m.o_full, 1);
     fence_mbar_init();
   }
@@ -234,63 +260,137 @@ __global__ void __launch_bounds__(kThreads, 1) linear_chunk_kernel(const __grid_
   for (int i = tid; i < kBox / 16; i += kThreads) {
     const uint4 z = make_uint4(0, 0, 0, 0);
     sts16(sb + L::v + 2 * kBox + 16 * i, z);
-    if (!two) {
-      sts16(sb + L::vb(0) + 16 * i, z);
-      sts16(sb + L::vb(1) + 16 * i, z);
+    if (!two)
       for (int part = 0; part < 3; ++part) sts16(sb + L::wv + (2 * part + 1) * kBox + 16 * i, z);
-    }
   }
   fence_async_smem();
   tc_fence_before();
   __syncthreads();
   tc_fence_after();
   const uint32_t tm = m.tmem;
+  const int n_chunks = u.last - u.first;
   bool bad = false;  // a bounded wait gave up
 
-  if (warp == kEpiWarps + kPrepWarps) {
+  if (warp == kLoadWarp) {
     // ---- loads ------------------------------------------------------------------
     if (lane == 0) {
       const int boxes = (FULL ? 2 : 1) * NK + (two ? 2 : 1);
       int issued = 0;
-      for (int c = u.first; c < u.last; ++c) {
-        const int it = c - u.first, st = it & 1;
+      for (int it = 0; it < n_chunks; ++it) {
+        const int st = it & 1, t = (u.first + it) * kC;
         if (it >= 2 && !mbar_wait(&m.empty[st], ((it >> 1) - 1) & 1)) {
           bad = true;
           break;
         }
         mbar_arrive_expect_tx(&m.full[st], boxes * kBox);
         for (int x = 0; x < NK; ++x) {
-          if (FULL) tma_load_4d(sb + L::q + (st * NK + x) * kBox, &p.tm_q, &m.full[st], 64 * x, u.hk, c * kC, u.b);
-          tma_load_4d(sb + L::k + (st * NK + x) * kBox, &p.tm_k, &m.full[st], 64 * x, u.hk, c * kC, u.b);
+          tma_load_4d(sb + L::k + (st * NK + x) * kBox, &p.tm_k, &m.full[st], 64 * x, u.hk, t, u.b);
+          if (FULL) tma_load_4d(sb + L::q + (st * NK + x) * kBox, &p.tm_q, &m.full[st], 64 * x, u.hk, t, u.b);
         }
-        tma_load_4d(sb + L::va(st), &p.tm_v, &m.full[st], 0, u.head0, c * kC, u.b);
+        tma_load_4d(sb + L::va(st), &p.tm_v, &m.full[st], 0, u.head0, t, u.b);
         if (two)
-          tma_load_4d(sb + L::vb(st), &p.tm_v, &m.full[st], WIDE ? 64 : 0, WIDE ? u.head0 : u.head0 + 1, c * kC, u.b);
+          tma_load_4d(sb + L::vb(st), &p.tm_v, &m.full[st], WIDE ? 64 : 0, WIDE ? u.head0 : u.head0 + 1, t, u.b);
         ++issued;
       }
       // No copy of this CTA may be in flight when it ends (also after a wait that gave up).
       for (int i = max(0, issued - 2); i < issued; ++i) bad |= !mbar_wait(&m.full[i & 1], (i >> 1) & 1);
     }
     __syncwarp();
+  } else if (warp == kMmaWarp) {
+    // ---- products -----------------------------------------------------------------
+    if (lane == 0) {
+      auto scores = [&](int it) {  // D
+        const int st = it & 1;
+        if (!mbar_wait(&m.full[st], (it >> 1) & 1)) return false;
+        tc_fence_after();
+        const uint32_t qs = sb + L::q + st * NK * kBox, ks = sb + L::k + st * NK * kBox;
+#pragma unroll
+        for (int kk = 0; kk < 4 * NK; ++kk) {
+          const uint32_t off = (kk >> 2) * kBox + (kk & 3) * 32u;
+          umma_f16(tm + kColD + 64 * st, desc_sw128(qs + off, 0, 1024), desc_sw128(ks + off, 0, 1024),
+                   idesc_bf16(64, 64, false, false), kk > 0);
+        }
+        umma_commit(&m.d_full[st]);
+        return true;
+      };
+      auto state = [&](int it) {  // dS^T
+        const int st = it & 1;
+        if (!mbar_wait(&m.wv_ready, it & 1)) return false;
+        if (it > 0 && !mbar_wait(&m.ds_free, (it - 1) & 1)) return false;
+        tc_fence_after();
+        const uint32_t ks = sb + L::k + st * NK * kBox;
+#pragma unroll
+        for (int part = 2; part >= 0; --part)  // the small parts first
+#pragma unroll
+          for (int kk = 0; kk < 4; ++kk)
+            umma_f16(tm + kColDS, desc_sw128(sb + L::wv + 2 * part * kBox + kk * 2048u, kBox, 1024),
+                     desc_sw128(ks + kk * 2048u, kBox, 1024), idesc_bf16(128, 64 * NK, true, true),
+                     part < 2 || kk > 0);
+        umma_commit(&m.ds_full);
+        return true;
+      };
+      auto inter = [&](int it) {  // OI^T
+        const int st = it & 1;
+        if (!mbar_wait(&m.s_ready, it & 1)) return false;
+        tc_fence_after();
+        const uint32_t qs = sb + L::q + st * NK * kBox;
+#pragma unroll
+        for (int kk = 0; kk < 4 * NK; ++kk)
+          umma_f16(tm + kColOI + 64 * st, desc_sw128(sb + L::s + (kk >> 2) * 2 * kBox + (kk & 3) * 32u, 0, 1024),
+                   desc_sw128(qs + (kk >> 2) * kBox + (kk & 3) * 32u, 0, 1024), idesc_bf16(128, 64, false, false),
+                   kk > 0);
+        return true;
+      };
+      auto within = [&](int it) {  // OP^T
+        const int st = it & 1;
+        if (!mbar_wait(&m.p_ready, it & 1)) return false;
+        tc_fence_after();
+        const int heads = WIDE ? 1 : u.nheads;
+        for (int x = 0; x < heads; ++x) {
+          // Wide: both tiles of v. Head x of a pair: its tile and the zero tile, in the order of the blocks.
+          const uint32_t base = sb + (WIDE || x == 0 ? L::va(st) : L::v + 2 * kBox);
+          const uint32_t step = WIDE ? L::vb(st) - L::va(st) : (st ? 2 * kBox : kBox);
+#pragma unroll
+          for (int kk = 0; kk < 4; ++kk)
+            umma_f16(tm + kColOP + 64 * st, desc_sw128(base + kk * 2048u, step, 1024),
+                     desc_sw128(sb + L::p + x * kBox + kk * 32u, 0, 1024), idesc_bf16(128, 64, true, false),
+                     x > 0 || kk > 0);
+        }
+        umma_commit(&m.o_full);
+        return true;
+      };
+      // The next chunk's scores and state product need nothing of this one's state.
+      bool ok = (!FULL || scores(0)) && state(0);
+      for (int it = 0; it < n_chunks && ok; ++it) {
+        const bool more = it + 1 < n_chunks;
+        if (FULL) ok = inter(it) && (!more || scores(it + 1)) && within(it);
+        if (ok && more) ok = state(it + 1);
+      }
+      bad = !ok;
+    }
+    __syncwarp();
   } else if (warp >= kEpiWarps) {
-    // ---- decays, weighted values, scores and state products ------------------------
+    // ---- decay sums and weighted values ---------------------------------------------
     const int pt = tid - 32 * kEpiWarps, pw = warp - kEpiWarps;
     const bool scan = pw < u.nheads;  // this warp sums head pw's decays
-    const float* g = l.decay + u.b * l.sg[0] + (u.head0 + pw) * l.sg[1];
+    const float* g = l.decay + u.b * l.sg[0] + (u.head0 + (scan ? pw : 0)) * l.sg[1];
     float g0 = 0.f, g1 = 0.f, seg_total = 0.f;
-    auto load_decays = [&](int c) {
-      const int64_t t = static_cast<int64_t>(c) * kC + 2 * lane;
-      g0 = t < u.len ? g[t * l.sg[2]] * kLog2e : 0.f;
-      g1 = t + 1 < u.len ? g[(t + 1) * l.sg[2]] * kLog2e : 0.f;
+    auto load_decays = [&](int it) {
+      const int64_t t = static_cast<int64_t>(u.first + it) * kC + 2 * lane;
+      g0 = t < u.len ? g[t * l.sg[2]] : 0.f;
+      g1 = t + 1 < u.len ? g[(t + 1) * l.sg[2]] : 0.f;
     };
-    if (scan) load_decays(u.first);
-    for (int c = u.first; c < u.last; ++c) {
-      const int it = c - u.first, st = it & 1;
+    if (scan) load_decays(0);
+    for (int it = 0; it < n_chunks; ++it) {
+      const int st = it & 1, sl = it % kSums;
+      const int live =
+          static_cast<int>(min(u.len - static_cast<int64_t>(u.first + it) * kC, static_cast<int64_t>(kC)));
+      // Also keeps the sums of the chunk kSums back until they have been read.
       bad |= !mbar_wait(&m.full[st], (it >> 1) & 1);
-      const int live = static_cast<int>(min(u.len - static_cast<int64_t>(c) * kC, static_cast<int64_t>(kC)));
       if (scan) {
-        const float x0 = g0 < kMinLog2 ? kMinLog2 : g0, x1 = g1 < kMinLog2 ? kMinLog2 : g1;  // NaN stays
-        if (c + 1 < u.last) load_decays(c + 1);
+        float x0 = g0 * kLog2e, x1 = g1 * kLog2e;
+        x0 = x0 < kMinLog2 ? kMinLog2 : x0, x1 = x1 < kMinLog2 ? kMinLog2 : x1;  // NaN stays
+        if (it + 1 < n_chunks) load_decays(it + 1);
         float f = x0 + x1, r = f;
 #pragma unroll
         for (int o = 1; o < 32; o <<= 1) {
@@ -303,89 +403,65 @@ __global__ void __launch_bounds__(kThreads, 1) linear_chunk_kernel(const __grid_
         if (lane == 0) before = 0.f;
         if (lane == 31) after = 0.f;
         const float c0 = before + x0, c1 = c0 + x1;
-        m.cs[st][pw][2 * lane] = c0;
-        m.cs[st][pw][2 * lane + 1] = c1;
-        m.ecs[st][pw][2 * lane] = ex2_approx(c0);
-        m.ecs[st][pw][2 * lane + 1] = ex2_approx(c1);
-        m.w[st][pw][2 * lane] = 2 * lane < live ? ex2_approx(after + x1) : 0.f;
-        m.w[st][pw][2 * lane + 1] = 2 * lane + 1 < live ? ex2_approx(after) : 0.f;
-        if (lane == 0) m.total[st][pw] = ex2_approx(r);
+        *reinterpret_cast<float2*>(&m.cs[sl][pw][2 * lane]) = make_float2(c0, c1);
+        *reinterpret_cast<float2*>(&m.ecs[sl][pw][2 * lane]) = make_float2(ex2_approx(c0), ex2_approx(c1));
+        *reinterpret_cast<float2*>(&m.w[sl][pw][2 * lane]) =
+            make_float2(2 * lane < live ? ex2_approx(after + x1) : 0.f, 2 * lane + 1 < live ? ex2_approx(after) : 0.f);
+        if (lane == 0) m.total[sl][pw] = ex2_approx(r);
         seg_total += r;
+        __syncwarp();
+        if (lane == 0) mbar_arrive(&m.sums[st]);
       }
       if (live < kC) {
-        // Rows past the length hold anything: as operands they must be zero.
-        const int bytes = (kC - live) * 128;
+        // Rows past the length hold anything: as operands they must be zero. (The scores may
+        // read k before or after: those columns are masked.)
+        const int vecs = (kC - live) * 8;
         const uint4 z = make_uint4(0, 0, 0, 0);
-        for (int i = pt; i < (NK + 2) * bytes / 16; i += 32 * kPrepWarps) {
-          const int box = i / (bytes / 16), at = i % (bytes / 16);
+        for (int i = pt; i < (NK + (two ? 2 : 1)) * vecs; i += 32 * kPrepWarps) {
+          const int box = i / vecs, at = i % vecs;
           const uint32_t base = box < NK ? L::k + (st * NK + box) * kBox : box == NK ? L::va(st) : L::vb(st);
           sts16(sb + base + live * 128 + 16 * at, z);
         }
-        fence_async_smem();
       }
       // The weighted-value tiles are free once the previous chunk's state product has read them.
-      if (it > 0) bad |= !mbar_wait(&m.ds_full[(it - 1) & 1], ((it - 1) >> 1) & 1);
+      if (it > 0) bad |= !mbar_wait(&m.ds_full, (it - 1) & 1);
       bad = bar_or(2, 32 * kPrepWarps, bad);
       if (bad) break;
-      if (FULL && pt == 0) {
-        tc_fence_after();
-        const uint32_t qs = sb + L::q + st * NK * kBox, ks = sb + L::k + st * NK * kBox;
+      // Each thread one 16-byte vector of the rows pt / 8 + 16 i, in every block.
+      const uint32_t off0 = (pt >> 3) * 128u + ((pt & 7u) << 4);  // any vector of the row: same place in and out
 #pragma unroll
-        for (int kk = 0; kk < 4 * NK; ++kk) {
-          const uint32_t off = (kk >> 2) * kBox + (kk & 3) * 32u;
-          umma_f16(tm + kColD + 64 * st, desc_sw128(qs + off, 0, 1024), desc_sw128(ks + off, 0, 1024),
-                   idesc_bf16(64, 64, false, false), kk > 0);
-        }
-        umma_commit(&m.d_full[st]);
-        mbar_arrive(&m.d_full[st]);
-      }
-      // Weighted values: each thread 16-byte vectors of one column group, rows pt / 8 + 16 i.
-      const int blocks = two ? 2 : 1;
-      for (int blk = 0; blk < blocks; ++blk) {
-        const uint32_t src = sb + (blk ? L::vb(st) : L::va(st));
-        const float* w = m.w[st][WIDE ? 0 : blk];
+      for (int blk = 0; blk < 2; ++blk) {
+        if (blk == 1 && !two) break;
+        const uint32_t src = sb + (blk ? L::vb(st) : L::va(st)) + off0, dst = sb + L::wv + blk * kBox + off0;
+        const float* w = m.w[sl][WIDE ? 0 : blk] + (pt >> 3);
+        uint4 x[kC / 16];
+#pragma unroll
+        for (int i = 0; i < kC / 16; ++i) x[i] = lds16(src + i * 2048u);
 #pragma unroll
         for (int i = 0; i < kC / 16; ++i) {
-          const int row = (pt >> 3) + 16 * i;
-          const uint32_t off = row * 128u + ((pt & 7u) << 4);  // any vector of the row: same place in and out
-          const float wj = w[row];
-          const uint4 x = lds16(src + off);
-          const uint32_t in[4] = {x.x, x.y, x.z, x.w};
+          const float wj = w[16 * i];
+          const uint32_t in[4] = {x[i].x, x[i].y, x[i].z, x[i].w};
           uint32_t hi[4], mid[4], lo[4];
 #pragma unroll
           for (int j = 0; j < 4; ++j) {
-            const float2 f = unpack_bf16x2(in[j]);
-            float a = f.x * wj, b = f.y * wj;
+            float a = __uint_as_float(in[j] << 16) * wj, b = __uint_as_float(in[j] & 0xffff0000u) * wj;
             hi[j] = take_bf16(a, b);
             mid[j] = take_bf16(a, b);
-            lo[j] = pack_bf16x2(a, b);
+            lo[j] = __byte_perm(__float_as_uint(a), __float_as_uint(b), 0x7632);
           }
-          const uint32_t dst = sb + L::wv + blk * kBox + off;
-          sts16(dst, make_uint4(hi[0], hi[1], hi[2], hi[3]));
-          sts16(dst + 2 * kBox, make_uint4(mid[0], mid[1], mid[2], mid[3]));
-          sts16(dst + 4 * kBox, make_uint4(lo[0], lo[1], lo[2], lo[3]));
+          sts16(dst + i * 2048u, make_uint4(hi[0], hi[1], hi[2], hi[3]));
+          sts16(dst + i * 2048u + 2 * kBox, make_uint4(mid[0], mid[1], mid[2], mid[3]));
+          sts16(dst + i * 2048u + 4 * kBox, make_uint4(lo[0], lo[1], lo[2], lo[3]));
         }
       }
       fence_async_smem();
-      bar_or(2, 32 * kPrepWarps, false);
-      if (pt == 0) {
-        tc_fence_after();
-        const uint32_t ks = sb + L::k + st * NK * kBox;
-#pragma unroll
-        for (int part = 2; part >= 0; --part)  // the small parts first
-#pragma unroll
-          for (int kk = 0; kk < 4; ++kk)
-            umma_f16(tm + kColDS + 128 * st, desc_sw128(sb + L::wv + 2 * part * kBox + kk * 2048u, kBox, 1024),
-                     desc_sw128(ks + kk * 2048u, kBox, 1024), idesc_bf16(128, 64 * NK, true, true),
-                     part < 2 || kk > 0);
-        umma_commit(&m.ds_full[st]);
-        mbar_arrive(&m.ds_full[st]);
-      }
+      __syncwarp();
+      if (lane == 0) mbar_arrive(&m.wv_ready);
     }
     if (!FULL && scan && lane == 0 && !bad)
       p.seg_decay[(static_cast<int64_t>(u.b) * l.H + u.head0 + pw) * p.segs + u.seg] = seg_total;
   } else {
-    // ---- scores to weights, outputs, state --------------------------------------------
+    // ---- scores to weights, state, outputs --------------------------------------------
     const int q4 = warp & 3, half = warp >> 2;
     const int row = 32 * q4 + lane;              // accumulator lane
     const int blk = row >> 6;                    // block of value columns
@@ -423,116 +499,113 @@ __global__ void __launch_bounds__(kThreads, 1) linear_chunk_kernel(const __grid_
                          pack_bf16x2(s[i + 4], s[i + 5]), pack_bf16x2(s[i + 6], s[i + 7])));
       }
       fence_async_smem();
+      tc_fence_before();
+      __syncwarp();
+      if (lane == 0) mbar_arrive(&m.s_ready);
     };
-    if (FULL) {
-      put_state();
-      bar_or(1, 32 * kEpiWarps, false);
-    }
-    for (int c = u.first; c < u.last; ++c) {
-      const int it = c - u.first, st = it & 1, ph = (it >> 1) & 1;
-      const int live = static_cast<int>(min(u.len - static_cast<int64_t>(c) * kC, static_cast<int64_t>(kC)));
+    if (FULL) put_state();
+    // This warp's part of the output: 32 tokens x 32 columns, staged and stored by itself.
+    const uint32_t stage = sb + L::o + warp * 2048u;
+    const int ocol = WIDE ? 32 * q4 : 32 * (q4 & 1);
+    const bool stores = ocol < l.P && (WIDE || blk < u.nheads);
+    for (int it = 0; it < n_chunks; ++it) {
+      const int st = it & 1, ph = (it >> 1) & 1, sl = it % kSums;
+      const int t0 = (u.first + it) * kC;
+      bad |= !mbar_wait(&m.sums[st], ph);
       if (FULL) {
-        const uint32_t qs = sb + L::q + st * NK * kBox;
-        if (tid == 0) {
-          bad |= !mbar_wait(&m.full[st], ph);
-          tc_fence_after();
-          if (!bad)
-#pragma unroll
-            for (int kk = 0; kk < 4 * NK; ++kk)
-              umma_f16(tm + kColOI, desc_sw128(sb + L::s + (kk >> 2) * 2 * kBox + (kk & 3) * 32u, 0, 1024),
-                       desc_sw128(qs + (kk >> 2) * kBox + (kk & 3) * 32u, 0, 1024), idesc_bf16(128, 64, false, false),
-                       kk > 0);
-        }
-        __syncwarp();
+        // P = D e^{c_i - c_j} for j <= i: rows 16 q4 + lane / 4 (+ 8), columns 32 half + ...
         bad |= !mbar_wait(&m.d_full[st], ph);
         tc_fence_after();
-        {
-          // P = D e^{c_i - c_j} for j <= i: rows 16 q4 + lane / 4 (+ 8), columns 32 half + ...
-          float d[16];
-          tmem_ld_frag(tm + kColD + 64 * st + 32 * half + tl, d);
-          tmem_wait_ld();
-          const int i0 = 16 * q4 + (lane >> 2);
-          const int heads = WIDE ? 1 : u.nheads;
-          for (int x = 0; x < heads; ++x) {
-            const float r0 = m.cs[st][x][i0], r1 = m.cs[st][x][i0 + 8];
+        float d[16];
+        tmem_ld_frag(tm + kColD + 64 * st + 32 * half + tl, d);
+        tmem_wait_ld();
+        tc_fence_before();
+        const int i0 = 16 * q4 + (lane >> 2);
+        const int heads = WIDE ? 1 : u.nheads;
+        for (int x = 0; x < heads; ++x) {
+          const float r0 = m.cs[sl][x][i0], r1 = m.cs[sl][x][i0 + 8];
 #pragma unroll
-            for (int y = 0; y < 4; ++y) {
-              const int j = 32 * half + 8 * y + 2 * (lane & 3);
-              const float2 cj = *reinterpret_cast<const float2*>(&m.cs[st][x][j]);
-              const float e00 = j <= i0 ? d[4 * y] * ex2_approx(r0 - cj.x) : 0.f;
-              const float e01 = j + 1 <= i0 ? d[4 * y + 1] * ex2_approx(r0 - cj.y) : 0.f;
-              const float e10 = j <= i0 + 8 ? d[4 * y + 2] * ex2_approx(r1 - cj.x) : 0.f;
-              const float e11 = j + 1 <= i0 + 8 ? d[4 * y + 3] * ex2_approx(r1 - cj.y) : 0.f;
-              sts4(sb + L::p + x * kBox + sw128_offset(i0, j), pack_bf16x2(e00, e01));
-              sts4(sb + L::p + x * kBox + sw128_offset(i0 + 8, j), pack_bf16x2(e10, e11));
-            }
+          for (int y = 0; y < 4; ++y) {
+            const int j = 32 * half + 8 * y + 2 * (lane & 3);
+            const float2 cj = *reinterpret_cast<const float2*>(&m.cs[sl][x][j]);
+            const float e00 = j <= i0 ? d[4 * y] * ex2_approx(r0 - cj.x) : 0.f;
+            const float e01 = j + 1 <= i0 ? d[4 * y + 1] * ex2_approx(r0 - cj.y) : 0.f;
+            const float e10 = j <= i0 + 8 ? d[4 * y + 2] * ex2_approx(r1 - cj.x) : 0.f;
+            const float e11 = j + 1 <= i0 + 8 ? d[4 * y + 3] * ex2_approx(r1 - cj.y) : 0.f;
+            sts4(sb + L::p + x * kBox + sw128_offset(i0, j), pack_bf16x2(e00, e01));
+            sts4(sb + L::p + x * kBox + sw128_offset(i0 + 8, j), pack_bf16x2(e10, e11));
           }
         }
         fence_async_smem();
-        tc_fence_before();
-        bad = bar_or(1, 32 * kEpiWarps, bad);
-        if (bad) break;
-        if (tid == 0) {
-          tc_fence_after();
-          const int heads = WIDE ? 1 : u.nheads;
-          for (int x = 0; x < heads; ++x) {
-            // Wide: both tiles of v. Head x of a pair: its tile and the zero tile, in the order of the blocks.
-            const uint32_t base = sb + (WIDE || x == 0 ? L::va(st) : L::v + 2 * kBox);
-            const uint32_t step = WIDE ? L::vb(st) - L::va(st) : (st ? 2 * kBox : kBox);
-#pragma unroll
-            for (int kk = 0; kk < 4; ++kk)
-              umma_f16(tm + kColOP, desc_sw128(base + kk * 2048u, step, 1024),
-                       desc_sw128(sb + L::p + x * kBox + kk * 32u, 0, 1024), idesc_bf16(128, 64, true, false),
-                       x > 0 || kk > 0);
-          }
-          umma_commit(&m.o_full);
-        }
         __syncwarp();
+        if (lane == 0) mbar_arrive(&m.p_ready);
       }
       // State after the chunk: S = e^{c_C} S + dS.
-      bad |= !mbar_wait(&m.ds_full[st], ph);
+      bad |= !mbar_wait(&m.ds_full, it & 1);
       tc_fence_after();
-      const float a = m.total[st][hd];
+      const float a = m.total[sl][hd];
 #pragma unroll
       for (int i = 0; i < kNS; i += 16) {
         float d[16];
-        tmem_ld16(tm + kColDS + 128 * st + half * kNS + i + tl, d);
+        tmem_ld16(tm + kColDS + half * kNS + i + tl, d);
         tmem_wait_ld();
 #pragma unroll
         for (int j = 0; j < 16; ++j) s[i + j] = fmaf(a, s[i + j], d[j]);
       }
+      tc_fence_before();
+      __syncwarp();
+      if (lane == 0) mbar_arrive(&m.ds_free);
       if (FULL) {
         bad |= !mbar_wait(&m.o_full, it & 1);
         tc_fence_after();
-        if (c + 1 < u.last) put_state();
-        bf16* o = static_cast<bf16*>(l.out) + u.b * l.so[0] + head * l.so[2] + col;
+      }
+      if (__any_sync(0xffffffffu, bad)) {
+        bad = true;
+        break;
+      }
+      // Every product of the chunk is done: its tiles, the state operand and P are free.
+      if (lane == 0) mbar_arrive(&m.empty[st]);
+      if (FULL) {
+        if (it + 1 < n_chunks) put_state();
+        if (lane == 0) tma_store_wait_read();
+        __syncwarp();
+        float2 e[4];
 #pragma unroll
-        for (int i = 0; i < 32; i += 16) {
+        for (int y = 0; y < 4; ++y) {
+          const int tt = 32 * half + 8 * y + 2 * (lane & 3);
+          e[y] = *reinterpret_cast<const float2*>(&m.ecs[sl][hd][tt]);
+        }
+        const int left = static_cast<int>(min(u.len - t0, static_cast<int64_t>(kC))) - 32 * half - 2 * (lane & 3);
+#pragma unroll
+        for (int sub = 0; sub < 2; ++sub) {
           float oi[16], op[16];
-          tmem_ld16(tm + kColOI + 32 * half + i + tl, oi);
-          tmem_ld16(tm + kColOP + 32 * half + i + tl, op);
+          tmem_ld_frag(tm + kColOI + 64 * st + 32 * half + tl + (16u * sub << 16), oi);
+          tmem_ld_frag(tm + kColOP + 64 * st + 32 * half + tl + (16u * sub << 16), op);
           tmem_wait_ld();
+          uint32_t o[8];  // [column group y][row group]: tokens 8 y + 2 (lane % 4) + {0, 1}
 #pragma unroll
-          for (int j = 0; j < 16; ++j) {
-            const int tt = 32 * half + i + j;
-            const int64_t t = static_cast<int64_t>(c) * kC + tt;
-            const float y = tt < live ? l.scale * fmaf(oi[j], m.ecs[st][hd][tt], op[j]) : 0.f;
-            if (on && t < l.T) o[t * l.so[1]] = __float2bfloat16_rn(y);
+          for (int y = 0; y < 4; ++y)
+#pragma unroll
+            for (int r = 0; r < 2; ++r) {
+              const float v0 = l.scale * fmaf(oi[4 * y + 2 * r], e[y].x, op[4 * y + 2 * r]);
+              const float v1 = l.scale * fmaf(oi[4 * y + 2 * r + 1], e[y].y, op[4 * y + 2 * r + 1]);
+              o[2 * y + r] = pack_bf16x2(8 * y < left ? v0 : 0.f, 8 * y + 1 < left ? v1 : 0.f);
+            }
+#pragma unroll
+          for (int y = 0; y < 4; y += 2) {
+            const int tok = 8 * (y + (lane >> 4)) + (lane & 7), chunk = 2 * sub + ((lane >> 3) & 1);
+            stsm_x4_t(stage + tok * 64u + ((chunk ^ ((tok >> 1) & 3)) << 4), o[2 * y], o[2 * y + 1], o[2 * y + 2],
+                      o[2 * y + 3]);
           }
         }
-        tc_fence_before();
-        bad = bar_or(1, 32 * kEpiWarps, bad);
-        if (bad) break;
-      } else {
-        tc_fence_before();
+        fence_async_smem();
         __syncwarp();
-        if (__any_sync(0xffffffffu, bad)) {
-          bad = true;
-          break;
-        }
+        if (lane == 0 && stores && t0 + 32 * half < l.T)
+          tma_store_4d(&p.tm_o, stage, ocol, head, t0 + 32 * half, u.b);
       }
-      if (lane == 0) mbar_arrive(&m.empty[st]);
     }
+    if (FULL && lane == 0) tma_store_wait_read();
+    __syncwarp();
     if (on && !bad) {
       float* to = nullptr;
       if (!FULL)
@@ -556,7 +629,7 @@ __global__ void __launch_bounds__(kThreads, 1) linear_chunk_kernel(const __grid_
       __threadfence_system();
     }
   }
-  if (warp == kEpiWarps + kPrepWarps) {
+  if (warp == kLoadWarp) {
     tc_fence_after();
     tmem_dealloc(tm, 512);
   }
@@ -614,9 +687,11 @@ bool encode_available() {
   return g_encode != nullptr;
 }
 
-// [B, T, heads, width] BF16 rows as a map with boxes of 64 tokens x 64 columns of one head,
-// 128-byte swizzled; columns past the width and tokens past T read as zero.
-bool encode(CUtensorMap* map, const void* base, int width, int heads, int T, int B, const int64_t* s) {
+// [B, T, heads, width] BF16 rows as a map with boxes of `side` tokens x `side` columns of one
+// head, swizzled over a row of the box; columns past the width and tokens past T read as
+// zero and are not written.
+bool encode(CUtensorMap* map, const void* base, int width, int heads, int T, int B, const int64_t* s,
+            unsigned side = 64) {
   const int64_t st[3] = {s[2], s[1], s[0]};
   const int ext[3] = {heads, T, B};
   const cuuint64_t dims[4] = {static_cast<cuuint64_t>(width), static_cast<cuuint64_t>(heads), static_cast<cuuint64_t>(T),
@@ -628,9 +703,10 @@ bool encode(CUtensorMap* map, const void* base, int width, int heads, int T, int
     if (bytes <= 0 || bytes % 16 || bytes >= (1ll << 40)) return false;
     strides[i] = static_cast<cuuint64_t>(bytes);
   }
-  const cuuint32_t box[4] = {64, 1, kC, 1}, one[4] = {1, 1, 1, 1};
+  const cuuint32_t box[4] = {side, 1, side, 1}, one[4] = {1, 1, 1, 1};
   return g_encode(map, CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, 4, const_cast<void*>(base), dims, strides, box, one,
-                  CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
+                  CU_TENSOR_MAP_INTERLEAVE_NONE,
+                  side == 64 ? CU_TENSOR_MAP_SWIZZLE_128B : CU_TENSOR_MAP_SWIZZLE_64B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
                   CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
 }
 
@@ -698,7 +774,7 @@ int launch_linear_chunks(const LinearParams& l, int dtype, void* workspace, int6
   if (!plan_of(l.B, l.T, l.H, l.Hq, l.N, l.P, dtype, x) || !encode_available()) return -1;
   ChunkParams p{};
   if (!encode(&p.tm_q, l.q, l.N, l.Hq, l.T, l.B, l.sq) || !encode(&p.tm_k, l.k, l.N, l.Hq, l.T, l.B, l.sk) ||
-      !encode(&p.tm_v, l.v, l.P, l.H, l.T, l.B, l.sv))
+      !encode(&p.tm_v, l.v, l.P, l.H, l.T, l.B, l.sv) || !encode(&p.tm_o, l.out, l.P, l.H, l.T, l.B, l.so, 32))
     return -1;
   if (x.rows * x.segs > 0x7fffffffll) return TF_ERR_SIZE;
   if (!workspace || reinterpret_cast<uintptr_t>(workspace) % 256) return TF_ERR_ARG;

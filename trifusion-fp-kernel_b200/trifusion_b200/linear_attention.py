@@ -118,16 +118,20 @@ def linear_attention(q, k, v, decay, state=None, *, slots=None, lengths=None, sc
     _lib.error_watch()
     _lib.check_device_error()
     nbytes = _lib.lib().tf_linear_attention_workspace_size(b, t, h, hq, n, p, dtype)
-    work = None
+    work, into = None, out
     if nbytes:  # the chunked form, whose tile loads need 16-byte rows
         q, k, v = (x if _aligned(x) else x.clone(memory_format=torch.contiguous_format) for x in (q, k, v))
         work = torch.empty(nbytes, dtype=torch.uint8, device=dev)
+        if not _aligned(out):
+            into = torch.empty((b, t, h, p), dtype=v.dtype, device=dev)
     strides = _lib.int64_array((*q.stride()[:3], *k.stride()[:3], *v.stride()[:3], *decay.stride(),
-                                *out.stride()[:3], *state.stride()[:2]))
+                                *into.stride()[:3], *state.stride()[:2]))
     _lib.launch("tf_linear_attention_fwd", dev, q.data_ptr(), k.data_ptr(), v.data_ptr(), dtype, decay.data_ptr(),
                 state.data_ptr(), state.shape[0], fresh, None if slots is None else slots.data_ptr(),
-                None if lengths is None else lengths.data_ptr(), out.data_ptr(), strides, b, t, h, hq, n, p,
+                None if lengths is None else lengths.data_ptr(), into.data_ptr(), strides, b, t, h, hq, n, p,
                 n ** -0.5 if scale is None else float(scale), None if work is None else work.data_ptr(), nbytes)
+    if into is not out:
+        out.copy_(into)
     return out, state
 
 
