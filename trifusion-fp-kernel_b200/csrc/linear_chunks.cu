@@ -45,11 +45,17 @@ using namespace sm100;
 
 constexpr int kC = 64;                // tokens of a chunk
 constexpr int kBox = 8192;            // bytes of a 64 x 64 BF16 tile
-constexpr int kEpiWarps = 8, kPrepWarps = 4;
-constexpr int kLoadWarp = kEpiWarps + kPrepWarps, kMmaWarp = kLoadWarp + 1;
-constexpr int kThreads = 32 * (kMmaWarp + 1);
+constexpr int kStages = 3;            // chunks in shared memory
 constexpr int kSums = 4;              // chunks whose decay sums are kept
 constexpr float kMinLog2 = -256.f;    // a decay below it is zero in FP32 against any state
+
+// Warps, by what they do; groups of four have the four quarters of the TMEM lanes.
+constexpr int kStateWarps = 8, kPrepWarp = 8, kScoreWarp = 12, kOutWarp = 16;
+constexpr int kLoadWarp = 20, kMmaWarp = 21, kSumWarp = 22;
+constexpr int kThreads = 24 * 32;
+// Registers of a thread: 24 warps have 80 at launch, 1920 together, and share them out again
+// as 8 * 112 + 4 * (64 + 72 + 72 + 48) = 1920.
+constexpr int kStateRegs = 112, kPrepRegs = 64, kScoreRegs = 72, kOutRegs = 72, kMiscRegs = 48;
 
 __device__ int g_linear_error = 0;    // 1: a bounded wait gave up
 
@@ -65,41 +71,44 @@ struct ChunkParams {
   int* err_host;
 };
 
-// Shared memory, in bytes from a 1024-byte boundary. The values of stage 1 and 0 lie
-// around one zero tile: a block's tile and the zero tile are the two 64-column blocks
-// of the operand of its head's OP product.
+// Shared memory, in bytes from a 1024-byte boundary. The value tiles of the stages lie
+// around one zero tile, a2 a1 a0 zero b0 b1 b2: a block's tile and the zero tile are the two
+// 64-column blocks of the operand of its head's OP product.
 template <int NK>
 struct Layout {
-  static constexpr int q = 0;                          // [stage][NK]
-  static constexpr int k = q + 2 * NK * kBox;          // [stage][NK]
-  static constexpr int v = k + 2 * NK * kBox;          // a1 a0 zero b0 b1
-  static constexpr int wv = v + 5 * kBox;              // [part][block]
-  static constexpr int s = wv + 6 * kBox;              // [NK] of 128 rows
-  static constexpr int p = s + 2 * NK * kBox;          // [block]
-  static constexpr int o = p + 2 * kBox;               // [warp] 32 tokens x 32 columns
-  static constexpr int misc = o + kEpiWarps * 2048;
-  static __device__ __forceinline__ uint32_t va(int stage) { return v + (stage ? 0 : 1) * kBox; }
-  static __device__ __forceinline__ uint32_t vb(int stage) { return v + (stage ? 4 : 3) * kBox; }
+  static constexpr int q = 0;                               // [stage][NK]
+  static constexpr int k = q + kStages * NK * kBox;         // [stage][NK]
+  static constexpr int v = k + kStages * NK * kBox;
+  static constexpr int zero = v + kStages * kBox;
+  static constexpr int p = zero + (kStages + 1) * kBox;     // [chunk & 1][head]
+  static constexpr int o = p + 4 * kBox;                    // [warp][half] 32 tokens x 32 columns
+  static constexpr int misc = o + 8 * 2048;
+  static __device__ __forceinline__ uint32_t va(int stage) { return zero - (stage + 1) * kBox; }
+  static __device__ __forceinline__ uint32_t vb(int stage) { return zero + (stage + 1) * kBox; }
 };
 struct alignas(16) Misc {
-  // Tiles loaded / free again; decay sums of a chunk there; scores there.
-  uint64_t full[2], empty[2], sums[2], d_full[2];
-  // Weighted values written, state product there, read; state operand written, P
-  // written, both output products there.
-  uint64_t wv_ready, ds_full, ds_free, s_ready, p_ready, o_full;
+  uint64_t full[kStages], empty[kStages];    // tiles loaded / every product of them done
+  uint64_t sums[kSums], sums_free[kSums];    // decay sums written / read
+  uint64_t d_full, d_free;                   // scores there / read
+  uint64_t p_ready[2], o_full[2], o_free;    // P written, both output products there / read
+  uint64_t wv_ready, ds_full, ds_free;       // weighted values written, state product there / read
+  uint64_t s_ready, oi_full;                 // state operand written / read
   uint32_t tmem;
-  alignas(16) float cs[kSums][2][kC];  // [chunk][head] log2 decays summed from the chunk's start
-  float ecs[kSums][2][kC];   // 2^cs
-  float w[kSums][2][kC];     // 2^(sum after the token), 0 past the length
-  float total[kSums][2];     // 2^(sum of the chunk)
+  alignas(16) float row[kSums][2][kC];  // [chunk][head] two factors of scale e^{c_i - c_j}, or c_i and
+  float col[kSums][2][kC];              // -c_j (log2) where a factor would leave FP32's range
+  float ecs[kSums][2][kC];              // scale e^{c_i}
+  float w[kSums][2][kC];                // e^{c_C - c_j}, 0 past the length
+  float total[kSums][2];                // e^{c_C}
+  int factors[kSums][2];                // row and col hold factors
 };
 template <int NK>
 constexpr int smem_bytes() {
   return Layout<NK>::misc + static_cast<int>(sizeof(Misc)) + 1024;
 }
 
-// TMEM columns: D and the outputs twice, so that the next chunk's start before this one's are read.
-constexpr uint32_t kColD = 0, kColDS = 128, kColOI = 256, kColOP = 384;
+// TMEM columns. The weighted values (three parts of 64 tokens) and the state (BF16) are
+// operands there: as shared-memory tiles they would cost 160 KB of its traffic a chunk.
+constexpr uint32_t kColD = 0, kColDS = 64, kColOI = 192, kColOP = 256, kColWV = 320, kColS = 416;
 
 constexpr uint32_t idesc_bf16(int m, int n, bool a_mn, bool b_mn) {
   return idesc_f16_f32(m, n, a_mn, b_mn) | (1u << 7) | (1u << 10);
@@ -117,11 +126,6 @@ __device__ __forceinline__ bool bar_or(int id, int n, bool x) {
 }
 __device__ __forceinline__ void mbar_arrive(uint64_t* bar) {
   asm volatile("{\n .reg .b64 st;\n mbarrier.arrive.shared::cta.b64 st, [%0];\n}\n" ::"r"(smem_u32(bar)) : "memory");
-}
-__device__ __forceinline__ uint4 lds16(uint32_t a) {
-  uint4 v;
-  asm volatile("ld.shared.v4.b32 {%0,%1,%2,%3}, [%4];" : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w) : "r"(a));
-  return v;
 }
 __device__ __forceinline__ void sts16(uint32_t a, uint4 v) {
   asm volatile("st.shared.v4.b32 [%0], {%1,%2,%3,%4};" ::"r"(a), "r"(v.x), "r"(v.y), "r"(v.z), "r"(v.w) : "memory");
@@ -154,13 +158,75 @@ __device__ __forceinline__ void tmem_ld_frag(uint32_t taddr, float (&r)[16]) {
       : "r"(taddr)
       : "memory");
 }
-// The upper halves of a and b as a BF16 pair (their first 8 significant bits), taken off
-// both. Twice, then what is left has 8 bits or fewer: three pairs hold 24 bits exactly.
-__device__ __forceinline__ uint32_t take_bf16(float& a, float& b) {
-  const uint32_t x = __float_as_uint(a), y = __float_as_uint(b);
-  a -= __uint_as_float(x & 0xffff0000u);
-  b -= __uint_as_float(y & 0xffff0000u);
-  return __byte_perm(x, y, 0x7632);
+// 16 lanes x 8 columns: thread t gives lanes t/4 and t/4 + 8, column 4 x + t % 4, as r[2 x]
+// and r[2 x + 1].
+__device__ __forceinline__ void tmem_st_16x128_x2(uint32_t taddr, const uint32_t (&r)[4]) {
+  asm volatile("tcgen05.st.sync.aligned.16x128b.x2.b32 [%0], {%1,%2,%3,%4};" ::"r"(taddr), "r"(r[0]), "r"(r[1]),
+               "r"(r[2]), "r"(r[3])
+               : "memory");
+}
+// A lane's 16 consecutive columns.
+__device__ __forceinline__ void tmem_st16(uint32_t taddr, const uint32_t (&r)[16]) {
+  asm volatile(
+      "tcgen05.st.sync.aligned.32x32b.x16.b32 [%0], {%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,%16};" ::"r"(
+          taddr),
+      "r"(r[0]), "r"(r[1]), "r"(r[2]), "r"(r[3]), "r"(r[4]), "r"(r[5]), "r"(r[6]), "r"(r[7]), "r"(r[8]), "r"(r[9]),
+      "r"(r[10]), "r"(r[11]), "r"(r[12]), "r"(r[13]), "r"(r[14]), "r"(r[15])
+      : "memory");
+}
+__device__ __forceinline__ void tmem_wait_st() { asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory"); }
+// The two halves of a shared-memory descriptor (sm100.cuh's desc_sw128 with 8-row groups of
+// 1024 bytes): the upper one is the same for all, the lower one has address and lbo.
+__device__ __forceinline__ uint32_t desc_lo(uint32_t saddr, uint32_t lbo) { return (saddr >> 4) | (lbo >> 4 << 16); }
+__device__ __forceinline__ uint64_t desc_of(uint32_t lo) {
+  return static_cast<uint64_t>((1024u >> 4) | (1u << 14) | (2u << 29)) << 32 | lo;
+}
+// D[tmem] (+)= A[tmem] * B[smem].
+__device__ __forceinline__ void umma_ts(uint32_t d_tmem, uint32_t a_tmem, uint64_t b_desc, uint32_t idesc,
+                                        uint32_t accumulate) {
+  asm volatile(
+      "{\n .reg .pred p;\n setp.ne.b32 p, %4, 0;\n"
+      " tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, p;\n}\n" ::"r"(d_tmem),
+      "r"(a_tmem), "l"(b_desc), "r"(idesc), "r"(accumulate)
+      : "memory");
+}
+// One lane of a converged warp; the code around it stays uniform.
+__device__ __forceinline__ bool elect_one() {
+  uint32_t x;
+  asm volatile("{\n .reg .pred p;\n elect.sync _|p, 0xffffffff;\n selp.u32 %0, 1, 0, p;\n}\n" : "=r"(x));
+  return x != 0;
+}
+// Two FP32 products or differences in one instruction.
+__device__ __forceinline__ float2 mul2(float2 a, float2 b) {
+  float2 r;
+  asm("{\n .reg .b64 x, y, z;\n mov.b64 x, {%2, %3};\n mov.b64 y, {%4, %5};\n mul.rn.f32x2 z, x, y;\n"
+      " mov.b64 {%0, %1}, z;\n}\n"
+      : "=f"(r.x), "=f"(r.y)
+      : "f"(a.x), "f"(a.y), "f"(b.x), "f"(b.y));
+  return r;
+}
+__device__ __forceinline__ float2 fma2(float2 a, float2 b, float2 c) {
+  float2 r;
+  asm("{\n .reg .b64 x, y, z, w;\n mov.b64 x, {%2, %3};\n mov.b64 y, {%4, %5};\n mov.b64 w, {%6, %7};\n"
+      " fma.rn.f32x2 z, x, y, w;\n mov.b64 {%0, %1}, z;\n}\n"
+      : "=f"(r.x), "=f"(r.y)
+      : "f"(a.x), "f"(a.y), "f"(b.x), "f"(b.y), "f"(c.x), "f"(c.y));
+  return r;
+}
+template <int N>
+__device__ __forceinline__ void more_registers() {
+  asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(N));
+}
+template <int N>
+__device__ __forceinline__ void fewer_registers() {
+  asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(N));
+}
+// The upper halves of x (their first 8 significant bits) as a BF16 pair, taken off x. Twice,
+// then what is left has 8 bits or fewer: three pairs hold 24 bits exactly.
+__device__ __forceinline__ uint32_t take_bf16(float2& x) {
+  const uint32_t a = __float_as_uint(x.x), b = __float_as_uint(x.y);
+  x = fma2(make_float2(__uint_as_float(a & 0xffff0000u), __uint_as_float(b & 0xffff0000u)), make_float2(-1.f, -1.f), x);
+  return __byte_perm(a, b, 0x7632);
 }
 
 // What a CTA works on.
@@ -242,43 +308,53 @@ __global__ void __launch_bounds__(kThreads, 1) linear_chunk_kernel(const __grid_
     tmem_relinquish();
   }
   if (tid == 0) {
-    for (int i = 0; i < 2; ++i) {
+    for (int i = 0; i < kStages; ++i) {
       mbar_init(&m.full[i], 1);
-      mbar_init(&m.empty[i], kEpiWarps);
-      mbar_init(&m.sums[i], u.nheads);
-      mbar_init(&m.d_full[i], 1);
+      mbar_init(&m.empty[i], 1);
     }
-    mbar_init(&m.wv_ready, kPrepWarps);
+    for (int i = 0; i < kSums; ++i) {
+      mbar_init(&m.sums[i], u.nheads);
+      mbar_init(&m.sums_free[i], kStateWarps + (FULL ? 4 : 0));
+    }
+    for (int i = 0; i < 2; ++i) {
+      mbar_init(&m.p_ready[i], 4);
+      mbar_init(&m.o_full[i], 1);
+    }
+    mbar_init(&m.d_full, 1);
+    mbar_init(&m.d_free, 4);
+    mbar_init(&m.o_free, 4);
+    mbar_init(&m.wv_ready, 4);
     mbar_init(&m.ds_full, 1);
-    mbar_init(&m.ds_free, kEpiWarps);
-    mbar_init(&m.s_ready, kEpiWarps);
-    mbar_init(&m.p_ready, kEpiWarps);
-    mbar_init(&m.o_full, 1);
+    mbar_init(&m.ds_free, kStateWarps);
+    mbar_init(&m.s_ready, kStateWarps);
+    mbar_init(&m.oi_full, 1);
     fence_mbar_init();
   }
-  // The zero tile, and the second block's tiles where there is none.
-  for (int i = tid; i < kBox / 16; i += kThreads) {
-    const uint4 z = make_uint4(0, 0, 0, 0);
-    sts16(sb + L::v + 2 * kBox + 16 * i, z);
-    if (!two)
-      for (int part = 0; part < 3; ++part) sts16(sb + L::wv + (2 * part + 1) * kBox + 16 * i, z);
-  }
+  if (FULL && !WIDE)
+    for (int i = tid; i < kBox / 16; i += kThreads) sts16(sb + L::zero + 16 * i, make_uint4(0, 0, 0, 0));
   fence_async_smem();
   tc_fence_before();
   __syncthreads();
   tc_fence_after();
   const uint32_t tm = m.tmem;
   const int n_chunks = u.last - u.first;
+  const int q4 = warp & 3;                  // quarter of the TMEM lanes
+  const uint32_t tl = (32u * q4) << 16;
   bool bad = false;  // a bounded wait gave up
+  // Live tokens of a chunk.
+  auto live_of = [&](int it) {
+    return static_cast<int>(min(u.len - static_cast<int64_t>(u.first + it) * kC, static_cast<int64_t>(kC)));
+  };
 
-  if (warp == kLoadWarp) {
-    // ---- loads ------------------------------------------------------------------
-    if (lane == 0) {
+  if (warp >= kLoadWarp) {
+    fewer_registers<kMiscRegs>();
+    if (warp == kLoadWarp && lane == 0) {
+      // ---- loads ----------------------------------------------------------------
       const int boxes = (FULL ? 2 : 1) * NK + (two ? 2 : 1);
       int issued = 0;
       for (int it = 0; it < n_chunks; ++it) {
-        const int st = it & 1, t = (u.first + it) * kC;
-        if (it >= 2 && !mbar_wait(&m.empty[st], ((it >> 1) - 1) & 1)) {
+        const int st = it % kStages, t = (u.first + it) * kC;
+        if (it >= kStages && !mbar_wait(&m.empty[st], (it / kStages - 1) & 1)) {
           bad = true;
           break;
         }
@@ -293,101 +369,113 @@ __global__ void __launch_bounds__(kThreads, 1) linear_chunk_kernel(const __grid_
         ++issued;
       }
       // No copy of this CTA may be in flight when it ends (also after a wait that gave up).
-      for (int i = max(0, issued - 2); i < issued; ++i) bad |= !mbar_wait(&m.full[i & 1], (i >> 1) & 1);
-    }
-    __syncwarp();
-  } else if (warp == kMmaWarp) {
-    // ---- products -----------------------------------------------------------------
-    if (lane == 0) {
+      for (int i = max(0, issued - kStages); i < issued; ++i) bad |= !mbar_wait(&m.full[i % kStages], (i / kStages) & 1);
+    } else if (warp == kMmaWarp) {
+      // ---- products ---------------------------------------------------------------
+      // The whole warp runs this, one lane issues: addresses stay in uniform registers.
       auto scores = [&](int it) {  // D
-        const int st = it & 1;
-        if (!mbar_wait(&m.full[st], (it >> 1) & 1)) return false;
+        const int st = it % kStages;
+        if (!mbar_wait(&m.full[st], (it / kStages) & 1)) return false;
+        if (it > 0 && !mbar_wait(&m.d_free, (it - 1) & 1)) return false;
         tc_fence_after();
-        const uint32_t qs = sb + L::q + st * NK * kBox, ks = sb + L::k + st * NK * kBox;
+        const uint32_t qd = desc_lo(sb + L::q + st * NK * kBox, 0), kd = desc_lo(sb + L::k + st * NK * kBox, 0);
+        if (elect_one()) {
 #pragma unroll
-        for (int kk = 0; kk < 4 * NK; ++kk) {
-          const uint32_t off = (kk >> 2) * kBox + (kk & 3) * 32u;
-          umma_f16(tm + kColD + 64 * st, desc_sw128(qs + off, 0, 1024), desc_sw128(ks + off, 0, 1024),
-                   idesc_bf16(64, 64, false, false), kk > 0);
+          for (int kk = 0; kk < 4 * NK; ++kk) {
+            const uint32_t off = ((kk >> 2) * kBox + (kk & 3) * 32u) >> 4;
+            umma_f16(tm + kColD, desc_of(qd + off), desc_of(kd + off), idesc_bf16(64, 64, false, false), kk > 0);
+          }
+          umma_commit(&m.d_full);
         }
-        umma_commit(&m.d_full[st]);
+        __syncwarp();
         return true;
       };
       auto state = [&](int it) {  // dS^T
-        const int st = it & 1;
+        const int st = it % kStages;
         if (!mbar_wait(&m.wv_ready, it & 1)) return false;
         if (it > 0 && !mbar_wait(&m.ds_free, (it - 1) & 1)) return false;
         tc_fence_after();
-        const uint32_t ks = sb + L::k + st * NK * kBox;
+        const uint32_t kd = desc_lo(sb + L::k + st * NK * kBox, kBox);
+        if (elect_one()) {
 #pragma unroll
-        for (int part = 2; part >= 0; --part)  // the small parts first
+          for (int part = 2; part >= 0; --part)  // the small parts first
 #pragma unroll
-          for (int kk = 0; kk < 4; ++kk)
-            umma_f16(tm + kColDS, desc_sw128(sb + L::wv + 2 * part * kBox + kk * 2048u, kBox, 1024),
-                     desc_sw128(ks + kk * 2048u, kBox, 1024), idesc_bf16(128, 64 * NK, true, true),
-                     part < 2 || kk > 0);
-        umma_commit(&m.ds_full);
+            for (int kk = 0; kk < 4; ++kk)
+              umma_ts(tm + kColDS, tm + kColWV + 32 * part + 8 * kk, desc_of(kd + (kk * 2048u >> 4)),
+                      idesc_bf16(128, 64 * NK, false, true), part < 2 || kk > 0);
+          umma_commit(&m.ds_full);
+          if (!FULL) umma_commit(&m.empty[st]);
+        }
+        __syncwarp();
         return true;
       };
       auto inter = [&](int it) {  // OI^T
-        const int st = it & 1;
+        const int st = it % kStages;
         if (!mbar_wait(&m.s_ready, it & 1)) return false;
+        if (it > 0 && !mbar_wait(&m.o_free, (it - 1) & 1)) return false;
         tc_fence_after();
-        const uint32_t qs = sb + L::q + st * NK * kBox;
+        const uint32_t qd = desc_lo(sb + L::q + st * NK * kBox, 0);
+        if (elect_one()) {
 #pragma unroll
-        for (int kk = 0; kk < 4 * NK; ++kk)
-          umma_f16(tm + kColOI + 64 * st, desc_sw128(sb + L::s + (kk >> 2) * 2 * kBox + (kk & 3) * 32u, 0, 1024),
-                   desc_sw128(qs + (kk >> 2) * kBox + (kk & 3) * 32u, 0, 1024), idesc_bf16(128, 64, false, false),
-                   kk > 0);
+          for (int kk = 0; kk < 4 * NK; ++kk)
+            umma_ts(tm + kColOI, tm + kColS + 8 * kk, desc_of(qd + (((kk >> 2) * kBox + (kk & 3) * 32u) >> 4)),
+                    idesc_bf16(128, 64, false, false), kk > 0);
+          umma_commit(&m.oi_full);
+        }
+        __syncwarp();
         return true;
       };
       auto within = [&](int it) {  // OP^T
-        const int st = it & 1;
-        if (!mbar_wait(&m.p_ready, it & 1)) return false;
+        const int st = it % kStages;
+        if (!mbar_wait(&m.p_ready[it & 1], (it >> 1) & 1)) return false;
         tc_fence_after();
-        const int heads = WIDE ? 1 : u.nheads;
-        for (int x = 0; x < heads; ++x) {
-          // Wide: both tiles of v. Head x of a pair: its tile and the zero tile, in the order of the blocks.
-          const uint32_t base = sb + (WIDE || x == 0 ? L::va(st) : L::v + 2 * kBox);
-          const uint32_t step = WIDE ? L::vb(st) - L::va(st) : (st ? 2 * kBox : kBox);
+        // Wide: both tiles of v. Head x of a pair: its tile and the zero tile, in the order of the blocks.
+        const uint32_t step = (WIDE ? 2 : 1) * (st + 1) * kBox;
+        const uint32_t v0 = desc_lo(sb + L::va(st), step), v1 = desc_lo(sb + L::zero, step);
+        const uint32_t pd = desc_lo(sb + L::p + 2 * (it & 1) * kBox, 0);
+        if (elect_one()) {
 #pragma unroll
           for (int kk = 0; kk < 4; ++kk)
-            umma_f16(tm + kColOP + 64 * st, desc_sw128(base + kk * 2048u, step, 1024),
-                     desc_sw128(sb + L::p + x * kBox + kk * 32u, 0, 1024), idesc_bf16(128, 64, true, false),
-                     x > 0 || kk > 0);
+            umma_f16(tm + kColOP, desc_of(v0 + (kk * 2048u >> 4)), desc_of(pd + (kk * 32u >> 4)),
+                     idesc_bf16(128, 64, true, false), kk > 0);
+          if (!WIDE && u.nheads == 2) {
+#pragma unroll
+            for (int kk = 0; kk < 4; ++kk)
+              umma_f16(tm + kColOP, desc_of(v1 + (kk * 2048u >> 4)), desc_of(pd + ((kBox + kk * 32u) >> 4)),
+                       idesc_bf16(128, 64, true, false), 1);
+          }
+          umma_commit(&m.o_full[it & 1]);
+          umma_commit(&m.empty[st]);  // the last product of this chunk's tiles
         }
-        umma_commit(&m.o_full);
+        __syncwarp();
         return true;
       };
-      // The next chunk's scores and state product need nothing of this one's state.
-      bool ok = (!FULL || scores(0)) && state(0);
-      for (int it = 0; it < n_chunks && ok; ++it) {
+      // The next chunk's scores and state product need nothing of this one's state. One place
+      // for each product in the code: a body that is run from many places falls out of the
+      // instruction cache.
+      bool ok = true;
+#pragma unroll 1
+      for (int it = -1; it < n_chunks && ok; ++it) {
         const bool more = it + 1 < n_chunks;
-        if (FULL) ok = inter(it) && (!more || scores(it + 1)) && within(it);
+        if (FULL && it >= 0) ok = inter(it);
+        if (FULL && ok && more) ok = scores(it + 1);
+        if (FULL && ok && it >= 0) ok = within(it);
         if (ok && more) ok = state(it + 1);
       }
       bad = !ok;
-    }
-    __syncwarp();
-  } else if (warp >= kEpiWarps) {
-    // ---- decay sums and weighted values ---------------------------------------------
-    const int pt = tid - 32 * kEpiWarps, pw = warp - kEpiWarps;
-    const bool scan = pw < u.nheads;  // this warp sums head pw's decays
-    const float* g = l.decay + u.b * l.sg[0] + (u.head0 + (scan ? pw : 0)) * l.sg[1];
-    float g0 = 0.f, g1 = 0.f, seg_total = 0.f;
-    auto load_decays = [&](int it) {
-      const int64_t t = static_cast<int64_t>(u.first + it) * kC + 2 * lane;
-      g0 = t < u.len ? g[t * l.sg[2]] : 0.f;
-      g1 = t + 1 < u.len ? g[(t + 1) * l.sg[2]] : 0.f;
-    };
-    if (scan) load_decays(0);
-    for (int it = 0; it < n_chunks; ++it) {
-      const int st = it & 1, sl = it % kSums;
-      const int live =
-          static_cast<int>(min(u.len - static_cast<int64_t>(u.first + it) * kC, static_cast<int64_t>(kC)));
-      // Also keeps the sums of the chunk kSums back until they have been read.
-      bad |= !mbar_wait(&m.full[st], (it >> 1) & 1);
-      if (scan) {
+    } else if (warp >= kSumWarp && warp - kSumWarp < u.nheads) {
+      // ---- decay sums of one head ----------------------------------------------------
+      const int pw = warp - kSumWarp;
+      const float* g = l.decay + u.b * l.sg[0] + (u.head0 + pw) * l.sg[1];
+      float g0 = 0.f, g1 = 0.f, seg_total = 0.f;
+      auto load_decays = [&](int it) {
+        const int64_t t = static_cast<int64_t>(u.first + it) * kC + 2 * lane;
+        g0 = t < u.len ? g[t * l.sg[2]] : 0.f;
+        g1 = t + 1 < u.len ? g[(t + 1) * l.sg[2]] : 0.f;
+      };
+      load_decays(0);
+      for (int it = 0; it < n_chunks; ++it) {
+        const int sl = it % kSums, live = live_of(it);
         float x0 = g0 * kLog2e, x1 = g1 * kLog2e;
         x0 = x0 < kMinLog2 ? kMinLog2 : x0, x1 = x1 < kMinLog2 ? kMinLog2 : x1;  // NaN stays
         if (it + 1 < n_chunks) load_decays(it + 1);
@@ -403,75 +491,255 @@ __global__ void __launch_bounds__(kThreads, 1) linear_chunk_kernel(const __grid_
         if (lane == 0) before = 0.f;
         if (lane == 31) after = 0.f;
         const float c0 = before + x0, c1 = c0 + x1;
-        *reinterpret_cast<float2*>(&m.cs[sl][pw][2 * lane]) = make_float2(c0, c1);
-        *reinterpret_cast<float2*>(&m.ecs[sl][pw][2 * lane]) = make_float2(ex2_approx(c0), ex2_approx(c1));
-        *reinterpret_cast<float2*>(&m.w[sl][pw][2 * lane]) =
-            make_float2(2 * lane < live ? ex2_approx(after + x1) : 0.f, 2 * lane + 1 < live ? ex2_approx(after) : 0.f);
-        if (lane == 0) m.total[sl][pw] = ex2_approx(r);
+        const float hi = warp_max(fmaxf(c0, c1)), lo = -warp_max(-fminf(c0, c1));
+        // e^{c_i - c_j} as a product of two factors within 2^+-120 of 1, where c spans no more.
+        const bool factors = hi - lo <= 240.f;
+        const float mid = 0.5f * (hi + lo);
+        bad |= it >= kSums && !mbar_wait(&m.sums_free[sl], (it / kSums - 1) & 1);
+        if (__any_sync(0xffffffffu, bad)) {
+          bad = true;
+          break;
+        }
+        auto put = [&](float* to, float a, float b) { *reinterpret_cast<float2*>(to + 2 * lane) = make_float2(a, b); };
+        if (factors) {
+          put(m.row[sl][pw], l.scale * ex2_approx(c0 - mid), l.scale * ex2_approx(c1 - mid));
+          put(m.col[sl][pw], ex2_approx(mid - c0), ex2_approx(mid - c1));
+        } else {
+          put(m.row[sl][pw], c0, c1);
+          put(m.col[sl][pw], -c0, -c1);
+        }
+        put(m.ecs[sl][pw], l.scale * ex2_approx(c0), l.scale * ex2_approx(c1));
+        put(m.w[sl][pw], 2 * lane < live ? ex2_approx(after + x1) : 0.f, 2 * lane + 1 < live ? ex2_approx(after) : 0.f);
+        if (lane == 0) {
+          m.total[sl][pw] = ex2_approx(r);
+          m.factors[sl][pw] = factors;
+        }
         seg_total += r;
         __syncwarp();
-        if (lane == 0) mbar_arrive(&m.sums[st]);
+        if (lane == 0) mbar_arrive(&m.sums[sl]);
       }
+      if (!FULL && lane == 0 && !bad)
+        p.seg_decay[(static_cast<int64_t>(u.b) * l.H + u.head0 + pw) * p.segs + u.seg] = seg_total;
+    }
+    __syncwarp();
+  } else if (warp >= kOutWarp) {
+    // ---- outputs ------------------------------------------------------------------------
+    fewer_registers<kOutRegs>();
+    if (FULL) {
+      const int hd = WIDE ? 0 : q4 >> 1, head = u.head0 + hd;
+      const int ocol = WIDE ? 32 * q4 : 32 * (q4 & 1);
+      const bool stores = ocol < l.P && hd < u.nheads;
+      const uint32_t stage = sb + L::o + q4 * 4096u;  // 32 tokens x 32 columns, twice
+      for (int it = 0; it < n_chunks; ++it) {
+        const int sl = it % kSums, t0 = (u.first + it) * kC;
+        bad |= !mbar_wait(&m.sums[sl], (it / kSums) & 1);
+        bad |= !mbar_wait(&m.o_full[it & 1], (it >> 1) & 1);
+        tc_fence_after();
+        if (__any_sync(0xffffffffu, bad)) {
+          bad = true;
+          break;
+        }
+        if (lane == 0) tma_store_wait_read();
+        __syncwarp();
+        const float* ecs = &m.ecs[sl][hd < u.nheads ? hd : 0][2 * (lane & 3)];
+        const int live = live_of(it) - 2 * (lane & 3);
+#pragma unroll 1
+        for (int i = 0; i < 4; ++i) {  // 32 tokens (half) x 16 lanes (sub)
+          const int half = i >> 1, sub = i & 1;
+          float oi[16], op[16];
+          tmem_ld_frag(tm + kColOI + 32 * half + tl + (16u * sub << 16), oi);
+          tmem_ld_frag(tm + kColOP + 32 * half + tl + (16u * sub << 16), op);
+          float2 e[4];
+#pragma unroll
+          for (int y = 0; y < 4; ++y) e[y] = *reinterpret_cast<const float2*>(ecs + 32 * half + 8 * y);
+          tmem_wait_ld();
+          uint32_t o[8];  // [token group y][row group]: tokens 8 y + 2 (lane % 4) + {0, 1}
+#pragma unroll
+          for (int y = 0; y < 4; ++y)
+#pragma unroll
+            for (int r = 0; r < 2; ++r) {
+              const float2 x = fma2(make_float2(oi[4 * y + 2 * r], oi[4 * y + 2 * r + 1]), e[y],
+                                    make_float2(op[4 * y + 2 * r], op[4 * y + 2 * r + 1]));
+              o[2 * y + r] = pack_bf16x2(x.x, x.y);
+            }
+          if (live_of(it) < kC) {  // rows past the length
+#pragma unroll
+            for (int y = 0; y < 4; ++y) {
+              const int left = live - 32 * half - 8 * y;
+              const uint32_t keep = left > 1 ? 0xffffffffu : left > 0 ? 0xffffu : 0u;
+              o[2 * y] &= keep;
+              o[2 * y + 1] &= keep;
+            }
+          }
+          const uint32_t to = stage + 2048u * half + (lane >> 4) * 512u + (lane & 7) * 64u +
+                              (((2 * sub + ((lane >> 3) & 1)) ^ ((lane >> 1) & 3)) << 4);
+          stsm_x4_t(to, o[0], o[1], o[2], o[3]);
+          stsm_x4_t(to + 1024u, o[4], o[5], o[6], o[7]);
+        }
+        tc_fence_before();
+        __syncwarp();
+        if (lane == 0) mbar_arrive(&m.o_free);
+        fence_async_smem();
+        __syncwarp();
+        if (lane == 0) {
+          mbar_arrive(&m.sums_free[sl]);
+          if (stores) {
+            tma_store_4d(&p.tm_o, stage, ocol, head, t0, u.b);
+            if (t0 + 32 < l.T) tma_store_4d(&p.tm_o, stage + 2048u, ocol, head, t0 + 32, u.b);
+          }
+        }
+      }
+      if (lane == 0) tma_store_wait_read();
+      __syncwarp();
+    }
+  } else if (warp >= kScoreWarp) {
+    // ---- scores to weights: P = D e^{c_i - c_j} for j <= i ------------------------------
+    fewer_registers<kScoreRegs>();
+    if (FULL) {
+      const int i0 = 16 * q4 + (lane >> 2);  // rows i0 and i0 + 8; columns 32 half + 8 y + 2 (lane % 4) + {0, 1}
+      const int heads = WIDE ? 1 : u.nheads;
+      for (int it = 0; it < n_chunks; ++it) {
+        const int sl = it % kSums;
+        bad |= !mbar_wait(&m.sums[sl], (it / kSums) & 1);
+        bad |= it >= 2 && !mbar_wait(&m.o_full[it & 1], ((it >> 1) - 1) & 1);  // P's tiles have been read
+        bad |= !mbar_wait(&m.d_full, it & 1);
+        tc_fence_after();
+        if (__any_sync(0xffffffffu, bad)) {
+          bad = true;
+          break;
+        }
+#pragma unroll 1
+        for (int half = 0; half < 2; ++half) {
+          float d[16];
+          tmem_ld_frag(tm + kColD + 32 * half + tl, d);
+          tmem_wait_ld();
+          if (half == 1) {
+            tc_fence_before();
+            __syncwarp();
+            if (lane == 0) mbar_arrive(&m.d_free);
+          }
+          const int j0 = 32 * half + 2 * (lane & 3);
+#pragma unroll 1
+          for (int x = 0; x < heads; ++x) {
+            const float r0 = m.row[sl][x][i0], r1 = m.row[sl][x][i0 + 8];
+            const float* cj = m.col[sl][x] + j0;
+            float2 e[8];  // [column group y][row group]
+            if (m.factors[sl][x]) {
+#pragma unroll
+              for (int y = 0; y < 4; ++y) {
+                const float2 c = *reinterpret_cast<const float2*>(cj + 8 * y);
+                e[2 * y] = mul2(make_float2(r0, r0), c);
+                e[2 * y + 1] = mul2(make_float2(r1, r1), c);
+              }
+            } else {
+#pragma unroll
+              for (int y = 0; y < 4; ++y) {
+                const float2 c = *reinterpret_cast<const float2*>(cj + 8 * y);
+                e[2 * y] = make_float2(l.scale * ex2_approx(r0 + c.x), l.scale * ex2_approx(r0 + c.y));
+                e[2 * y + 1] = make_float2(l.scale * ex2_approx(r1 + c.x), l.scale * ex2_approx(r1 + c.y));
+              }
+            }
+            const uint32_t ps = sb + L::p + (2 * (it & 1) + x) * kBox + i0 * 128u;
+            uint32_t o[8];
+#pragma unroll
+            for (int y = 0; y < 4; ++y)
+#pragma unroll
+              for (int r = 0; r < 2; ++r) {
+                const float2 w = mul2(e[2 * y + r], make_float2(d[4 * y + 2 * r], d[4 * y + 2 * r + 1]));
+                const int left = i0 + 8 * r - j0 - 8 * y;  // columns j <= row: left >= 0, left >= 1
+                o[2 * y + r] = pack_bf16x2(left >= 0 ? w.x : 0.f, left >= 1 ? w.y : 0.f);
+              }
+#pragma unroll
+            for (int y = 0; y < 4; ++y) {
+              const uint32_t to = ps + (((4 * half + y) ^ (lane >> 2)) << 4) + 4 * (lane & 3);
+              sts4(to, o[2 * y]);
+              sts4(to + 1024u, o[2 * y + 1]);
+            }
+          }
+        }
+        fence_async_smem();
+        __syncwarp();
+        if (lane == 0) mbar_arrive(&m.p_ready[it & 1]);
+      }
+    }
+  } else if (warp >= kPrepWarp) {
+    // ---- weighted values, transposed into TMEM -------------------------------------------
+    fewer_registers<kPrepRegs>();
+    const int pt = tid - 32 * kPrepWarp;
+    const int blk = q4 >> 1;                       // block of value columns of this warp's lanes
+    const int hd = WIDE ? 0 : blk;
+    const bool mine = blk == 0 || two;
+    if (!mine) {  // lanes without values stay zero
+      const uint32_t z[16] = {};
+      for (int i = 0; i < 6; ++i) tmem_st16(tm + kColWV + 16 * i + tl, z);
+    }
+    for (int it = 0; it < n_chunks; ++it) {
+      const int st = it % kStages, sl = it % kSums, live = live_of(it);
+      bad |= !mbar_wait(&m.full[st], (it / kStages) & 1);
+      bad |= !mbar_wait(&m.sums[sl], (it / kSums) & 1);
       if (live < kC) {
         // Rows past the length hold anything: as operands they must be zero. (The scores may
         // read k before or after: those columns are masked.)
         const int vecs = (kC - live) * 8;
-        const uint4 z = make_uint4(0, 0, 0, 0);
-        for (int i = pt; i < (NK + (two ? 2 : 1)) * vecs; i += 32 * kPrepWarps) {
+        for (int i = pt; i < (NK + (two ? 2 : 1)) * vecs; i += 128) {
           const int box = i / vecs, at = i % vecs;
           const uint32_t base = box < NK ? L::k + (st * NK + box) * kBox : box == NK ? L::va(st) : L::vb(st);
-          sts16(sb + base + live * 128 + 16 * at, z);
+          sts16(sb + base + live * 128 + 16 * at, make_uint4(0, 0, 0, 0));
         }
+        fence_async_smem();
+        bad = bar_or(2, 128, bad);
       }
-      // The weighted-value tiles are free once the previous chunk's state product has read them.
+      if (__any_sync(0xffffffffu, bad)) {
+        bad = true;
+        break;
+      }
+      // The operand is free once the previous chunk's state product has read it.
       if (it > 0) bad |= !mbar_wait(&m.ds_full, (it - 1) & 1);
-      bad = bar_or(2, 32 * kPrepWarps, bad);
-      if (bad) break;
-      // Each thread one 16-byte vector of the rows pt / 8 + 16 i, in every block.
-      const uint32_t off0 = (pt >> 3) * 128u + ((pt & 7u) << 4);  // any vector of the row: same place in and out
-#pragma unroll
-      for (int blk = 0; blk < 2; ++blk) {
-        if (blk == 1 && !two) break;
-        const uint32_t src = sb + (blk ? L::vb(st) : L::va(st)) + off0, dst = sb + L::wv + blk * kBox + off0;
-        const float* w = m.w[sl][WIDE ? 0 : blk] + (pt >> 3);
-        uint4 x[kC / 16];
-#pragma unroll
-        for (int i = 0; i < kC / 16; ++i) x[i] = lds16(src + i * 2048u);
-#pragma unroll
-        for (int i = 0; i < kC / 16; ++i) {
-          const float wj = w[16 * i];
-          const uint32_t in[4] = {x[i].x, x[i].y, x[i].z, x[i].w};
-          uint32_t hi[4], mid[4], lo[4];
+      tc_fence_after();
+      if (mine) {
+        const float* w = &m.w[sl][hd][2 * (lane & 3)];
+        const uint32_t src = sb + (blk ? L::vb(st) : L::va(st)) + (lane >> 4) * 1024u + (lane & 7) * 128u;
+        const uint32_t chunk = (4 * (q4 & 1) + ((lane >> 3) & 1)) ^ (lane & 7);
+#pragma unroll 2
+        for (int i = 0; i < 8; ++i) {  // 16 lanes (sub) x 16 tokens
+          const int sub = i & 1, x = i >> 1;
+          uint32_t in[4], hi[4], mid[4], lo[4];
+          asm volatile("ldmatrix.sync.aligned.m8n8.x4.trans.shared.b16 {%0,%1,%2,%3}, [%4];"
+                       : "=r"(in[0]), "=r"(in[1]), "=r"(in[2]), "=r"(in[3])
+                       : "r"(src + x * 2048u + ((chunk ^ (2 * sub)) << 4))
+                       : "memory");
+          const float2 wj[2] = {*reinterpret_cast<const float2*>(w + 16 * x),
+                                *reinterpret_cast<const float2*>(w + 16 * x + 8)};
 #pragma unroll
           for (int j = 0; j < 4; ++j) {
-            float a = __uint_as_float(in[j] << 16) * wj, b = __uint_as_float(in[j] & 0xffff0000u) * wj;
-            hi[j] = take_bf16(a, b);
-            mid[j] = take_bf16(a, b);
-            lo[j] = __byte_perm(__float_as_uint(a), __float_as_uint(b), 0x7632);
+            float2 y = mul2(make_float2(__uint_as_float(in[j] << 16), __uint_as_float(in[j] & 0xffff0000u)), wj[j >> 1]);
+            hi[j] = take_bf16(y);
+            mid[j] = take_bf16(y);
+            lo[j] = __byte_perm(__float_as_uint(y.x), __float_as_uint(y.y), 0x7632);
           }
-          sts16(dst + i * 2048u, make_uint4(hi[0], hi[1], hi[2], hi[3]));
-          sts16(dst + i * 2048u + 2 * kBox, make_uint4(mid[0], mid[1], mid[2], mid[3]));
-          sts16(dst + i * 2048u + 4 * kBox, make_uint4(lo[0], lo[1], lo[2], lo[3]));
+          const uint32_t to = tm + kColWV + 8 * x + tl + (16u * sub << 16);
+          tmem_st_16x128_x2(to, hi);
+          tmem_st_16x128_x2(to + 32, mid);
+          tmem_st_16x128_x2(to + 64, lo);
         }
       }
-      fence_async_smem();
+      tmem_wait_st();
+      tc_fence_before();
       __syncwarp();
       if (lane == 0) mbar_arrive(&m.wv_ready);
     }
-    if (!FULL && scan && lane == 0 && !bad)
-      p.seg_decay[(static_cast<int64_t>(u.b) * l.H + u.head0 + pw) * p.segs + u.seg] = seg_total;
   } else {
-    // ---- scores to weights, state, outputs --------------------------------------------
-    const int q4 = warp & 3, half = warp >> 2;
+    // ---- state ------------------------------------------------------------------------------
+    more_registers<kStateRegs>();
+    const int half = warp >> 2;
     const int row = 32 * q4 + lane;              // accumulator lane
     const int blk = row >> 6;                    // block of value columns
     const int hd = WIDE ? 0 : blk;               // head of the CTA
     const int col = WIDE ? row : row & 63;       // value column in the head
-    const bool on = col < l.P && (WIDE || blk < u.nheads);
+    const bool on = col < l.P && hd < u.nheads;
     const int head = u.head0 + hd;
-    constexpr int kNS = 32 * NK;                 // state values of a thread: columns half * kNS ..
+    constexpr int kNS = 32 * NK;                 // state values of a thread: key columns half * kNS ..
     const int64_t srow = static_cast<int64_t>(u.b) * l.H + head;
-    const uint32_t tl = (32u * q4) << 16;
     float s[kNS];
 #pragma unroll
     for (int i = 0; i < kNS; ++i) s[i] = 0.f;
@@ -489,123 +757,61 @@ __global__ void __launch_bounds__(kThreads, 1) linear_chunk_kernel(const __grid_
         }
       }
     }
-    // The state as the BF16 operand of q S: row p, 64 columns n a tile.
+    // The state rounded to BF16, as the operand of q S.
     auto put_state = [&]() {
 #pragma unroll
-      for (int i = 0; i < kNS; i += 8) {
-        const int n = half * kNS + i;
-        sts16(sb + L::s + (n >> 6) * 2 * kBox + sw128_offset(row, n & 63),
-              make_uint4(pack_bf16x2(s[i], s[i + 1]), pack_bf16x2(s[i + 2], s[i + 3]),
-                         pack_bf16x2(s[i + 4], s[i + 5]), pack_bf16x2(s[i + 6], s[i + 7])));
+      for (int i = 0; i < kNS; i += 32) {
+        uint32_t r[16];
+#pragma unroll
+        for (int j = 0; j < 16; ++j) r[j] = pack_bf16x2(s[i + 2 * j], s[i + 2 * j + 1]);
+        tmem_st16(tm + kColS + (half * kNS + i) / 2 + tl, r);
       }
-      fence_async_smem();
+      tmem_wait_st();
       tc_fence_before();
       __syncwarp();
       if (lane == 0) mbar_arrive(&m.s_ready);
     };
     if (FULL) put_state();
-    // This warp's part of the output: 32 tokens x 32 columns, staged and stored by itself.
-    const uint32_t stage = sb + L::o + warp * 2048u;
-    const int ocol = WIDE ? 32 * q4 : 32 * (q4 & 1);
-    const bool stores = ocol < l.P && (WIDE || blk < u.nheads);
     for (int it = 0; it < n_chunks; ++it) {
-      const int st = it & 1, ph = (it >> 1) & 1, sl = it % kSums;
-      const int t0 = (u.first + it) * kC;
-      bad |= !mbar_wait(&m.sums[st], ph);
-      if (FULL) {
-        // P = D e^{c_i - c_j} for j <= i: rows 16 q4 + lane / 4 (+ 8), columns 32 half + ...
-        bad |= !mbar_wait(&m.d_full[st], ph);
-        tc_fence_after();
-        float d[16];
-        tmem_ld_frag(tm + kColD + 64 * st + 32 * half + tl, d);
-        tmem_wait_ld();
-        tc_fence_before();
-        const int i0 = 16 * q4 + (lane >> 2);
-        const int heads = WIDE ? 1 : u.nheads;
-        for (int x = 0; x < heads; ++x) {
-          const float r0 = m.cs[sl][x][i0], r1 = m.cs[sl][x][i0 + 8];
-#pragma unroll
-          for (int y = 0; y < 4; ++y) {
-            const int j = 32 * half + 8 * y + 2 * (lane & 3);
-            const float2 cj = *reinterpret_cast<const float2*>(&m.cs[sl][x][j]);
-            const float e00 = j <= i0 ? d[4 * y] * ex2_approx(r0 - cj.x) : 0.f;
-            const float e01 = j + 1 <= i0 ? d[4 * y + 1] * ex2_approx(r0 - cj.y) : 0.f;
-            const float e10 = j <= i0 + 8 ? d[4 * y + 2] * ex2_approx(r1 - cj.x) : 0.f;
-            const float e11 = j + 1 <= i0 + 8 ? d[4 * y + 3] * ex2_approx(r1 - cj.y) : 0.f;
-            sts4(sb + L::p + x * kBox + sw128_offset(i0, j), pack_bf16x2(e00, e01));
-            sts4(sb + L::p + x * kBox + sw128_offset(i0 + 8, j), pack_bf16x2(e10, e11));
-          }
-        }
-        fence_async_smem();
-        __syncwarp();
-        if (lane == 0) mbar_arrive(&m.p_ready);
-      }
-      // State after the chunk: S = e^{c_C} S + dS.
+      const int sl = it % kSums;
+      // S = e^{c_C} S + dS.
+      bad |= !mbar_wait(&m.sums[sl], (it / kSums) & 1);
       bad |= !mbar_wait(&m.ds_full, it & 1);
       tc_fence_after();
-      const float a = m.total[sl][hd];
-#pragma unroll
-      for (int i = 0; i < kNS; i += 16) {
-        float d[16];
-        tmem_ld16(tm + kColDS + half * kNS + i + tl, d);
-        tmem_wait_ld();
-#pragma unroll
-        for (int j = 0; j < 16; ++j) s[i + j] = fmaf(a, s[i + j], d[j]);
-      }
-      tc_fence_before();
-      __syncwarp();
-      if (lane == 0) mbar_arrive(&m.ds_free);
-      if (FULL) {
-        bad |= !mbar_wait(&m.o_full, it & 1);
-        tc_fence_after();
-      }
       if (__any_sync(0xffffffffu, bad)) {
         bad = true;
         break;
       }
-      // Every product of the chunk is done: its tiles, the state operand and P are free.
-      if (lane == 0) mbar_arrive(&m.empty[st]);
-      if (FULL) {
-        if (it + 1 < n_chunks) put_state();
-        if (lane == 0) tma_store_wait_read();
-        __syncwarp();
-        float2 e[4];
+      const float a = m.total[sl][hd < u.nheads ? hd : 0];
 #pragma unroll
-        for (int y = 0; y < 4; ++y) {
-          const int tt = 32 * half + 8 * y + 2 * (lane & 3);
-          e[y] = *reinterpret_cast<const float2*>(&m.ecs[sl][hd][tt]);
+      for (int i = 0; i < kNS; i += 32) {
+        float d[32];
+        tmem_ld16(tm + kColDS + half * kNS + i + tl, *reinterpret_cast<float(*)[16]>(d));
+        tmem_ld16(tm + kColDS + half * kNS + i + 16 + tl, *reinterpret_cast<float(*)[16]>(d + 16));
+        tmem_wait_ld();
+#pragma unroll
+        for (int j = 0; j < 32; j += 2) {
+          const float2 x = fma2(make_float2(a, a), make_float2(s[i + j], s[i + j + 1]), make_float2(d[j], d[j + 1]));
+          s[i + j] = x.x;
+          s[i + j + 1] = x.y;
         }
-        const int left = static_cast<int>(min(u.len - t0, static_cast<int64_t>(kC))) - 32 * half - 2 * (lane & 3);
-#pragma unroll
-        for (int sub = 0; sub < 2; ++sub) {
-          float oi[16], op[16];
-          tmem_ld_frag(tm + kColOI + 64 * st + 32 * half + tl + (16u * sub << 16), oi);
-          tmem_ld_frag(tm + kColOP + 64 * st + 32 * half + tl + (16u * sub << 16), op);
-          tmem_wait_ld();
-          uint32_t o[8];  // [column group y][row group]: tokens 8 y + 2 (lane % 4) + {0, 1}
-#pragma unroll
-          for (int y = 0; y < 4; ++y)
-#pragma unroll
-            for (int r = 0; r < 2; ++r) {
-              const float v0 = l.scale * fmaf(oi[4 * y + 2 * r], e[y].x, op[4 * y + 2 * r]);
-              const float v1 = l.scale * fmaf(oi[4 * y + 2 * r + 1], e[y].y, op[4 * y + 2 * r + 1]);
-              o[2 * y + r] = pack_bf16x2(8 * y < left ? v0 : 0.f, 8 * y + 1 < left ? v1 : 0.f);
-            }
-#pragma unroll
-          for (int y = 0; y < 4; y += 2) {
-            const int tok = 8 * (y + (lane >> 4)) + (lane & 7), chunk = 2 * sub + ((lane >> 3) & 1);
-            stsm_x4_t(stage + tok * 64u + ((chunk ^ ((tok >> 1) & 3)) << 4), o[2 * y], o[2 * y + 1], o[2 * y + 2],
-                      o[2 * y + 3]);
-          }
+      }
+      tc_fence_before();
+      __syncwarp();
+      if (lane == 0) {
+        mbar_arrive(&m.ds_free);
+        mbar_arrive(&m.sums_free[sl]);
+      }
+      if (FULL && it + 1 < n_chunks) {
+        bad |= !mbar_wait(&m.oi_full, it & 1);  // the operand has been read
+        tc_fence_after();
+        if (__any_sync(0xffffffffu, bad)) {
+          bad = true;
+          break;
         }
-        fence_async_smem();
-        __syncwarp();
-        if (lane == 0 && stores && t0 + 32 * half < l.T)
-          tma_store_4d(&p.tm_o, stage, ocol, head, t0 + 32 * half, u.b);
+        put_state();
       }
     }
-    if (FULL && lane == 0) tma_store_wait_read();
-    __syncwarp();
     if (on && !bad) {
       float* to = nullptr;
       if (!FULL)
