@@ -49,13 +49,14 @@ constexpr int kStages = 3;            // chunks in shared memory
 constexpr int kSums = 4;              // chunks whose decay sums are kept
 constexpr float kMinLog2 = -256.f;    // a decay below it is zero in FP32 against any state
 
-// Warps, by what they do; groups of four have the four quarters of the TMEM lanes.
-constexpr int kStateWarps = 8, kPrepWarp = 8, kScoreWarp = 12, kOutWarp = 16;
-constexpr int kLoadWarp = 20, kMmaWarp = 21, kSumWarp = 22;
-constexpr int kThreads = 24 * 32;
-// Registers of a thread: 24 warps have 80 at launch, 1920 together, and share them out again
-// as 8 * 112 + 4 * (64 + 72 + 72 + 48) = 1920.
-constexpr int kStateRegs = 112, kPrepRegs = 64, kScoreRegs = 72, kOutRegs = 72, kMiscRegs = 48;
+// Warps, by what they do; groups of four have the four quarters of the TMEM lanes, pairs of
+// groups the two halves of a chunk's tokens.
+constexpr int kPrepWarp = 4, kScoreWarp = 12, kOutWarp = 20;  // (state: 0)
+constexpr int kLoadWarp = 28, kSumWarp = 29, kStateMmaWarp = 30, kOutMmaWarp = 31;
+constexpr int kThreads = 32 * 32;
+// Registers of a thread: 32 warps have 64 at launch, 2048 together, and share them out again
+// as 4 * 160 + 8 * 56 + 20 * 48 = 2048.
+constexpr int kStateRegs = 160, kOutRegs = 56, kOtherRegs = 48;
 
 __device__ int g_linear_error = 0;    // 1: a bounded wait gave up
 
@@ -91,7 +92,8 @@ struct alignas(16) Misc {
   uint64_t sums[kSums], sums_free[kSums];    // decay sums written / read
   uint64_t d_full, d_free;                   // scores there / read
   uint64_t p_ready[2], o_full[2], o_free;    // P written, both output products there / read
-  uint64_t wv_ready, ds_full, ds_free;       // weighted values written, state product there / read
+  uint64_t wv_ready[2], wv_free[2];          // weighted values of half a chunk written / read
+  uint64_t ds_full, ds_free;                 // state product there / read
   uint64_t s_ready, oi_full;                 // state operand written / read
   uint32_t tmem;
   alignas(16) float row[kSums][2][kC];  // [chunk][head] two factors of scale e^{c_i - c_j}, or c_i and
@@ -175,6 +177,14 @@ __device__ __forceinline__ void tmem_st16(uint32_t taddr, const uint32_t (&r)[16
       : "memory");
 }
 __device__ __forceinline__ void tmem_wait_st() { asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory"); }
+// As tmem_ld_frag, 16 columns.
+__device__ __forceinline__ void tmem_ld_frag2(uint32_t taddr, float (&r)[8]) {
+  uint32_t* u = reinterpret_cast<uint32_t*>(r);
+  asm volatile("tcgen05.ld.sync.aligned.16x256b.x2.b32 {%0,%1,%2,%3,%4,%5,%6,%7}, [%8];"
+               : "=r"(u[0]), "=r"(u[1]), "=r"(u[2]), "=r"(u[3]), "=r"(u[4]), "=r"(u[5]), "=r"(u[6]), "=r"(u[7])
+               : "r"(taddr)
+               : "memory");
+}
 // The two halves of a shared-memory descriptor (sm100.cuh's desc_sw128 with 8-row groups of
 // 1024 bytes): the upper one is the same for all, the lower one has address and lbo.
 __device__ __forceinline__ uint32_t desc_lo(uint32_t saddr, uint32_t lbo) { return (saddr >> 4) | (lbo >> 4 << 16); }
@@ -310,23 +320,24 @@ __global__ void __launch_bounds__(kThreads, 1) linear_chunk_kernel(const __grid_
   if (tid == 0) {
     for (int i = 0; i < kStages; ++i) {
       mbar_init(&m.full[i], 1);
-      mbar_init(&m.empty[i], 1);
+      mbar_init(&m.empty[i], FULL ? 2 : 1);
     }
     for (int i = 0; i < kSums; ++i) {
-      mbar_init(&m.sums[i], u.nheads);
-      mbar_init(&m.sums_free[i], kStateWarps + (FULL ? 4 : 0));
+      mbar_init(&m.sums[i], 1);
+      mbar_init(&m.sums_free[i], FULL ? 12 : 4);
     }
     for (int i = 0; i < 2; ++i) {
-      mbar_init(&m.p_ready[i], 4);
+      mbar_init(&m.p_ready[i], 8);
       mbar_init(&m.o_full[i], 1);
+      mbar_init(&m.wv_ready[i], 4);
+      mbar_init(&m.wv_free[i], 1);
     }
     mbar_init(&m.d_full, 1);
-    mbar_init(&m.d_free, 4);
-    mbar_init(&m.o_free, 4);
-    mbar_init(&m.wv_ready, 4);
+    mbar_init(&m.d_free, 8);
+    mbar_init(&m.o_free, 8);
     mbar_init(&m.ds_full, 1);
-    mbar_init(&m.ds_free, kStateWarps);
-    mbar_init(&m.s_ready, kStateWarps);
+    mbar_init(&m.ds_free, 4);
+    mbar_init(&m.s_ready, 4);
     mbar_init(&m.oi_full, 1);
     fence_mbar_init();
   }
@@ -347,7 +358,7 @@ __global__ void __launch_bounds__(kThreads, 1) linear_chunk_kernel(const __grid_
   };
 
   if (warp >= kLoadWarp) {
-    fewer_registers<kMiscRegs>();
+    fewer_registers<kOtherRegs>();
     if (warp == kLoadWarp && lane == 0) {
       // ---- loads ----------------------------------------------------------------
       const int boxes = (FULL ? 2 : 1) * NK + (two ? 2 : 1);
@@ -370,9 +381,10 @@ __global__ void __launch_bounds__(kThreads, 1) linear_chunk_kernel(const __grid_
       }
       // No copy of this CTA may be in flight when it ends (also after a wait that gave up).
       for (int i = max(0, issued - kStages); i < issued; ++i) bad |= !mbar_wait(&m.full[i % kStages], (i / kStages) & 1);
-    } else if (warp == kMmaWarp) {
-      // ---- products ---------------------------------------------------------------
+    } else if (warp == kStateMmaWarp) {
+      // ---- products that need nothing of the state before --------------------------
       // The whole warp runs this, one lane issues: addresses stay in uniform registers.
+      // (Two warps for the products: with one, its waits and issue were the longest path.)
       auto scores = [&](int it) {  // D
         const int st = it % kStages;
         if (!mbar_wait(&m.full[st], (it / kStages) & 1)) return false;
@@ -392,25 +404,37 @@ __global__ void __launch_bounds__(kThreads, 1) linear_chunk_kernel(const __grid_
       };
       auto state = [&](int it) {  // dS^T
         const int st = it % kStages;
-        if (!mbar_wait(&m.wv_ready, it & 1)) return false;
-        if (it > 0 && !mbar_wait(&m.ds_free, (it - 1) & 1)) return false;
-        tc_fence_after();
         const uint32_t kd = desc_lo(sb + L::k + st * NK * kBox, kBox);
-        if (elect_one()) {
+        if (it > 0 && !mbar_wait(&m.ds_free, (it - 1) & 1)) return false;
+#pragma unroll 1
+        for (int half = 0; half < 2; ++half) {
+          if (!mbar_wait(&m.wv_ready[half], it & 1)) return false;
+          tc_fence_after();
+          if (elect_one()) {
 #pragma unroll
-          for (int part = 2; part >= 0; --part)  // the small parts first
+            for (int part = 2; part >= 0; --part)  // the small parts first
 #pragma unroll
-            for (int kk = 0; kk < 4; ++kk)
-              umma_ts(tm + kColDS, tm + kColWV + 32 * part + 8 * kk, desc_of(kd + (kk * 2048u >> 4)),
-                      idesc_bf16(128, 64 * NK, false, true), part < 2 || kk > 0);
-          umma_commit(&m.ds_full);
-          if (!FULL) umma_commit(&m.empty[st]);
+              for (int kk = 0; kk < 2; ++kk)
+                umma_ts(tm + kColDS, tm + kColWV + 32 * part + 16 * half + 8 * kk,
+                        desc_of(kd + (half * 4096u + kk * 2048u >> 4)), idesc_bf16(128, 64 * NK, false, true),
+                        half > 0 || part < 2 || kk > 0);
+            umma_commit(&m.wv_free[half]);
+            if (half == 1) umma_commit(&m.ds_full);
+            if (half == 1) umma_commit(&m.empty[st]);
+          }
+          __syncwarp();
         }
-        __syncwarp();
         return true;
       };
+      bool ok = true;
+#pragma unroll 1
+      for (int it = 0; it < n_chunks && ok; ++it) ok = (!FULL || scores(it)) && state(it);
+      bad = !ok;
+    } else if (FULL && warp == kOutMmaWarp) {
+      // ---- the output's products ------------------------------------------------------
       auto inter = [&](int it) {  // OI^T
         const int st = it % kStages;
+        if (!mbar_wait(&m.full[st], (it / kStages) & 1)) return false;
         if (!mbar_wait(&m.s_ready, it & 1)) return false;
         if (it > 0 && !mbar_wait(&m.o_free, (it - 1) & 1)) return false;
         tc_fence_after();
@@ -445,93 +469,89 @@ __global__ void __launch_bounds__(kThreads, 1) linear_chunk_kernel(const __grid_
                        idesc_bf16(128, 64, true, false), 1);
           }
           umma_commit(&m.o_full[it & 1]);
-          umma_commit(&m.empty[st]);  // the last product of this chunk's tiles
+          umma_commit(&m.empty[st]);
         }
         __syncwarp();
         return true;
       };
-      // The next chunk's scores and state product need nothing of this one's state. One place
-      // for each product in the code: a body that is run from many places falls out of the
-      // instruction cache.
       bool ok = true;
 #pragma unroll 1
-      for (int it = -1; it < n_chunks && ok; ++it) {
-        const bool more = it + 1 < n_chunks;
-        if (FULL && it >= 0) ok = inter(it);
-        if (FULL && ok && more) ok = scores(it + 1);
-        if (FULL && ok && it >= 0) ok = within(it);
-        if (ok && more) ok = state(it + 1);
-      }
+      for (int it = 0; it < n_chunks && ok; ++it) ok = inter(it) && within(it);
       bad = !ok;
-    } else if (warp >= kSumWarp && warp - kSumWarp < u.nheads) {
-      // ---- decay sums of one head ----------------------------------------------------
-      const int pw = warp - kSumWarp;
-      const float* g = l.decay + u.b * l.sg[0] + (u.head0 + pw) * l.sg[1];
-      float g0 = 0.f, g1 = 0.f, seg_total = 0.f;
+    } else if (warp == kSumWarp) {
+      // ---- decay sums -------------------------------------------------------------------
+      const float* g = l.decay + u.b * l.sg[0] + u.head0 * l.sg[1];
+      float g0[2] = {}, g1[2] = {}, seg_total[2] = {};
       auto load_decays = [&](int it) {
         const int64_t t = static_cast<int64_t>(u.first + it) * kC + 2 * lane;
-        g0 = t < u.len ? g[t * l.sg[2]] : 0.f;
-        g1 = t + 1 < u.len ? g[(t + 1) * l.sg[2]] : 0.f;
+#pragma unroll
+        for (int x = 0; x < (WIDE ? 1 : 2); ++x) {
+          g0[x] = x < u.nheads && t < u.len ? g[x * l.sg[1] + t * l.sg[2]] : 0.f;
+          g1[x] = x < u.nheads && t + 1 < u.len ? g[x * l.sg[1] + (t + 1) * l.sg[2]] : 0.f;
+        }
       };
       load_decays(0);
+#pragma unroll 1
       for (int it = 0; it < n_chunks; ++it) {
         const int sl = it % kSums, live = live_of(it);
-        float x0 = g0 * kLog2e, x1 = g1 * kLog2e;
-        x0 = x0 < kMinLog2 ? kMinLog2 : x0, x1 = x1 < kMinLog2 ? kMinLog2 : x1;  // NaN stays
+        float x0[2] = {g0[0], g0[1]}, x1[2] = {g1[0], g1[1]};
         if (it + 1 < n_chunks) load_decays(it + 1);
-        float f = x0 + x1, r = f;
-#pragma unroll
-        for (int o = 1; o < 32; o <<= 1) {
-          const float a = __shfl_up_sync(0xffffffffu, f, o), b = __shfl_down_sync(0xffffffffu, r, o);
-          if (lane >= o) f += a;
-          if (lane + o < 32) r += b;
-        }
-        // Before / after this pair, without subtracting large sums.
-        float before = __shfl_up_sync(0xffffffffu, f, 1), after = __shfl_down_sync(0xffffffffu, r, 1);
-        if (lane == 0) before = 0.f;
-        if (lane == 31) after = 0.f;
-        const float c0 = before + x0, c1 = c0 + x1;
-        const float hi = warp_max(fmaxf(c0, c1)), lo = -warp_max(-fminf(c0, c1));
-        // e^{c_i - c_j} as a product of two factors within 2^+-120 of 1, where c spans no more.
-        const bool factors = hi - lo <= 240.f;
-        const float mid = 0.5f * (hi + lo);
         bad |= it >= kSums && !mbar_wait(&m.sums_free[sl], (it / kSums - 1) & 1);
         if (__any_sync(0xffffffffu, bad)) {
           bad = true;
           break;
         }
-        auto put = [&](float* to, float a, float b) { *reinterpret_cast<float2*>(to + 2 * lane) = make_float2(a, b); };
-        if (factors) {
-          put(m.row[sl][pw], l.scale * ex2_approx(c0 - mid), l.scale * ex2_approx(c1 - mid));
-          put(m.col[sl][pw], ex2_approx(mid - c0), ex2_approx(mid - c1));
-        } else {
-          put(m.row[sl][pw], c0, c1);
-          put(m.col[sl][pw], -c0, -c1);
+#pragma unroll
+        for (int x = 0; x < (WIDE ? 1 : 2); ++x) {
+          if (x == u.nheads) break;
+          float a0 = x0[x] * kLog2e, a1 = x1[x] * kLog2e;
+          a0 = a0 < kMinLog2 ? kMinLog2 : a0, a1 = a1 < kMinLog2 ? kMinLog2 : a1;  // NaN stays
+          float f = a0 + a1, r = f;
+#pragma unroll
+          for (int o = 1; o < 32; o <<= 1) {
+            const float a = __shfl_up_sync(0xffffffffu, f, o), b = __shfl_down_sync(0xffffffffu, r, o);
+            if (lane >= o) f += a;
+            if (lane + o < 32) r += b;
+          }
+          // Before / after this pair, without subtracting large sums.
+          float before = __shfl_up_sync(0xffffffffu, f, 1), after = __shfl_down_sync(0xffffffffu, r, 1);
+          if (lane == 0) before = 0.f;
+          if (lane == 31) after = 0.f;
+          const float c0 = before + a0, c1 = c0 + a1;
+          const float hi = warp_max(fmaxf(c0, c1)), lo = -warp_max(-fminf(c0, c1));
+          // e^{c_i - c_j} as a product of two factors within 2^+-120 of 1, where c spans no more.
+          const bool factors = hi - lo <= 240.f;
+          const float mid = 0.5f * (hi + lo);
+          auto put = [&](float* to, float a, float b) { *reinterpret_cast<float2*>(to + 2 * lane) = make_float2(a, b); };
+          put(m.row[sl][x], factors ? l.scale * ex2_approx(c0 - mid) : c0, factors ? l.scale * ex2_approx(c1 - mid) : c1);
+          put(m.col[sl][x], factors ? ex2_approx(mid - c0) : -c0, factors ? ex2_approx(mid - c1) : -c1);
+          put(m.ecs[sl][x], l.scale * ex2_approx(c0), l.scale * ex2_approx(c1));
+          put(m.w[sl][x], 2 * lane < live ? ex2_approx(after + a1) : 0.f, 2 * lane + 1 < live ? ex2_approx(after) : 0.f);
+          if (lane == 0) {
+            m.total[sl][x] = ex2_approx(r);
+            m.factors[sl][x] = factors;
+          }
+          seg_total[x] += r;
         }
-        put(m.ecs[sl][pw], l.scale * ex2_approx(c0), l.scale * ex2_approx(c1));
-        put(m.w[sl][pw], 2 * lane < live ? ex2_approx(after + x1) : 0.f, 2 * lane + 1 < live ? ex2_approx(after) : 0.f);
-        if (lane == 0) {
-          m.total[sl][pw] = ex2_approx(r);
-          m.factors[sl][pw] = factors;
-        }
-        seg_total += r;
         __syncwarp();
         if (lane == 0) mbar_arrive(&m.sums[sl]);
       }
       if (!FULL && lane == 0 && !bad)
-        p.seg_decay[(static_cast<int64_t>(u.b) * l.H + u.head0 + pw) * p.segs + u.seg] = seg_total;
+        for (int x = 0; x < u.nheads; ++x)
+          p.seg_decay[(static_cast<int64_t>(u.b) * l.H + u.head0 + x) * p.segs + u.seg] = seg_total[x];
     }
     __syncwarp();
   } else if (warp >= kOutWarp) {
     // ---- outputs ------------------------------------------------------------------------
     fewer_registers<kOutRegs>();
     if (FULL) {
+      const int half = (warp - kOutWarp) >> 2;  // 32 tokens
       const int hd = WIDE ? 0 : q4 >> 1, head = u.head0 + hd;
       const int ocol = WIDE ? 32 * q4 : 32 * (q4 & 1);
       const bool stores = ocol < l.P && hd < u.nheads;
-      const uint32_t stage = sb + L::o + q4 * 4096u;  // 32 tokens x 32 columns, twice
+      const uint32_t stage = sb + L::o + (warp - kOutWarp) * 2048u;  // 32 tokens x 32 columns
       for (int it = 0; it < n_chunks; ++it) {
-        const int sl = it % kSums, t0 = (u.first + it) * kC;
+        const int sl = it % kSums, t0 = (u.first + it) * kC + 32 * half;
         bad |= !mbar_wait(&m.sums[sl], (it / kSums) & 1);
         bad |= !mbar_wait(&m.o_full[it & 1], (it >> 1) & 1);
         tc_fence_after();
@@ -541,52 +561,35 @@ __global__ void __launch_bounds__(kThreads, 1) linear_chunk_kernel(const __grid_
         }
         if (lane == 0) tma_store_wait_read();
         __syncwarp();
-        const float* ecs = &m.ecs[sl][hd < u.nheads ? hd : 0][2 * (lane & 3)];
-        const int live = live_of(it) - 2 * (lane & 3);
-#pragma unroll 1
-        for (int i = 0; i < 4; ++i) {  // 32 tokens (half) x 16 lanes (sub)
-          const int half = i >> 1, sub = i & 1;
-          float oi[16], op[16];
-          tmem_ld_frag(tm + kColOI + 32 * half + tl + (16u * sub << 16), oi);
-          tmem_ld_frag(tm + kColOP + 32 * half + tl + (16u * sub << 16), op);
-          float2 e[4];
-#pragma unroll
-          for (int y = 0; y < 4; ++y) e[y] = *reinterpret_cast<const float2*>(ecs + 32 * half + 8 * y);
+        const float* ecs = &m.ecs[sl][hd < u.nheads ? hd : 0][32 * half + 2 * (lane & 3)];
+        const int live = live_of(it) - 32 * half - 2 * (lane & 3);
+#pragma unroll 2
+        for (int i = 0; i < 4; ++i) {  // 16 lanes (sub) x 16 tokens
+          const int x = i >> 1, sub = i & 1;
+          float oi[8], op[8];
+          tmem_ld_frag2(tm + kColOI + 32 * half + 16 * x + tl + (16u * sub << 16), oi);
+          tmem_ld_frag2(tm + kColOP + 32 * half + 16 * x + tl + (16u * sub << 16), op);
+          const float2 e[2] = {*reinterpret_cast<const float2*>(ecs + 16 * x),
+                               *reinterpret_cast<const float2*>(ecs + 16 * x + 8)};
           tmem_wait_ld();
-          uint32_t o[8];  // [token group y][row group]: tokens 8 y + 2 (lane % 4) + {0, 1}
+          uint32_t o[4];  // [token group y][row group]: tokens 8 y + 2 (lane % 4) + {0, 1}
 #pragma unroll
-          for (int y = 0; y < 4; ++y)
-#pragma unroll
-            for (int r = 0; r < 2; ++r) {
-              const float2 x = fma2(make_float2(oi[4 * y + 2 * r], oi[4 * y + 2 * r + 1]), e[y],
-                                    make_float2(op[4 * y + 2 * r], op[4 * y + 2 * r + 1]));
-              o[2 * y + r] = pack_bf16x2(x.x, x.y);
-            }
-          if (live_of(it) < kC) {  // rows past the length
-#pragma unroll
-            for (int y = 0; y < 4; ++y) {
-              const int left = live - 32 * half - 8 * y;
-              const uint32_t keep = left > 1 ? 0xffffffffu : left > 0 ? 0xffffu : 0u;
-              o[2 * y] &= keep;
-              o[2 * y + 1] &= keep;
-            }
+          for (int j = 0; j < 4; ++j) {
+            const float2 y = fma2(make_float2(oi[2 * j], oi[2 * j + 1]), e[j >> 1], make_float2(op[2 * j], op[2 * j + 1]));
+            const int left = live - 16 * x - 8 * (j >> 1);  // rows past the length are zero
+            o[j] = pack_bf16x2(y.x, y.y) & (left > 1 ? 0xffffffffu : left > 0 ? 0xffffu : 0u);
           }
-          const uint32_t to = stage + 2048u * half + (lane >> 4) * 512u + (lane & 7) * 64u +
-                              (((2 * sub + ((lane >> 3) & 1)) ^ ((lane >> 1) & 3)) << 4);
-          stsm_x4_t(to, o[0], o[1], o[2], o[3]);
-          stsm_x4_t(to + 1024u, o[4], o[5], o[6], o[7]);
+          stsm_x4_t(stage + x * 1024u + (lane >> 4) * 512u + (lane & 7) * 64u +
+                        (((2 * sub + ((lane >> 3) & 1)) ^ ((lane >> 1) & 3)) << 4),
+                    o[0], o[1], o[2], o[3]);
         }
         tc_fence_before();
-        __syncwarp();
-        if (lane == 0) mbar_arrive(&m.o_free);
         fence_async_smem();
         __syncwarp();
         if (lane == 0) {
+          mbar_arrive(&m.o_free);
           mbar_arrive(&m.sums_free[sl]);
-          if (stores) {
-            tma_store_4d(&p.tm_o, stage, ocol, head, t0, u.b);
-            if (t0 + 32 < l.T) tma_store_4d(&p.tm_o, stage + 2048u, ocol, head, t0 + 32, u.b);
-          }
+          if (stores && t0 < l.T) tma_store_4d(&p.tm_o, stage, ocol, head, t0, u.b);
         }
       }
       if (lane == 0) tma_store_wait_read();
@@ -594,9 +597,11 @@ __global__ void __launch_bounds__(kThreads, 1) linear_chunk_kernel(const __grid_
     }
   } else if (warp >= kScoreWarp) {
     // ---- scores to weights: P = D e^{c_i - c_j} for j <= i ------------------------------
-    fewer_registers<kScoreRegs>();
+    fewer_registers<kOtherRegs>();
     if (FULL) {
-      const int i0 = 16 * q4 + (lane >> 2);  // rows i0 and i0 + 8; columns 32 half + 8 y + 2 (lane % 4) + {0, 1}
+      const int half = (warp - kScoreWarp) >> 2;  // 32 columns
+      // Rows i0 and i0 + 8, columns j0 + 8 y + {0, 1}.
+      const int i0 = 16 * q4 + (lane >> 2), j0 = 32 * half + 2 * (lane & 3);
       const int heads = WIDE ? 1 : u.nheads;
       for (int it = 0; it < n_chunks; ++it) {
         const int sl = it % kSums;
@@ -608,17 +613,19 @@ __global__ void __launch_bounds__(kThreads, 1) linear_chunk_kernel(const __grid_
           bad = true;
           break;
         }
-#pragma unroll 1
-        for (int half = 0; half < 2; ++half) {
+        const int live = live_of(it);
+        if (live < kC) {  // as the prepared values: rows past the length are zero before v is an operand
+          const int st = it % kStages, vecs = (kC - live) * 8;
+          for (int i = tid - 32 * kScoreWarp; i < (WIDE || u.nheads == 2 ? 2 : 1) * vecs; i += 256)
+            sts16(sb + (i < vecs ? L::va(st) : L::vb(st)) + live * 128 + 16 * (i % vecs), make_uint4(0, 0, 0, 0));
+        }
+        {
           float d[16];
           tmem_ld_frag(tm + kColD + 32 * half + tl, d);
           tmem_wait_ld();
-          if (half == 1) {
-            tc_fence_before();
-            __syncwarp();
-            if (lane == 0) mbar_arrive(&m.d_free);
-          }
-          const int j0 = 32 * half + 2 * (lane & 3);
+          tc_fence_before();
+          __syncwarp();
+          if (lane == 0) mbar_arrive(&m.d_free);
 #pragma unroll 1
           for (int x = 0; x < heads; ++x) {
             const float r0 = m.row[sl][x][i0], r1 = m.row[sl][x][i0 + 8];
@@ -664,14 +671,14 @@ __global__ void __launch_bounds__(kThreads, 1) linear_chunk_kernel(const __grid_
     }
   } else if (warp >= kPrepWarp) {
     // ---- weighted values, transposed into TMEM -------------------------------------------
-    fewer_registers<kPrepRegs>();
-    const int pt = tid - 32 * kPrepWarp;
+    fewer_registers<kOtherRegs>();
+    const int pt = tid - 32 * kPrepWarp, half = (warp - kPrepWarp) >> 2;  // 32 tokens
     const int blk = q4 >> 1;                       // block of value columns of this warp's lanes
     const int hd = WIDE ? 0 : blk;
     const bool mine = blk == 0 || two;
     if (!mine) {  // lanes without values stay zero
       const uint32_t z[16] = {};
-      for (int i = 0; i < 6; ++i) tmem_st16(tm + kColWV + 16 * i + tl, z);
+      for (int i = 0; i < 3; ++i) tmem_st16(tm + kColWV + 32 * i + 16 * half + tl, z);
     }
     for (int it = 0; it < n_chunks; ++it) {
       const int st = it % kStages, sl = it % kSums, live = live_of(it);
@@ -681,27 +688,27 @@ __global__ void __launch_bounds__(kThreads, 1) linear_chunk_kernel(const __grid_
         // Rows past the length hold anything: as operands they must be zero. (The scores may
         // read k before or after: those columns are masked.)
         const int vecs = (kC - live) * 8;
-        for (int i = pt; i < (NK + (two ? 2 : 1)) * vecs; i += 128) {
+        for (int i = pt; i < (NK + (two ? 2 : 1)) * vecs; i += 256) {
           const int box = i / vecs, at = i % vecs;
           const uint32_t base = box < NK ? L::k + (st * NK + box) * kBox : box == NK ? L::va(st) : L::vb(st);
           sts16(sb + base + live * 128 + 16 * at, make_uint4(0, 0, 0, 0));
         }
         fence_async_smem();
-        bad = bar_or(2, 128, bad);
+        bad = bar_or(2, 256, bad);
       }
       if (__any_sync(0xffffffffu, bad)) {
         bad = true;
         break;
       }
       // The operand is free once the previous chunk's state product has read it.
-      if (it > 0) bad |= !mbar_wait(&m.ds_full, (it - 1) & 1);
+      if (it > 0) bad |= !mbar_wait(&m.wv_free[half], (it - 1) & 1);
       tc_fence_after();
       if (mine) {
-        const float* w = &m.w[sl][hd][2 * (lane & 3)];
-        const uint32_t src = sb + (blk ? L::vb(st) : L::va(st)) + (lane >> 4) * 1024u + (lane & 7) * 128u;
+        const float* w = &m.w[sl][hd][32 * half + 2 * (lane & 3)];
+        const uint32_t src = sb + (blk ? L::vb(st) : L::va(st)) + half * 4096u + (lane >> 4) * 1024u + (lane & 7) * 128u;
         const uint32_t chunk = (4 * (q4 & 1) + ((lane >> 3) & 1)) ^ (lane & 7);
 #pragma unroll 2
-        for (int i = 0; i < 8; ++i) {  // 16 lanes (sub) x 16 tokens
+        for (int i = 0; i < 4; ++i) {  // 16 lanes (sub) x 16 tokens
           const int sub = i & 1, x = i >> 1;
           uint32_t in[4], hi[4], mid[4], lo[4];
           asm volatile("ldmatrix.sync.aligned.m8n8.x4.trans.shared.b16 {%0,%1,%2,%3}, [%4];"
@@ -717,7 +724,7 @@ __global__ void __launch_bounds__(kThreads, 1) linear_chunk_kernel(const __grid_
             mid[j] = take_bf16(y);
             lo[j] = __byte_perm(__float_as_uint(y.x), __float_as_uint(y.y), 0x7632);
           }
-          const uint32_t to = tm + kColWV + 8 * x + tl + (16u * sub << 16);
+          const uint32_t to = tm + kColWV + 16 * half + 8 * x + tl + (16u * sub << 16);
           tmem_st_16x128_x2(to, hi);
           tmem_st_16x128_x2(to + 32, mid);
           tmem_st_16x128_x2(to + 64, lo);
@@ -726,19 +733,18 @@ __global__ void __launch_bounds__(kThreads, 1) linear_chunk_kernel(const __grid_
       tmem_wait_st();
       tc_fence_before();
       __syncwarp();
-      if (lane == 0) mbar_arrive(&m.wv_ready);
+      if (lane == 0) mbar_arrive(&m.wv_ready[half]);
     }
   } else {
     // ---- state ------------------------------------------------------------------------------
     more_registers<kStateRegs>();
-    const int half = warp >> 2;
     const int row = 32 * q4 + lane;              // accumulator lane
     const int blk = row >> 6;                    // block of value columns
     const int hd = WIDE ? 0 : blk;               // head of the CTA
     const int col = WIDE ? row : row & 63;       // value column in the head
     const bool on = col < l.P && hd < u.nheads;
     const int head = u.head0 + hd;
-    constexpr int kNS = 32 * NK;                 // state values of a thread: key columns half * kNS ..
+    constexpr int kNS = 64 * NK;                 // state values of a thread: the key columns of a value
     const int64_t srow = static_cast<int64_t>(u.b) * l.H + head;
     float s[kNS];
 #pragma unroll
@@ -752,8 +758,7 @@ __global__ void __launch_bounds__(kThreads, 1) linear_chunk_kernel(const __grid_
       if (from && on) {
 #pragma unroll
         for (int i = 0; i < kNS; ++i) {
-          const int n = half * kNS + i;
-          if (n < l.N) s[i] = from[n * l.P + col];
+          if (i < l.N) s[i] = from[i * l.P + col];
         }
       }
     }
@@ -764,7 +769,7 @@ __global__ void __launch_bounds__(kThreads, 1) linear_chunk_kernel(const __grid_
         uint32_t r[16];
 #pragma unroll
         for (int j = 0; j < 16; ++j) r[j] = pack_bf16x2(s[i + 2 * j], s[i + 2 * j + 1]);
-        tmem_st16(tm + kColS + (half * kNS + i) / 2 + tl, r);
+        tmem_st16(tm + kColS + i / 2 + tl, r);
       }
       tmem_wait_st();
       tc_fence_before();
@@ -786,8 +791,8 @@ __global__ void __launch_bounds__(kThreads, 1) linear_chunk_kernel(const __grid_
 #pragma unroll
       for (int i = 0; i < kNS; i += 32) {
         float d[32];
-        tmem_ld16(tm + kColDS + half * kNS + i + tl, *reinterpret_cast<float(*)[16]>(d));
-        tmem_ld16(tm + kColDS + half * kNS + i + 16 + tl, *reinterpret_cast<float(*)[16]>(d + 16));
+        tmem_ld16(tm + kColDS + i + tl, *reinterpret_cast<float(*)[16]>(d));
+        tmem_ld16(tm + kColDS + i + 16 + tl, *reinterpret_cast<float(*)[16]>(d + 16));
         tmem_wait_ld();
 #pragma unroll
         for (int j = 0; j < 32; j += 2) {
@@ -821,8 +826,7 @@ __global__ void __launch_bounds__(kThreads, 1) linear_chunk_kernel(const __grid_
       if (to)
 #pragma unroll
         for (int i = 0; i < kNS; ++i) {
-          const int n = half * kNS + i;
-          if (n < l.N) to[n * l.P + col] = s[i];
+          if (i < l.N) to[i * l.P + col] = s[i];
         }
     }
   }
