@@ -295,13 +295,15 @@ __global__ void __launch_bounds__(kThreads, 1) linear_chunk_kernel(const __grid_
                             : max(min(static_cast<int64_t>(live_chunks), static_cast<int64_t>(u.first + p.seg_chunks)),
                                   static_cast<int64_t>(u.first)) * kC;
     const int64_t t1 = min(static_cast<int64_t>(l.T), static_cast<int64_t>(u.first + p.seg_chunks) * kC);
-    const int width = u.nheads * l.P;
-    for (int64_t i = tid; i < (t1 - t0) * width; i += kThreads) {
-      const int64_t t = t0 + i / width;
-      const int c = static_cast<int>(i % width);
-      static_cast<bf16*>(l.out)[u.b * l.so[0] + t * l.so[1] + (u.head0 + c / l.P) * l.so[2] + c % l.P] =
-          __float2bfloat16_rn(dead && slot >= 0 && t < u.len ? __int_as_float(0x7fc00000) : 0.f);
-    }
+    const uint32_t word = dead && slot >= 0 ? 0x7fc07fc0u : 0u;
+    const int vecs = u.nheads * l.P / 8, rows = kThreads / vecs;  // 16-byte vectors of a token; tokens at a time
+    const int c = tid % vecs * 8;
+    bf16* o = static_cast<bf16*>(l.out) + u.b * l.so[0] + (u.head0 + c / l.P) * l.so[2] + c % l.P;
+    if (tid < rows * vecs)
+      for (int64_t t = t0 + tid / vecs; t < t1; t += rows) {
+        const uint32_t x = t < u.len ? word : 0u;
+        *reinterpret_cast<uint4*>(o + t * l.so[1]) = make_uint4(x, x, x, x);
+      }
     if (dead) return;
     if (live_chunks == 0 && u.seg == 0 && l.fresh)
       for (int i = tid; i < u.nheads * l.N * l.P; i += kThreads)
