@@ -91,9 +91,9 @@ struct alignas(16) Misc {
   uint64_t full[kStages], empty[kStages];    // tiles loaded / every product of them done
   uint64_t sums[kSums], sums_free[kSums];    // decay sums written / read
   uint64_t d_full, d_free;                   // scores there / read
-  uint64_t p_ready[2], o_full[2], o_free;    // P written, both output products there / read
-  uint64_t wv_ready[2], wv_free[2];          // weighted values of half a chunk written / read
-  uint64_t ds_full, ds_free;                 // state product there / read
+  uint64_t p_ready[2], o_full[2], o_free[2]; // P written, both output products there / read
+  uint64_t wv_ready[2][2], wv_free[2][2];    // [buffer][half] weighted values written / read
+  uint64_t ds_full[2], ds_free[2];           // state product there / read
   uint64_t s_ready, oi_full;                 // state operand written / read
   uint32_t tmem;
   alignas(16) float row[kSums][2][kC];  // [chunk][head] two factors of scale e^{c_i - c_j}, or c_i and
@@ -110,7 +110,16 @@ constexpr int smem_bytes() {
 
 // TMEM columns. The weighted values (three parts of 64 tokens) and the state (BF16) are
 // operands there: as shared-memory tiles they would cost 160 KB of its traffic a chunk.
-constexpr uint32_t kColD = 0, kColDS = 64, kColOI = 192, kColOP = 256, kColWV = 320, kColS = 416;
+// What the 512 columns leave room for is held twice, so that the next chunk's is formed
+// while this one's is read: the output products where N <= 64; for a segment's own state,
+// its weighted values and products.
+template <int NK, bool FULL>
+struct Tmem {
+  static constexpr int o_bufs = NK == 1 ? 2 : 1, wv_bufs = FULL ? 1 : 2, ds_bufs = FULL ? 1 : 2;
+  static constexpr uint32_t d = 0, ds = FULL ? 64 : 0, oi = ds + 64 * NK * ds_bufs, op = oi + (FULL ? 64 * o_bufs : 0),
+                            wv = op + (FULL ? 64 * o_bufs : 0), s = wv + 96 * wv_bufs, end = s + (FULL ? 32 * NK : 0);
+  static_assert(end <= 512, "TMEM has 512 columns");
+};
 
 constexpr uint32_t idesc_bf16(int m, int n, bool a_mn, bool b_mn) {
   return idesc_f16_f32(m, n, a_mn, b_mn) | (1u << 7) | (1u << 10);
@@ -149,17 +158,6 @@ __device__ __forceinline__ void tma_store_4d(const void* tmap, uint32_t src, int
   asm volatile("cp.async.bulk.commit_group;" ::: "memory");
 }
 __device__ __forceinline__ void tma_store_wait_read() { asm volatile("cp.async.bulk.wait_group.read 0;" ::: "memory"); }
-// 16 TMEM lanes x 32 columns as m16n8 fragments: thread t gets lanes t/4 and t/4 + 8,
-// columns 8 x + 2 (t % 4) + {0, 1}, as r[4 x + 0..1] and r[4 x + 2..3].
-__device__ __forceinline__ void tmem_ld_frag(uint32_t taddr, float (&r)[16]) {
-  uint32_t* u = reinterpret_cast<uint32_t*>(r);
-  asm volatile(
-      "tcgen05.ld.sync.aligned.16x256b.x4.b32 {%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15}, [%16];"
-      : "=r"(u[0]), "=r"(u[1]), "=r"(u[2]), "=r"(u[3]), "=r"(u[4]), "=r"(u[5]), "=r"(u[6]), "=r"(u[7]),
-        "=r"(u[8]), "=r"(u[9]), "=r"(u[10]), "=r"(u[11]), "=r"(u[12]), "=r"(u[13]), "=r"(u[14]), "=r"(u[15])
-      : "r"(taddr)
-      : "memory");
-}
 // 16 lanes x 8 columns: thread t gives lanes t/4 and t/4 + 8, column 4 x + t % 4, as r[2 x]
 // and r[2 x + 1].
 __device__ __forceinline__ void tmem_st_16x128_x2(uint32_t taddr, const uint32_t (&r)[4]) {
@@ -177,7 +175,8 @@ __device__ __forceinline__ void tmem_st16(uint32_t taddr, const uint32_t (&r)[16
       : "memory");
 }
 __device__ __forceinline__ void tmem_wait_st() { asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory"); }
-// As tmem_ld_frag, 16 columns.
+// 16 TMEM lanes x 16 columns as m16n8 fragments: thread t gets lanes t/4 and t/4 + 8,
+// columns 8 x + 2 (t % 4) + {0, 1}, as r[4 x + 0..1] and r[4 x + 2..3].
 __device__ __forceinline__ void tmem_ld_frag2(uint32_t taddr, float (&r)[8]) {
   uint32_t* u = reinterpret_cast<uint32_t*>(r);
   asm volatile("tcgen05.ld.sync.aligned.16x256b.x2.b32 {%0,%1,%2,%3,%4,%5,%6,%7}, [%8];"
@@ -271,6 +270,7 @@ __device__ __forceinline__ Unit unit_of(const ChunkParams& p, int x) {
 template <int NK, bool WIDE, bool FULL>
 __global__ void __launch_bounds__(kThreads, 1) linear_chunk_kernel(const __grid_constant__ ChunkParams p) {
   using L = Layout<NK>;
+  using C = Tmem<NK, FULL>;
   extern __shared__ unsigned char smem_raw[];
   const uint32_t sb = (smem_u32(smem_raw) + 1023u) & ~1023u;
   Misc& m = *reinterpret_cast<Misc*>(smem_raw + (sb - smem_u32(smem_raw)) + L::misc);
@@ -331,20 +331,25 @@ __global__ void __launch_bounds__(kThreads, 1) linear_chunk_kernel(const __grid_
     for (int i = 0; i < 2; ++i) {
       mbar_init(&m.p_ready[i], 8);
       mbar_init(&m.o_full[i], 1);
-      mbar_init(&m.wv_ready[i], 4);
-      mbar_init(&m.wv_free[i], 1);
+      mbar_init(&m.o_free[i], 8);
+      for (int j = 0; j < 2; ++j) {
+        mbar_init(&m.wv_ready[i][j], 4);
+        mbar_init(&m.wv_free[i][j], 1);
+      }
+      mbar_init(&m.ds_full[i], 1);
+      mbar_init(&m.ds_free[i], 4);
     }
     mbar_init(&m.d_full, 1);
     mbar_init(&m.d_free, 8);
-    mbar_init(&m.o_free, 8);
-    mbar_init(&m.ds_full, 1);
-    mbar_init(&m.ds_free, 4);
     mbar_init(&m.s_ready, 4);
     mbar_init(&m.oi_full, 1);
     fence_mbar_init();
   }
-  if (FULL && !WIDE)
-    for (int i = tid; i < kBox / 16; i += kThreads) sts16(sb + L::zero + 16 * i, make_uint4(0, 0, 0, 0));
+  if (FULL) {  // the zero tile, and P's tiles: what lies above the diagonal is never written
+    if (!WIDE)
+      for (int i = tid; i < kBox / 16; i += kThreads) sts16(sb + L::zero + 16 * i, make_uint4(0, 0, 0, 0));
+    for (int i = tid; i < 4 * kBox / 16; i += kThreads) sts16(sb + L::p + 16 * i, make_uint4(0, 0, 0, 0));
+  }
   fence_async_smem();
   tc_fence_before();
   __syncthreads();
@@ -397,7 +402,7 @@ __global__ void __launch_bounds__(kThreads, 1) linear_chunk_kernel(const __grid_
 #pragma unroll
           for (int kk = 0; kk < 4 * NK; ++kk) {
             const uint32_t off = ((kk >> 2) * kBox + (kk & 3) * 32u) >> 4;
-            umma_f16(tm + kColD, desc_of(qd + off), desc_of(kd + off), idesc_bf16(64, 64, false, false), kk > 0);
+            umma_f16(tm + C::d, desc_of(qd + off), desc_of(kd + off), idesc_bf16(64, 64, false, false), kk > 0);
           }
           umma_commit(&m.d_full);
         }
@@ -405,23 +410,23 @@ __global__ void __launch_bounds__(kThreads, 1) linear_chunk_kernel(const __grid_
         return true;
       };
       auto state = [&](int it) {  // dS^T
-        const int st = it % kStages;
+        const int st = it % kStages, wb = it % C::wv_bufs, db = it % C::ds_bufs;
         const uint32_t kd = desc_lo(sb + L::k + st * NK * kBox, kBox);
-        if (it > 0 && !mbar_wait(&m.ds_free, (it - 1) & 1)) return false;
+        if (it >= C::ds_bufs && !mbar_wait(&m.ds_free[db], (it / C::ds_bufs - 1) & 1)) return false;
 #pragma unroll 1
         for (int half = 0; half < 2; ++half) {
-          if (!mbar_wait(&m.wv_ready[half], it & 1)) return false;
+          if (!mbar_wait(&m.wv_ready[wb][half], (it / C::wv_bufs) & 1)) return false;
           tc_fence_after();
           if (elect_one()) {
 #pragma unroll
             for (int part = 2; part >= 0; --part)  // the small parts first
 #pragma unroll
               for (int kk = 0; kk < 2; ++kk)
-                umma_ts(tm + kColDS, tm + kColWV + 32 * part + 16 * half + 8 * kk,
+                umma_ts(tm + C::ds + 64 * NK * db, tm + C::wv + 96 * wb + 32 * part + 16 * half + 8 * kk,
                         desc_of(kd + (half * 4096u + kk * 2048u >> 4)), idesc_bf16(128, 64 * NK, false, true),
                         half > 0 || part < 2 || kk > 0);
-            umma_commit(&m.wv_free[half]);
-            if (half == 1) umma_commit(&m.ds_full);
+            umma_commit(&m.wv_free[wb][half]);
+            if (half == 1) umma_commit(&m.ds_full[db]);
             if (half == 1) umma_commit(&m.empty[st]);
           }
           __syncwarp();
@@ -438,13 +443,14 @@ __global__ void __launch_bounds__(kThreads, 1) linear_chunk_kernel(const __grid_
         const int st = it % kStages;
         if (!mbar_wait(&m.full[st], (it / kStages) & 1)) return false;
         if (!mbar_wait(&m.s_ready, it & 1)) return false;
-        if (it > 0 && !mbar_wait(&m.o_free, (it - 1) & 1)) return false;
+        const int ob = it % C::o_bufs;
+        if (it >= C::o_bufs && !mbar_wait(&m.o_free[ob], (it / C::o_bufs - 1) & 1)) return false;
         tc_fence_after();
         const uint32_t qd = desc_lo(sb + L::q + st * NK * kBox, 0);
         if (elect_one()) {
 #pragma unroll
           for (int kk = 0; kk < 4 * NK; ++kk)
-            umma_ts(tm + kColOI, tm + kColS + 8 * kk, desc_of(qd + (((kk >> 2) * kBox + (kk & 3) * 32u) >> 4)),
+            umma_ts(tm + C::oi + 64 * ob, tm + C::s + 8 * kk, desc_of(qd + (((kk >> 2) * kBox + (kk & 3) * 32u) >> 4)),
                     idesc_bf16(128, 64, false, false), kk > 0);
           umma_commit(&m.oi_full);
         }
@@ -462,12 +468,12 @@ __global__ void __launch_bounds__(kThreads, 1) linear_chunk_kernel(const __grid_
         if (elect_one()) {
 #pragma unroll
           for (int kk = 0; kk < 4; ++kk)
-            umma_f16(tm + kColOP, desc_of(v0 + (kk * 2048u >> 4)), desc_of(pd + (kk * 32u >> 4)),
+            umma_f16(tm + C::op + 64 * (it % C::o_bufs), desc_of(v0 + (kk * 2048u >> 4)), desc_of(pd + (kk * 32u >> 4)),
                      idesc_bf16(128, 64, true, false), kk > 0);
           if (!WIDE && u.nheads == 2) {
 #pragma unroll
             for (int kk = 0; kk < 4; ++kk)
-              umma_f16(tm + kColOP, desc_of(v1 + (kk * 2048u >> 4)), desc_of(pd + ((kBox + kk * 32u) >> 4)),
+              umma_f16(tm + C::op + 64 * (it % C::o_bufs), desc_of(v1 + (kk * 2048u >> 4)), desc_of(pd + ((kBox + kk * 32u) >> 4)),
                        idesc_bf16(128, 64, true, false), 1);
           }
           umma_commit(&m.o_full[it & 1]);
@@ -564,13 +570,14 @@ __global__ void __launch_bounds__(kThreads, 1) linear_chunk_kernel(const __grid_
         if (lane == 0) tma_store_wait_read();
         __syncwarp();
         const float* ecs = &m.ecs[sl][hd < u.nheads ? hd : 0][32 * half + 2 * (lane & 3)];
-        const int live = live_of(it) - 32 * half - 2 * (lane & 3);
+        const uint32_t from = tm + C::oi + 64 * (it % C::o_bufs) + 32 * half + tl;
+        const int live = live_of(it);
 #pragma unroll 2
         for (int i = 0; i < 4; ++i) {  // 16 lanes (sub) x 16 tokens
           const int x = i >> 1, sub = i & 1;
           float oi[8], op[8];
-          tmem_ld_frag2(tm + kColOI + 32 * half + 16 * x + tl + (16u * sub << 16), oi);
-          tmem_ld_frag2(tm + kColOP + 32 * half + 16 * x + tl + (16u * sub << 16), op);
+          tmem_ld_frag2(from + 16 * x + (16u * sub << 16), oi);
+          tmem_ld_frag2(from + (C::op - C::oi) + 16 * x + (16u * sub << 16), op);
           const float2 e[2] = {*reinterpret_cast<const float2*>(ecs + 16 * x),
                                *reinterpret_cast<const float2*>(ecs + 16 * x + 8)};
           tmem_wait_ld();
@@ -578,8 +585,14 @@ __global__ void __launch_bounds__(kThreads, 1) linear_chunk_kernel(const __grid_
 #pragma unroll
           for (int j = 0; j < 4; ++j) {
             const float2 y = fma2(make_float2(oi[2 * j], oi[2 * j + 1]), e[j >> 1], make_float2(op[2 * j], op[2 * j + 1]));
-            const int left = live - 16 * x - 8 * (j >> 1);  // rows past the length are zero
-            o[j] = pack_bf16x2(y.x, y.y) & (left > 1 ? 0xffffffffu : left > 0 ? 0xffffu : 0u);
+            o[j] = pack_bf16x2(y.x, y.y);
+          }
+          if (live < kC) {  // rows past the length are zero
+#pragma unroll
+            for (int j = 0; j < 4; ++j) {
+              const int left = live - 32 * half - 2 * (lane & 3) - 16 * x - 8 * (j >> 1);
+              o[j] &= left > 1 ? 0xffffffffu : left > 0 ? 0xffffu : 0u;
+            }
           }
           stsm_x4_t(stage + x * 1024u + (lane >> 4) * 512u + (lane & 7) * 64u +
                         (((2 * sub + ((lane >> 3) & 1)) ^ ((lane >> 1) & 3)) << 4),
@@ -589,7 +602,7 @@ __global__ void __launch_bounds__(kThreads, 1) linear_chunk_kernel(const __grid_
         fence_async_smem();
         __syncwarp();
         if (lane == 0) {
-          mbar_arrive(&m.o_free);
+          mbar_arrive(&m.o_free[it % C::o_bufs]);
           mbar_arrive(&m.sums_free[sl]);
           if (stores && t0 < l.T) tma_store_4d(&p.tm_o, stage, ocol, head, t0, u.b);
         }
@@ -602,9 +615,18 @@ __global__ void __launch_bounds__(kThreads, 1) linear_chunk_kernel(const __grid_
     fewer_registers<kOtherRegs>();
     if (FULL) {
       const int half = (warp - kScoreWarp) >> 2;  // 32 columns
-      // Rows i0 and i0 + 8, columns j0 + 8 y + {0, 1}.
+      // Rows i0 and i0 + 8; 16 columns at a time: j0 + 16 z + 8 y + {0, 1}, y < 2. Columns past
+      // the warp's last row are left alone.
       const int i0 = 16 * q4 + (lane >> 2), j0 = 32 * half + 2 * (lane & 3);
+      const int steps = min(2, max(0, q4 + 1 - 2 * half));
       const int heads = WIDE ? 1 : u.nheads;
+      // Pairs of the last step that lie on or below the diagonal, [y][row group].
+      uint32_t keep[4];
+#pragma unroll
+      for (int j = 0; j < 4; ++j) {
+        const int left = i0 + 8 * (j & 1) - (j0 + 16 * (q4 - 2 * half) + 8 * (j >> 1));
+        keep[j] = left >= 1 ? 0xffffffffu : left == 0 ? 0xffffu : 0u;
+      }
       for (int it = 0; it < n_chunks; ++it) {
         const int sl = it % kSums;
         bad |= !mbar_wait(&m.sums[sl], (it / kSums) & 1);
@@ -621,51 +643,47 @@ __global__ void __launch_bounds__(kThreads, 1) linear_chunk_kernel(const __grid_
           for (int i = tid - 32 * kScoreWarp; i < (WIDE || u.nheads == 2 ? 2 : 1) * vecs; i += 256)
             sts16(sb + (i < vecs ? L::va(st) : L::vb(st)) + live * 128 + 16 * (i % vecs), make_uint4(0, 0, 0, 0));
         }
-        {
-          float d[16];
-          tmem_ld_frag(tm + kColD + 32 * half + tl, d);
+#pragma unroll 1
+        for (int z = 0; z < steps; ++z) {
+          float d[8];
+          tmem_ld_frag2(tm + C::d + 32 * half + 16 * z + tl, d);
           tmem_wait_ld();
-          tc_fence_before();
-          __syncwarp();
-          if (lane == 0) mbar_arrive(&m.d_free);
+          const bool diagonal = 2 * half + z == q4;
 #pragma unroll 1
           for (int x = 0; x < heads; ++x) {
-            const float r0 = m.row[sl][x][i0], r1 = m.row[sl][x][i0 + 8];
-            const float* cj = m.col[sl][x] + j0;
-            float2 e[8];  // [column group y][row group]
+            const float r[2] = {m.row[sl][x][i0], m.row[sl][x][i0 + 8]};
+            const float* cj = m.col[sl][x] + j0 + 16 * z;
+            const float2 c[2] = {*reinterpret_cast<const float2*>(cj), *reinterpret_cast<const float2*>(cj + 8)};
+            uint32_t o[4];  // [y][row group]
             if (m.factors[sl][x]) {
 #pragma unroll
-              for (int y = 0; y < 4; ++y) {
-                const float2 c = *reinterpret_cast<const float2*>(cj + 8 * y);
-                e[2 * y] = mul2(make_float2(r0, r0), c);
-                e[2 * y + 1] = mul2(make_float2(r1, r1), c);
+              for (int j = 0; j < 4; ++j) {
+                const float2 e = mul2(make_float2(r[j & 1], r[j & 1]), c[j >> 1]);
+                const float2 w = mul2(e, make_float2(d[2 * j], d[2 * j + 1]));
+                o[j] = pack_bf16x2(w.x, w.y);
               }
             } else {
 #pragma unroll
-              for (int y = 0; y < 4; ++y) {
-                const float2 c = *reinterpret_cast<const float2*>(cj + 8 * y);
-                e[2 * y] = make_float2(l.scale * ex2_approx(r0 + c.x), l.scale * ex2_approx(r0 + c.y));
-                e[2 * y + 1] = make_float2(l.scale * ex2_approx(r1 + c.x), l.scale * ex2_approx(r1 + c.y));
-              }
+              for (int j = 0; j < 4; ++j)
+                o[j] = pack_bf16x2(l.scale * ex2_approx(r[j & 1] + c[j >> 1].x) * d[2 * j],
+                                   l.scale * ex2_approx(r[j & 1] + c[j >> 1].y) * d[2 * j + 1]);
             }
-            const uint32_t ps = sb + L::p + (2 * (it & 1) + x) * kBox + i0 * 128u;
-            uint32_t o[8];
+            if (diagonal) {
 #pragma unroll
-            for (int y = 0; y < 4; ++y)
+              for (int j = 0; j < 4; ++j) o[j] &= keep[j];
+            }
+            const uint32_t ps = sb + L::p + (2 * (it & 1) + x) * kBox + i0 * 128u + 4 * (lane & 3);
 #pragma unroll
-              for (int r = 0; r < 2; ++r) {
-                const float2 w = mul2(e[2 * y + r], make_float2(d[4 * y + 2 * r], d[4 * y + 2 * r + 1]));
-                const int left = i0 + 8 * r - j0 - 8 * y;  // columns j <= row: left >= 0, left >= 1
-                o[2 * y + r] = pack_bf16x2(left >= 0 ? w.x : 0.f, left >= 1 ? w.y : 0.f);
-              }
-#pragma unroll
-            for (int y = 0; y < 4; ++y) {
-              const uint32_t to = ps + (((4 * half + y) ^ (lane >> 2)) << 4) + 4 * (lane & 3);
+            for (int y = 0; y < 2; ++y) {
+              const uint32_t to = ps + (((4 * half + 2 * z + y) ^ (lane >> 2)) << 4);
               sts4(to, o[2 * y]);
               sts4(to + 1024u, o[2 * y + 1]);
             }
           }
         }
+        tc_fence_before();
+        __syncwarp();
+        if (lane == 0) mbar_arrive(&m.d_free);
         fence_async_smem();
         __syncwarp();
         if (lane == 0) mbar_arrive(&m.p_ready[it & 1]);
@@ -680,10 +698,10 @@ __global__ void __launch_bounds__(kThreads, 1) linear_chunk_kernel(const __grid_
     const bool mine = blk == 0 || two;
     if (!mine) {  // lanes without values stay zero
       const uint32_t z[16] = {};
-      for (int i = 0; i < 3; ++i) tmem_st16(tm + kColWV + 32 * i + 16 * half + tl, z);
+      for (int i = 0; i < 3 * C::wv_bufs; ++i) tmem_st16(tm + C::wv + 32 * i + 16 * half + tl, z);
     }
     for (int it = 0; it < n_chunks; ++it) {
-      const int st = it % kStages, sl = it % kSums, live = live_of(it);
+      const int st = it % kStages, sl = it % kSums, live = live_of(it), wb = it % C::wv_bufs;
       bad |= !mbar_wait(&m.full[st], (it / kStages) & 1);
       bad |= !mbar_wait(&m.sums[sl], (it / kSums) & 1);
       if (live < kC) {
@@ -702,8 +720,8 @@ __global__ void __launch_bounds__(kThreads, 1) linear_chunk_kernel(const __grid_
         bad = true;
         break;
       }
-      // The operand is free once the previous chunk's state product has read it.
-      if (it > 0) bad |= !mbar_wait(&m.wv_free[half], (it - 1) & 1);
+      // The operand is free once the state product before has read it.
+      if (it >= C::wv_bufs) bad |= !mbar_wait(&m.wv_free[wb][half], (it / C::wv_bufs - 1) & 1);
       tc_fence_after();
       if (mine) {
         const float* w = &m.w[sl][hd][32 * half + 2 * (lane & 3)];
@@ -726,7 +744,7 @@ __global__ void __launch_bounds__(kThreads, 1) linear_chunk_kernel(const __grid_
             mid[j] = take_bf16(y);
             lo[j] = __byte_perm(__float_as_uint(y.x), __float_as_uint(y.y), 0x7632);
           }
-          const uint32_t to = tm + kColWV + 16 * half + 8 * x + tl + (16u * sub << 16);
+          const uint32_t to = tm + C::wv + 96 * wb + 16 * half + 8 * x + tl + (16u * sub << 16);
           tmem_st_16x128_x2(to, hi);
           tmem_st_16x128_x2(to + 32, mid);
           tmem_st_16x128_x2(to + 64, lo);
@@ -735,7 +753,7 @@ __global__ void __launch_bounds__(kThreads, 1) linear_chunk_kernel(const __grid_
       tmem_wait_st();
       tc_fence_before();
       __syncwarp();
-      if (lane == 0) mbar_arrive(&m.wv_ready[half]);
+      if (lane == 0) mbar_arrive(&m.wv_ready[wb][half]);
     }
   } else {
     // ---- state ------------------------------------------------------------------------------
@@ -771,7 +789,7 @@ __global__ void __launch_bounds__(kThreads, 1) linear_chunk_kernel(const __grid_
         uint32_t r[16];
 #pragma unroll
         for (int j = 0; j < 16; ++j) r[j] = pack_bf16x2(s[i + 2 * j], s[i + 2 * j + 1]);
-        tmem_st16(tm + kColS + i / 2 + tl, r);
+        tmem_st16(tm + C::s + i / 2 + tl, r);
       }
       tmem_wait_st();
       tc_fence_before();
@@ -780,10 +798,10 @@ __global__ void __launch_bounds__(kThreads, 1) linear_chunk_kernel(const __grid_
     };
     if (FULL) put_state();
     for (int it = 0; it < n_chunks; ++it) {
-      const int sl = it % kSums;
+      const int sl = it % kSums, db = it % C::ds_bufs;
       // S = e^{c_C} S + dS.
       bad |= !mbar_wait(&m.sums[sl], (it / kSums) & 1);
-      bad |= !mbar_wait(&m.ds_full, it & 1);
+      bad |= !mbar_wait(&m.ds_full[db], (it / C::ds_bufs) & 1);
       tc_fence_after();
       if (__any_sync(0xffffffffu, bad)) {
         bad = true;
@@ -793,8 +811,8 @@ __global__ void __launch_bounds__(kThreads, 1) linear_chunk_kernel(const __grid_
 #pragma unroll
       for (int i = 0; i < kNS; i += 32) {
         float d[32];
-        tmem_ld16(tm + kColDS + i + tl, *reinterpret_cast<float(*)[16]>(d));
-        tmem_ld16(tm + kColDS + i + 16 + tl, *reinterpret_cast<float(*)[16]>(d + 16));
+        tmem_ld16(tm + C::ds + 64 * NK * db + i + tl, *reinterpret_cast<float(*)[16]>(d));
+        tmem_ld16(tm + C::ds + 64 * NK * db + i + 16 + tl, *reinterpret_cast<float(*)[16]>(d + 16));
         tmem_wait_ld();
 #pragma unroll
         for (int j = 0; j < 32; j += 2) {
@@ -806,7 +824,7 @@ __global__ void __launch_bounds__(kThreads, 1) linear_chunk_kernel(const __grid_
       tc_fence_before();
       __syncwarp();
       if (lane == 0) {
-        mbar_arrive(&m.ds_free);
+        mbar_arrive(&m.ds_free[db]);
         mbar_arrive(&m.sums_free[sl]);
       }
       if (FULL && it + 1 < n_chunks) {
