@@ -45,14 +45,15 @@ using namespace sm100;
 
 constexpr int kC = 64;                // tokens of a chunk
 constexpr int kBox = 8192;            // bytes of a 64 x 64 BF16 tile
-constexpr int kStages = 3;            // chunks in shared memory
 constexpr int kSums = 4;              // chunks whose decay sums are kept
 constexpr float kMinLog2 = -256.f;    // a decay below it is zero in FP32 against any state
 
 // Warps, by what they do; groups of four have the four quarters of the TMEM lanes, pairs of
 // groups the two halves of a chunk's tokens.
 constexpr int kPrepWarp = 4, kScoreWarp = 12, kOutWarp = 20;  // (state: 0)
-constexpr int kLoadWarp = 28, kSumWarp = 29, kStateMmaWarp = 30, kOutMmaWarp = 31;
+// A quarter's warps share a scheduler, and the later a chunk's rows the more scores they have:
+// the last quarter's gets the lightest of the single warps.
+constexpr int kSumWarp = 28, kStateMmaWarp = 29, kOutMmaWarp = 30, kLoadWarp = 31;
 constexpr int kThreads = 32 * 32;
 // Registers of a thread: 32 warps have 64 at launch, 2048 together, and share them out again
 // as 4 * 160 + 8 * 56 + 20 * 48 = 2048.
@@ -72,29 +73,16 @@ struct ChunkParams {
   int* err_host;
 };
 
-// Shared memory, in bytes from a 1024-byte boundary. The value tiles of the stages lie
-// around one zero tile, a2 a1 a0 zero b0 b1 b2: a block's tile and the zero tile are the two
-// 64-column blocks of the operand of its head's OP product.
-template <int NK>
-struct Layout {
-  static constexpr int q = 0;                               // [stage][NK]
-  static constexpr int k = q + kStages * NK * kBox;         // [stage][NK]
-  static constexpr int v = k + kStages * NK * kBox;
-  static constexpr int zero = v + kStages * kBox;
-  static constexpr int p = zero + (kStages + 1) * kBox;     // [chunk & 1][head]
-  static constexpr int o = p + 4 * kBox;                    // [warp][half] 32 tokens x 32 columns
-  static constexpr int misc = o + 8 * 2048;
-  static __device__ __forceinline__ uint32_t va(int stage) { return zero - (stage + 1) * kBox; }
-  static __device__ __forceinline__ uint32_t vb(int stage) { return zero + (stage + 1) * kBox; }
-};
+template <int STAGES>
 struct alignas(16) Misc {
-  uint64_t full[kStages], empty[kStages];    // tiles loaded / every product of them done
+  uint64_t full[STAGES], empty[STAGES];      // tiles loaded / every product of them done
   uint64_t sums[kSums], sums_free[kSums];    // decay sums written / read
-  uint64_t d_full, d_free;                   // scores there / read
-  uint64_t p_ready[2], o_full[2], o_free[2]; // P written, both output products there / read
+  uint64_t d_full[2];                        // scores there
+  uint64_t p_ready[2], o_full[2];            // P written, both output products there
+  uint64_t oi_free, op_free[2];              // the products read
   uint64_t wv_ready[2][2], wv_free[2][2];    // [buffer][half] weighted values written / read
   uint64_t ds_full[2], ds_free[2];           // state product there / read
-  uint64_t s_ready, oi_full;                 // state operand written / read
+  uint64_t s_ready, s_free;                  // state operand written / read
   uint32_t tmem;
   alignas(16) float row[kSums][2][kC];  // [chunk][head] two factors of scale e^{c_i - c_j}, or c_i and
   float col[kSums][2][kC];              // -c_j (log2) where a factor would leave FP32's range
@@ -103,21 +91,56 @@ struct alignas(16) Misc {
   float total[kSums][2];                // e^{c_C}
   int factors[kSums][2];                // row and col hold factors
 };
-template <int NK>
-constexpr int smem_bytes() {
-  return Layout<NK>::misc + static_cast<int>(sizeof(Misc)) + 1024;
-}
+// Shared memory, in bytes from a 1024-byte boundary: as many stages (chunks) as fit, up to
+// six. The value tiles of a pair of heads lie around one zero tile, .. a1 a0 zero b0 b1 ..: a
+// head's tile and the zero tile are the two 64-column blocks of the operand of its OP product.
+template <int NK, bool WIDE, bool FULL>
+struct Layout {
+  static constexpr int tiles = (FULL ? 2 : 1) * NK + 2;     // of a stage
+  static constexpr int fixed = FULL ? (WIDE ? 2 : 5) * kBox + 8 * 2048 : 0;
+  static constexpr int fit = (232448 - 1024 - static_cast<int>(sizeof(Misc<6>)) - fixed) / (tiles * kBox);
+  static constexpr int stages = fit > 6 ? 6 : fit;
+  static constexpr bool zero_tile = FULL && !WIDE;
+  static constexpr int k = 0;                               // [stage][NK]
+  static constexpr int q = k + stages * NK * kBox;          // [stage][NK]
+  static constexpr int v = q + (FULL ? stages * NK * kBox : 0);
+  static constexpr int zero = v + stages * kBox;
+  static constexpr int p = v + (2 * stages + (zero_tile ? 1 : 0)) * kBox;  // [chunk & 1][head]
+  static constexpr int o = p + (FULL ? (WIDE ? 2 : 4) * kBox : 0);         // [warp] 32 tokens x 32 columns
+  static constexpr int misc = o + (FULL ? 8 * 2048 : 0);
+  static constexpr int bytes = misc + static_cast<int>(sizeof(Misc<stages>)) + 1024;
+  static_assert(stages >= 3 && bytes <= 232448, "shared memory of a CTA");
+  static __device__ __forceinline__ uint32_t va(int stage) {
+    return zero_tile ? zero - (stage + 1) * kBox : v + 2 * stage * kBox;
+  }
+  static __device__ __forceinline__ uint32_t vb(int stage) {
+    return zero_tile ? zero + (stage + 1) * kBox : v + (2 * stage + 1) * kBox;
+  }
+  static __device__ __forceinline__ uint32_t ptile(int it, int head) {
+    return p + (WIDE ? it & 1 : 2 * (it & 1) + head) * kBox;
+  }
+};
+// The stage of a chunk and the parity of its turn there.
+template <int STAGES>
+struct Ring {
+  int st = 0;
+  uint32_t ph = 0;
+  __device__ __forceinline__ void next() {
+    if (++st == STAGES) st = 0, ph ^= 1;
+  }
+};
 
 // TMEM columns. The weighted values (three parts of 64 tokens) and the state (BF16) are
 // operands there: as shared-memory tiles they would cost 160 KB of its traffic a chunk.
-// What the 512 columns leave room for is held twice, so that the next chunk's is formed
-// while this one's is read: the output products where N <= 64; for a segment's own state,
-// its weighted values and products.
+// D and then OP of a chunk share 64 columns, and neighbouring chunks have two sets of them,
+// so that one's D is formed while the other's OP is read. What the 512 columns leave room for
+// is held twice as well: the weighted values where N <= 64; for a segment's own state, its
+// weighted values and products.
 template <int NK, bool FULL>
 struct Tmem {
-  static constexpr int o_bufs = NK == 1 ? 2 : 1, wv_bufs = FULL ? 1 : 2, ds_bufs = FULL ? 1 : 2;
-  static constexpr uint32_t d = 0, ds = FULL ? 64 : 0, oi = ds + 64 * NK * ds_bufs, op = oi + (FULL ? 64 * o_bufs : 0),
-                            wv = op + (FULL ? 64 * o_bufs : 0), s = wv + 96 * wv_bufs, end = s + (FULL ? 32 * NK : 0);
+  static constexpr int wv_bufs = FULL && NK == 2 ? 1 : 2, ds_bufs = FULL ? 1 : 2;
+  static constexpr uint32_t x = 0, ds = FULL ? 128 : 0, oi = ds + 64 * NK * ds_bufs, wv = oi + (FULL ? 64 : 0),
+                            s = wv + 96 * wv_bufs, end = s + (FULL ? 32 * NK : 0);
   static_assert(end <= 512, "TMEM has 512 columns");
 };
 
@@ -269,11 +292,12 @@ __device__ __forceinline__ Unit unit_of(const ChunkParams& p, int x) {
 // FULL: the outputs and the final state; otherwise a segment's own state from zero.
 template <int NK, bool WIDE, bool FULL>
 __global__ void __launch_bounds__(kThreads, 1) linear_chunk_kernel(const __grid_constant__ ChunkParams p) {
-  using L = Layout<NK>;
+  using L = Layout<NK, WIDE, FULL>;
+  constexpr int kStages = L::stages;
   using C = Tmem<NK, FULL>;
   extern __shared__ unsigned char smem_raw[];
   const uint32_t sb = (smem_u32(smem_raw) + 1023u) & ~1023u;
-  Misc& m = *reinterpret_cast<Misc*>(smem_raw + (sb - smem_u32(smem_raw)) + L::misc);
+  Misc<kStages>& m = *reinterpret_cast<Misc<kStages>*>(smem_raw + (sb - smem_u32(smem_raw)) + L::misc);
   const LinearParams& l = p.l;
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
   const Unit u = unit_of<WIDE>(p, blockIdx.x);
@@ -331,7 +355,8 @@ __global__ void __launch_bounds__(kThreads, 1) linear_chunk_kernel(const __grid_
     for (int i = 0; i < 2; ++i) {
       mbar_init(&m.p_ready[i], 8);
       mbar_init(&m.o_full[i], 1);
-      mbar_init(&m.o_free[i], 8);
+      mbar_init(&m.op_free[i], 8);
+      mbar_init(&m.d_full[i], 1);
       for (int j = 0; j < 2; ++j) {
         mbar_init(&m.wv_ready[i][j], 4);
         mbar_init(&m.wv_free[i][j], 1);
@@ -339,16 +364,15 @@ __global__ void __launch_bounds__(kThreads, 1) linear_chunk_kernel(const __grid_
       mbar_init(&m.ds_full[i], 1);
       mbar_init(&m.ds_free[i], 4);
     }
-    mbar_init(&m.d_full, 1);
-    mbar_init(&m.d_free, 8);
+    mbar_init(&m.oi_free, 8);
     mbar_init(&m.s_ready, 4);
-    mbar_init(&m.oi_full, 1);
+    mbar_init(&m.s_free, 1);
     fence_mbar_init();
   }
   if (FULL) {  // the zero tile, and P's tiles: what lies above the diagonal is never written
     if (!WIDE)
       for (int i = tid; i < kBox / 16; i += kThreads) sts16(sb + L::zero + 16 * i, make_uint4(0, 0, 0, 0));
-    for (int i = tid; i < 4 * kBox / 16; i += kThreads) sts16(sb + L::p + 16 * i, make_uint4(0, 0, 0, 0));
+    for (int i = tid; i < (WIDE ? 2 : 4) * kBox / 16; i += kThreads) sts16(sb + L::p + 16 * i, make_uint4(0, 0, 0, 0));
   }
   fence_async_smem();
   tc_fence_before();
@@ -364,15 +388,16 @@ __global__ void __launch_bounds__(kThreads, 1) linear_chunk_kernel(const __grid_
     return static_cast<int>(min(u.len - static_cast<int64_t>(u.first + it) * kC, static_cast<int64_t>(kC)));
   };
 
-  if (warp >= kLoadWarp) {
+  if (warp >= kSumWarp) {
     fewer_registers<kOtherRegs>();
     if (warp == kLoadWarp && lane == 0) {
       // ---- loads ----------------------------------------------------------------
       const int boxes = (FULL ? 2 : 1) * NK + (two ? 2 : 1);
       int issued = 0;
-      for (int it = 0; it < n_chunks; ++it) {
-        const int st = it % kStages, t = (u.first + it) * kC;
-        if (it >= kStages && !mbar_wait(&m.empty[st], (it / kStages - 1) & 1)) {
+      Ring<kStages> ring;
+      for (int it = 0; it < n_chunks; ++it, ring.next()) {
+        const int st = ring.st, t = (u.first + it) * kC;
+        if (it >= kStages && !mbar_wait(&m.empty[st], ring.ph ^ 1)) {
           bad = true;
           break;
         }
@@ -392,25 +417,26 @@ __global__ void __launch_bounds__(kThreads, 1) linear_chunk_kernel(const __grid_
       // ---- products that need nothing of the state before --------------------------
       // The whole warp runs this, one lane issues: addresses stay in uniform registers.
       // (Two warps for the products: with one, its waits and issue were the longest path.)
+      Ring<kStages> ring;
       auto scores = [&](int it) {  // D
-        const int st = it % kStages;
-        if (!mbar_wait(&m.full[st], (it / kStages) & 1)) return false;
-        if (it > 0 && !mbar_wait(&m.d_free, (it - 1) & 1)) return false;
+        const int st = ring.st;
+        if (!mbar_wait(&m.full[st], ring.ph)) return false;
+        if (it >= 2 && !mbar_wait(&m.op_free[it & 1], ((it >> 1) - 1) & 1)) return false;
         tc_fence_after();
         const uint32_t qd = desc_lo(sb + L::q + st * NK * kBox, 0), kd = desc_lo(sb + L::k + st * NK * kBox, 0);
         if (elect_one()) {
 #pragma unroll
           for (int kk = 0; kk < 4 * NK; ++kk) {
             const uint32_t off = ((kk >> 2) * kBox + (kk & 3) * 32u) >> 4;
-            umma_f16(tm + C::d, desc_of(qd + off), desc_of(kd + off), idesc_bf16(64, 64, false, false), kk > 0);
+            umma_f16(tm + C::x + 64 * (it & 1), desc_of(qd + off), desc_of(kd + off), idesc_bf16(64, 64, false, false), kk > 0);
           }
-          umma_commit(&m.d_full);
+          umma_commit(&m.d_full[it & 1]);
         }
         __syncwarp();
         return true;
       };
       auto state = [&](int it) {  // dS^T
-        const int st = it % kStages, wb = it % C::wv_bufs, db = it % C::ds_bufs;
+        const int st = ring.st, wb = it % C::wv_bufs, db = it % C::ds_bufs;
         const uint32_t kd = desc_lo(sb + L::k + st * NK * kBox, kBox);
         if (it >= C::ds_bufs && !mbar_wait(&m.ds_free[db], (it / C::ds_bufs - 1) & 1)) return false;
 #pragma unroll 1
@@ -435,45 +461,45 @@ __global__ void __launch_bounds__(kThreads, 1) linear_chunk_kernel(const __grid_
       };
       bool ok = true;
 #pragma unroll 1
-      for (int it = 0; it < n_chunks && ok; ++it) ok = (!FULL || scores(it)) && state(it);
+      for (int it = 0; it < n_chunks && ok; ++it, ring.next()) ok = (!FULL || scores(it)) && state(it);
       bad = !ok;
     } else if (FULL && warp == kOutMmaWarp) {
       // ---- the output's products ------------------------------------------------------
+      Ring<kStages> ring;
       auto inter = [&](int it) {  // OI^T
-        const int st = it % kStages;
-        if (!mbar_wait(&m.full[st], (it / kStages) & 1)) return false;
+        const int st = ring.st;
+        if (!mbar_wait(&m.full[st], ring.ph)) return false;
         if (!mbar_wait(&m.s_ready, it & 1)) return false;
-        const int ob = it % C::o_bufs;
-        if (it >= C::o_bufs && !mbar_wait(&m.o_free[ob], (it / C::o_bufs - 1) & 1)) return false;
+        if (it > 0 && !mbar_wait(&m.oi_free, (it - 1) & 1)) return false;
         tc_fence_after();
         const uint32_t qd = desc_lo(sb + L::q + st * NK * kBox, 0);
         if (elect_one()) {
 #pragma unroll
           for (int kk = 0; kk < 4 * NK; ++kk)
-            umma_ts(tm + C::oi + 64 * ob, tm + C::s + 8 * kk, desc_of(qd + (((kk >> 2) * kBox + (kk & 3) * 32u) >> 4)),
+            umma_ts(tm + C::oi, tm + C::s + 8 * kk, desc_of(qd + (((kk >> 2) * kBox + (kk & 3) * 32u) >> 4)),
                     idesc_bf16(128, 64, false, false), kk > 0);
-          umma_commit(&m.oi_full);
+          umma_commit(&m.s_free);
         }
         __syncwarp();
         return true;
       };
       auto within = [&](int it) {  // OP^T
-        const int st = it % kStages;
+        const int st = ring.st;
         if (!mbar_wait(&m.p_ready[it & 1], (it >> 1) & 1)) return false;
         tc_fence_after();
         // Wide: both tiles of v. Head x of a pair: its tile and the zero tile, in the order of the blocks.
-        const uint32_t step = (WIDE ? 2 : 1) * (st + 1) * kBox;
+        const uint32_t step = WIDE ? kBox : (st + 1) * kBox;
         const uint32_t v0 = desc_lo(sb + L::va(st), step), v1 = desc_lo(sb + L::zero, step);
-        const uint32_t pd = desc_lo(sb + L::p + 2 * (it & 1) * kBox, 0);
+        const uint32_t pd = desc_lo(sb + L::ptile(it, 0), 0);
         if (elect_one()) {
 #pragma unroll
           for (int kk = 0; kk < 4; ++kk)
-            umma_f16(tm + C::op + 64 * (it % C::o_bufs), desc_of(v0 + (kk * 2048u >> 4)), desc_of(pd + (kk * 32u >> 4)),
+            umma_f16(tm + C::x + 64 * (it & 1), desc_of(v0 + (kk * 2048u >> 4)), desc_of(pd + (kk * 32u >> 4)),
                      idesc_bf16(128, 64, true, false), kk > 0);
           if (!WIDE && u.nheads == 2) {
 #pragma unroll
             for (int kk = 0; kk < 4; ++kk)
-              umma_f16(tm + C::op + 64 * (it % C::o_bufs), desc_of(v1 + (kk * 2048u >> 4)), desc_of(pd + ((kBox + kk * 32u) >> 4)),
+              umma_f16(tm + C::x + 64 * (it & 1), desc_of(v1 + (kk * 2048u >> 4)), desc_of(pd + ((kBox + kk * 32u) >> 4)),
                        idesc_bf16(128, 64, true, false), 1);
           }
           umma_commit(&m.o_full[it & 1]);
@@ -484,69 +510,84 @@ __global__ void __launch_bounds__(kThreads, 1) linear_chunk_kernel(const __grid_
       };
       bool ok = true;
 #pragma unroll 1
-      for (int it = 0; it < n_chunks && ok; ++it) ok = inter(it) && within(it);
+      for (int it = 0; it < n_chunks && ok; ++it, ring.next()) ok = inter(it) && within(it);
       bad = !ok;
     } else if (warp == kSumWarp) {
       // ---- decay sums -------------------------------------------------------------------
-      const float* g = l.decay + u.b * l.sg[0] + u.head0 * l.sg[1];
-      float g0[2] = {}, g1[2] = {}, seg_total[2] = {};
+      // A head has all lanes, or each of two heads half of them; a lane has kT neighbouring tokens.
+      constexpr int kT = WIDE ? 2 : 4, kLanes = kC / kT;
+      const int x = lane / kLanes, tok = lane % kLanes * kT;
+      const bool mine = x < u.nheads;
+      const float* g = l.decay + u.b * l.sg[0] + (u.head0 + (mine ? x : 0)) * l.sg[1];
+      float next[kT], seg_total = 0.f;
       auto load_decays = [&](int it) {
-        const int64_t t = static_cast<int64_t>(u.first + it) * kC + 2 * lane;
+        const int64_t t = static_cast<int64_t>(u.first + it) * kC + tok;
 #pragma unroll
-        for (int x = 0; x < (WIDE ? 1 : 2); ++x) {
-          g0[x] = x < u.nheads && t < u.len ? g[x * l.sg[1] + t * l.sg[2]] : 0.f;
-          g1[x] = x < u.nheads && t + 1 < u.len ? g[x * l.sg[1] + (t + 1) * l.sg[2]] : 0.f;
-        }
+        for (int j = 0; j < kT; ++j) next[j] = mine && t + j < u.len ? g[(t + j) * l.sg[2]] : 0.f;
       };
       load_decays(0);
 #pragma unroll 1
       for (int it = 0; it < n_chunks; ++it) {
         const int sl = it % kSums, live = live_of(it);
-        float x0[2] = {g0[0], g0[1]}, x1[2] = {g1[0], g1[1]};
+        float c[kT], after[kT];
+#pragma unroll
+        for (int j = 0; j < kT; ++j) {
+          const float a = next[j] * kLog2e;
+          c[j] = a < kMinLog2 ? kMinLog2 : a;  // NaN stays
+        }
         if (it + 1 < n_chunks) load_decays(it + 1);
+        // Sums up to each token, and of those after it, without subtracting large sums.
+        after[kT - 1] = 0.f;
+#pragma unroll
+        for (int j = kT - 2; j >= 0; --j) after[j] = after[j + 1] + c[j + 1];
+        float r = after[0] + c[0];
+#pragma unroll
+        for (int j = 1; j < kT; ++j) c[j] += c[j - 1];
+        float f = c[kT - 1];
+#pragma unroll
+        for (int o = 1; o < kLanes; o <<= 1) {
+          const float a = __shfl_up_sync(0xffffffffu, f, o, kLanes), b = __shfl_down_sync(0xffffffffu, r, o, kLanes);
+          if (lane % kLanes >= o) f += a;
+          if (lane % kLanes + o < kLanes) r += b;
+        }
+        float before = __shfl_up_sync(0xffffffffu, f, 1, kLanes), behind = __shfl_down_sync(0xffffffffu, r, 1, kLanes);
+        const float total = __shfl_sync(0xffffffffu, r, 0, kLanes), mid = 0.5f * total;
+        if (lane % kLanes == 0) before = 0.f;
+        if (lane % kLanes == kLanes - 1) behind = 0.f;
+        // e^{c_i - c_j} as a product of two factors, where none leaves 2^+-120.
+        bool near = true;
+#pragma unroll
+        for (int j = 0; j < kT; ++j) {
+          c[j] += before;
+          after[j] += behind;
+          near = near && fabsf(c[j] - mid) <= 120.f;
+        }
+        const uint32_t votes = __ballot_sync(0xffffffffu, near);
+        const bool factors = WIDE ? votes == 0xffffffffu : (votes >> (16 * x) & 0xffffu) == 0xffffu;
         bad |= it >= kSums && !mbar_wait(&m.sums_free[sl], (it / kSums - 1) & 1);
         if (__any_sync(0xffffffffu, bad)) {
           bad = true;
           break;
         }
 #pragma unroll
-        for (int x = 0; x < (WIDE ? 1 : 2); ++x) {
-          if (x == u.nheads) break;
-          float a0 = x0[x] * kLog2e, a1 = x1[x] * kLog2e;
-          a0 = a0 < kMinLog2 ? kMinLog2 : a0, a1 = a1 < kMinLog2 ? kMinLog2 : a1;  // NaN stays
-          float f = a0 + a1, r = f;
-#pragma unroll
-          for (int o = 1; o < 32; o <<= 1) {
-            const float a = __shfl_up_sync(0xffffffffu, f, o), b = __shfl_down_sync(0xffffffffu, r, o);
-            if (lane >= o) f += a;
-            if (lane + o < 32) r += b;
-          }
-          // Before / after this pair, without subtracting large sums.
-          float before = __shfl_up_sync(0xffffffffu, f, 1), after = __shfl_down_sync(0xffffffffu, r, 1);
-          if (lane == 0) before = 0.f;
-          if (lane == 31) after = 0.f;
-          const float c0 = before + a0, c1 = c0 + a1;
-          const float hi = warp_max(fmaxf(c0, c1)), lo = -warp_max(-fminf(c0, c1));
-          // e^{c_i - c_j} as a product of two factors within 2^+-120 of 1, where c spans no more.
-          const bool factors = hi - lo <= 240.f;
-          const float mid = 0.5f * (hi + lo);
-          auto put = [&](float* to, float a, float b) { *reinterpret_cast<float2*>(to + 2 * lane) = make_float2(a, b); };
+        for (int j = 0; j < kT; j += 2) {
+          auto put = [&](float* to, float a, float b) { *reinterpret_cast<float2*>(to + tok + j) = make_float2(a, b); };
+          const float c0 = c[j], c1 = c[j + 1];
           put(m.row[sl][x], factors ? l.scale * ex2_approx(c0 - mid) : c0, factors ? l.scale * ex2_approx(c1 - mid) : c1);
           put(m.col[sl][x], factors ? ex2_approx(mid - c0) : -c0, factors ? ex2_approx(mid - c1) : -c1);
           put(m.ecs[sl][x], l.scale * ex2_approx(c0), l.scale * ex2_approx(c1));
-          put(m.w[sl][x], 2 * lane < live ? ex2_approx(after + a1) : 0.f, 2 * lane + 1 < live ? ex2_approx(after) : 0.f);
-          if (lane == 0) {
-            m.total[sl][x] = ex2_approx(r);
-            m.factors[sl][x] = factors;
-          }
-          seg_total[x] += r;
+          put(m.w[sl][x], tok + j < live ? ex2_approx(after[j]) : 0.f, tok + j + 1 < live ? ex2_approx(after[j + 1]) : 0.f);
         }
+        if (lane % kLanes == 0) {
+          m.total[sl][x] = ex2_approx(total);
+          m.factors[sl][x] = factors;
+        }
+        seg_total += total;
         __syncwarp();
         if (lane == 0) mbar_arrive(&m.sums[sl]);
       }
-      if (!FULL && lane == 0 && !bad)
-        for (int x = 0; x < u.nheads; ++x)
-          p.seg_decay[(static_cast<int64_t>(u.b) * l.H + u.head0 + x) * p.segs + u.seg] = seg_total[x];
+      if (!FULL && mine && lane % kLanes == 0 && !bad)
+        p.seg_decay[(static_cast<int64_t>(u.b) * l.H + u.head0 + x) * p.segs + u.seg] = seg_total;
     }
     __syncwarp();
   } else if (warp >= kOutWarp) {
@@ -570,21 +611,28 @@ __global__ void __launch_bounds__(kThreads, 1) linear_chunk_kernel(const __grid_
         if (lane == 0) tma_store_wait_read();
         __syncwarp();
         const float* ecs = &m.ecs[sl][hd < u.nheads ? hd : 0][32 * half + 2 * (lane & 3)];
-        const uint32_t from = tm + C::oi + 64 * (it % C::o_bufs) + 32 * half + tl;
+        const uint32_t from = tm + 32 * half + tl;
         const int live = live_of(it);
-#pragma unroll 2
-        for (int i = 0; i < 4; ++i) {  // 16 lanes (sub) x 16 tokens
+        // All of q S first, whose columns the next chunk waits for: [16 tokens][16 lanes].
+        float oi[4][8];
+#pragma unroll
+        for (int i = 0; i < 4; ++i) tmem_ld_frag2(from + C::oi + 16 * (i >> 1) + (16u * (i & 1) << 16), oi[i]);
+        tmem_wait_ld();
+        tc_fence_before();
+        __syncwarp();
+        if (lane == 0) mbar_arrive(&m.oi_free);
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
           const int x = i >> 1, sub = i & 1;
-          float oi[8], op[8];
-          tmem_ld_frag2(from + 16 * x + (16u * sub << 16), oi);
-          tmem_ld_frag2(from + (C::op - C::oi) + 16 * x + (16u * sub << 16), op);
+          float op[8];
+          tmem_ld_frag2(from + C::x + 64 * (it & 1) + 16 * x + (16u * sub << 16), op);
           const float2 e[2] = {*reinterpret_cast<const float2*>(ecs + 16 * x),
                                *reinterpret_cast<const float2*>(ecs + 16 * x + 8)};
           tmem_wait_ld();
           uint32_t o[4];  // [token group y][row group]: tokens 8 y + 2 (lane % 4) + {0, 1}
 #pragma unroll
           for (int j = 0; j < 4; ++j) {
-            const float2 y = fma2(make_float2(oi[2 * j], oi[2 * j + 1]), e[j >> 1], make_float2(op[2 * j], op[2 * j + 1]));
+            const float2 y = fma2(make_float2(oi[i][2 * j], oi[i][2 * j + 1]), e[j >> 1], make_float2(op[2 * j], op[2 * j + 1]));
             o[j] = pack_bf16x2(y.x, y.y);
           }
           if (live < kC) {  // rows past the length are zero
@@ -602,7 +650,7 @@ __global__ void __launch_bounds__(kThreads, 1) linear_chunk_kernel(const __grid_
         fence_async_smem();
         __syncwarp();
         if (lane == 0) {
-          mbar_arrive(&m.o_free[it % C::o_bufs]);
+          mbar_arrive(&m.op_free[it & 1]);
           mbar_arrive(&m.sums_free[sl]);
           if (stores && t0 < l.T) tma_store_4d(&p.tm_o, stage, ocol, head, t0, u.b);
         }
@@ -627,11 +675,12 @@ __global__ void __launch_bounds__(kThreads, 1) linear_chunk_kernel(const __grid_
         const int left = i0 + 8 * (j & 1) - (j0 + 16 * (q4 - 2 * half) + 8 * (j >> 1));
         keep[j] = left >= 1 ? 0xffffffffu : left == 0 ? 0xffffu : 0u;
       }
-      for (int it = 0; it < n_chunks; ++it) {
+      Ring<kStages> ring;
+      for (int it = 0; it < n_chunks; ++it, ring.next()) {
         const int sl = it % kSums;
         bad |= !mbar_wait(&m.sums[sl], (it / kSums) & 1);
         bad |= it >= 2 && !mbar_wait(&m.o_full[it & 1], ((it >> 1) - 1) & 1);  // P's tiles have been read
-        bad |= !mbar_wait(&m.d_full, it & 1);
+        bad |= !mbar_wait(&m.d_full[it & 1], (it >> 1) & 1);
         tc_fence_after();
         if (__any_sync(0xffffffffu, bad)) {
           bad = true;
@@ -639,14 +688,14 @@ __global__ void __launch_bounds__(kThreads, 1) linear_chunk_kernel(const __grid_
         }
         const int live = live_of(it);
         if (live < kC) {  // as the prepared values: rows past the length are zero before v is an operand
-          const int st = it % kStages, vecs = (kC - live) * 8;
+          const int st = ring.st, vecs = (kC - live) * 8;
           for (int i = tid - 32 * kScoreWarp; i < (WIDE || u.nheads == 2 ? 2 : 1) * vecs; i += 256)
             sts16(sb + (i < vecs ? L::va(st) : L::vb(st)) + live * 128 + 16 * (i % vecs), make_uint4(0, 0, 0, 0));
         }
 #pragma unroll 1
         for (int z = 0; z < steps; ++z) {
           float d[8];
-          tmem_ld_frag2(tm + C::d + 32 * half + 16 * z + tl, d);
+          tmem_ld_frag2(tm + C::x + 64 * (it & 1) + 32 * half + 16 * z + tl, d);
           tmem_wait_ld();
           const bool diagonal = 2 * half + z == q4;
 #pragma unroll 1
@@ -672,7 +721,7 @@ __global__ void __launch_bounds__(kThreads, 1) linear_chunk_kernel(const __grid_
 #pragma unroll
               for (int j = 0; j < 4; ++j) o[j] &= keep[j];
             }
-            const uint32_t ps = sb + L::p + (2 * (it & 1) + x) * kBox + i0 * 128u + 4 * (lane & 3);
+            const uint32_t ps = sb + L::ptile(it, x) + i0 * 128u + 4 * (lane & 3);
 #pragma unroll
             for (int y = 0; y < 2; ++y) {
               const uint32_t to = ps + (((4 * half + 2 * z + y) ^ (lane >> 2)) << 4);
@@ -682,8 +731,6 @@ __global__ void __launch_bounds__(kThreads, 1) linear_chunk_kernel(const __grid_
           }
         }
         tc_fence_before();
-        __syncwarp();
-        if (lane == 0) mbar_arrive(&m.d_free);
         fence_async_smem();
         __syncwarp();
         if (lane == 0) mbar_arrive(&m.p_ready[it & 1]);
@@ -700,9 +747,10 @@ __global__ void __launch_bounds__(kThreads, 1) linear_chunk_kernel(const __grid_
       const uint32_t z[16] = {};
       for (int i = 0; i < 3 * C::wv_bufs; ++i) tmem_st16(tm + C::wv + 32 * i + 16 * half + tl, z);
     }
-    for (int it = 0; it < n_chunks; ++it) {
-      const int st = it % kStages, sl = it % kSums, live = live_of(it), wb = it % C::wv_bufs;
-      bad |= !mbar_wait(&m.full[st], (it / kStages) & 1);
+    Ring<kStages> ring;
+    for (int it = 0; it < n_chunks; ++it, ring.next()) {
+      const int st = ring.st, sl = it % kSums, live = live_of(it), wb = it % C::wv_bufs;
+      bad |= !mbar_wait(&m.full[st], ring.ph);
       bad |= !mbar_wait(&m.sums[sl], (it / kSums) & 1);
       if (live < kC) {
         // Rows past the length hold anything: as operands they must be zero. (The scores may
@@ -828,7 +876,7 @@ __global__ void __launch_bounds__(kThreads, 1) linear_chunk_kernel(const __grid_
         mbar_arrive(&m.sums_free[sl]);
       }
       if (FULL && it + 1 < n_chunks) {
-        bad |= !mbar_wait(&m.oi_full, it & 1);  // the operand has been read
+        bad |= !mbar_wait(&m.s_free, it & 1);  // the operand has been read
         tc_fence_after();
         if (__any_sync(0xffffffffu, bad)) {
           bad = true;
@@ -970,7 +1018,7 @@ bool plan_of(int B, int T, int H, int Hq, int N, int P, int dtype, Plan& x) {
 template <int NK, bool WIDE, bool FULL>
 void launch_chunks(const ChunkParams& p, unsigned grid, cudaStream_t stream) {
   auto kernel = linear_chunk_kernel<NK, WIDE, FULL>;
-  constexpr int bytes = smem_bytes<NK>();
+  constexpr int bytes = Layout<NK, WIDE, FULL>::bytes;
   static std::atomic<uint64_t> ready{0};  // devices on which the kernel has its shared memory size
   int dev = 0;
   cudaGetDevice(&dev);
