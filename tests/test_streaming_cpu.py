@@ -142,3 +142,18 @@ def test_c_abi_validates_on_the_host():
     assert attention(b=0) == attention(h=0, hq=1) == attention(t=0) == _lib.TF_OK
     assert attention(state=ctypes.c_void_p(4100)) == _lib.TF_ERR_LAYOUT
     assert attention(strides=_lib.int64_array([8] * 15 + [6, 8])) == _lib.TF_ERR_LAYOUT
+
+
+@pytest.mark.parametrize("first", ["linear_attention_step", "linear_attention", "apply_rotary", "linear_recurrence"])
+def test_exports_do_not_depend_on_the_order_of_imports(first):
+    """No export shares its name with a module of the package, which would take its place."""
+    import subprocess
+    import sys
+    from pathlib import Path
+
+    root = Path(__file__).resolve().parent.parent / "trifusion-fp-kernel_b200"
+    code = (f"import sys; sys.path.insert(0, {str(root)!r}); import trifusion_b200 as t; "
+            f"exec('import trifusion_b200.{first}') if {first!r} == 'linear_recurrence' else getattr(t, {first!r}); "
+            "assert all(callable(getattr(t, n)) for n in ('linear_attention', 'linear_attention_step', "
+            "'apply_rotary', 'rotary_frequencies'))")
+    subprocess.run([sys.executable, "-c", code], check=True)

@@ -19,8 +19,8 @@ _EXPORTS = {
     "check_device_error": ("._lib", "check_device_error"),
     "rotary_frequencies": (".rotary", "rotary_frequencies"),
     "apply_rotary": (".rotary", "apply_rotary"),
-    "linear_attention": (".linear_attention", "linear_attention"),
-    "linear_attention_step": (".linear_attention", "linear_attention_step"),
+    "linear_attention": (".linear_recurrence", "linear_attention"),
+    "linear_attention_step": (".linear_recurrence", "linear_attention_step"),
 }
 
 

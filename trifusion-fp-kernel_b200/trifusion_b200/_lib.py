@@ -197,12 +197,7 @@ def require_cuda(op, *tensors):
     return dev
 
 
-def no_gradient(op, *tensors):
-    """Refuse operands that autograd would expect a gradient for (there is no backward pass)."""
-    import torch
-
-    if torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in tensors):
-        raise RuntimeError(f"{op}: no backward pass; detach the operands or call it under torch.no_grad()")
+NO_GRADIENT = "no backward pass; detach the operands or call it under torch.no_grad()"
 
 
 def launch(fn, device, *args):
@@ -212,6 +207,34 @@ def launch(fn, device, *args):
     with torch.cuda.device(device):
         stream = torch.cuda.current_stream(device).cuda_stream
         check(getattr(lib(), fn)(*args, stream))
+
+
+def launcher(fn):
+    """As :func:`launch` for one entry point, for operators whose kernels are shorter than the
+    host's work around them: ``launcher(fn)(device_index, *args)`` changes the current device
+    only where it has to and asks for the stream's handle alone."""
+    import torch
+
+    raw_stream = getattr(torch._C, "_cuda_getCurrentRawStream", None)
+    if raw_stream is None:
+        def raw_stream(index):
+            return torch.cuda.current_stream(index).cuda_stream
+    current = torch.cuda.current_device
+    call = None
+
+    def run(index, *args):
+        nonlocal call
+        if call is None:
+            call = getattr(lib(), fn)
+        if current() == index:
+            status = call(*args, raw_stream(index))
+        else:
+            with torch.cuda.device(index):
+                status = call(*args, raw_stream(index))
+        if status != TF_OK:
+            check(status)
+
+    return run
 
 
 _workspaces = {}

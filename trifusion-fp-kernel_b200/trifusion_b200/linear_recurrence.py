@@ -1,0 +1,208 @@
+"""Linear attention with a decay for each head and a carried state.
+
+    S_t = e^(decay_t) S_(t-1) + k_t v_t^T          (N x P, FP32)
+    o_t = scale * q_t S_t
+
+``fused_mamba`` and ``fused_recurrence`` run a whole padded clip from a zero state.
+These two run a causal recurrence of the same chunked kind over a stream:
+``linear_attention`` a piece of any length (a prompt), ``linear_attention_step`` one
+token for each row, both from and into states that the caller keeps, as one
+tensor or as a pool with a slot for each row.
+"""
+
+from __future__ import annotations
+
+import functools
+import struct
+
+import torch
+
+from . import _lib
+
+_launch = _lib.launcher("tf_linear_attention_fwd")
+_pack = struct.Struct("17q").pack
+_DTYPES = {torch.float32: _lib.TF_F32, torch.bfloat16: _lib.TF_BF16}
+
+
+def _operands(op, dtype, q, k, v, decay, hq, h, n, p):
+    """What both forms ask of their operands, shapes apart; returns the C ABI's dtype."""
+    if hq < 1 or h % hq:
+        raise ValueError(f"{op}: H must be divisible by Hq")
+    if n % 8 or p % 8 or n < 8 or p < 8 or n > 256 or p > 256:
+        raise ValueError(f"{op}: N and P must be multiples of 8 from 8 to 256")
+    code = _DTYPES.get(dtype)
+    if code is None:
+        raise TypeError(f"{op}: expected float32 or bfloat16, got {dtype}")
+    if k.dtype != dtype or v.dtype != dtype:
+        raise TypeError(f"{op}: q, k and v must have one dtype")
+    if decay.dtype != torch.float32:
+        raise TypeError(f"{op}: decay must be float32")
+    if (q.requires_grad or k.requires_grad or v.requires_grad or decay.requires_grad) and torch.is_grad_enabled():
+        raise RuntimeError(f"{op}: {_lib.NO_GRADIENT}")
+    return code
+
+
+def _check_state(op, state, slots, b, h, n, p):
+    """Checks a state and its slots; returns the state's strides over slots and heads."""
+    if state.dtype != torch.float32 or state.dim() != 4 or tuple(state.shape[1:]) != (h, n, p):
+        raise ValueError(f"{op}: state must be float32 [slots,H,N,P]")
+    s0, s1, s2, s3 = state.stride()
+    if s3 != 1 or s2 != p or s0 % 4 or s1 % 4 or state.data_ptr() % 16:
+        raise ValueError(f"{op}: state must be contiguous over [N,P], its heads on 16-byte boundaries")
+    if (s1 < n * p and h > 1) or (s0 < n * p and state.shape[0] > 1):
+        raise ValueError(f"{op}: the states of a pool must not overlap")
+    if slots is None:
+        if state.shape[0] != b:
+            raise ValueError(f"{op}: without slots, state must have one entry for each row")
+    elif slots.dtype != torch.int64 or tuple(slots.shape) != (b,):
+        raise ValueError(f"{op}: slots must be int64 [B]")
+    return s0, s1
+
+
+def _check_out(op, out, v):
+    if out.shape != v.shape or out.dtype != v.dtype or out.stride(-1) != 1:
+        raise ValueError(f"{op}: out must be like v with a unit stride in the last dimension")
+
+
+def _check_device(op, index, *tensors):
+    if index < 0 or any(t is not None and t.get_device() != index for t in tensors):
+        raise RuntimeError(f"{op}: all tensors must be CUDA tensors on one device")
+
+
+def _aligned(x):
+    """Whether tile loads and stores can address ``x`` ([B,T,heads,width] BF16)."""
+    if x.data_ptr() % 16:
+        return False
+    (b, t, h, _), (sb, st, sh, _) = x.shape, x.stride()
+    return not ((b > 1 and (sb % 8 or sb <= 0)) or (t > 1 and (st % 8 or st <= 0)) or (h > 1 and (sh % 8 or sh <= 0)))
+
+
+@functools.lru_cache(maxsize=1024)
+def _workspace_size(*sizes):
+    return _lib.lib().tf_linear_attention_workspace_size(*sizes)
+
+
+def linear_attention(q, k, v, decay, state=None, *, slots=None, lengths=None, scale=None, out=None):
+    """A piece of T tokens for each row: returns ``(out, state)``.
+
+    * ``q``, ``k`` [B,T,Hq,N], ``v`` [B,T,H,P], BF16 or FP32, H a multiple of Hq, N and P
+      multiples of 8 up to 256; ``decay`` FP32 [B,H,T], or [H] for one decay a head: natural
+      logs, at most 0 in use; ``-inf`` forgets everything before.
+    * ``state`` FP32 [B,H,N,P] is the state before the first token and is overwritten by
+      the state after the last. With ``slots`` (int64 [B]) it is a pool [slots,H,N,P] and row
+      b works on entry ``slots[b]``. A row with a negative slot is padding: its output is
+      zero and no state changes. A slot past the pool, or one that an earlier row has, gives
+      NaN outputs and changes no state. ``None``: rows start at zero and a new [B,H,N,P] is
+      returned.
+    * ``lengths`` (int64 [B], on the device): tokens at or past a row's length are not
+      read, and their output is zero.
+    * ``scale`` defaults to ``N ** -0.5``; ``out``: a preallocated output like v with a unit
+      stride in the last dimension.
+
+    BF16 operands with N and P up to 128 run on the tensor cores in chunks of 64 tokens
+    (FP32 sums and state); a non-finite value in v or k then also reaches the earlier
+    tokens of its chunk. FP32 operands, wider heads and short pieces run token by token.
+    There is no backward pass.
+    """
+    op = "linear_attention"
+    shape = q.shape
+    if len(shape) != 4 or v.dim() != 4 or k.shape != shape:
+        raise ValueError(f"{op}: q and k must be [B,T,Hq,N] and v [B,T,H,P]")
+    b, t, hq, n = shape
+    vb, vt, h, p = v.shape
+    if vb != b or vt != t:
+        raise ValueError(f"{op}: q and k must be [B,T,Hq,N] and v [B,T,H,P]")
+    dtype, index = _operands(op, q.dtype, q, k, v, decay, hq, h, n, p), q.get_device()
+    sg, shape = decay.stride(), tuple(decay.shape)
+    if shape == (h,) and sg:
+        sg = (0, sg[0], 0)
+    elif shape != (b, h, t):
+        raise ValueError(f"{op}: decay must be [B,H,T] or [H]")
+    fresh = state is None
+    if not fresh:
+        ss = _check_state(op, state, slots, b, h, n, p)
+    elif slots is not None:
+        raise ValueError(f"{op}: slots need a state")
+    if lengths is not None and (lengths.dtype != torch.int64 or tuple(lengths.shape) != (b,)):
+        raise ValueError(f"{op}: lengths must be int64 [B]")
+    if out is not None:
+        _check_out(op, out, v)
+    _check_device(op, index, k, v, decay, state, slots, lengths, out)
+    q, k, v = [x if x.stride(3) == 1 else x.contiguous() for x in (q, k, v)]
+    if slots is not None:
+        slots = slots.contiguous()
+    if lengths is not None:
+        lengths = lengths.contiguous()
+    if out is None:
+        out = torch.empty_like(v, memory_format=torch.contiguous_format)
+    if fresh:
+        state = torch.empty((b, h, n, p), dtype=torch.float32, device=v.device)
+        ss = (h * n * p, n * p)
+    _lib.error_watch()
+    _lib.check_device_error()
+    nbytes = _workspace_size(b, t, h, hq, n, p, dtype)
+    work, into = None, out
+    if nbytes:  # the chunked form, whose tile loads need 16-byte rows
+        q, k, v = [x if _aligned(x) else x.clone(memory_format=torch.contiguous_format) for x in (q, k, v)]
+        if not _aligned(out):
+            into = torch.empty((b, t, h, p), dtype=v.dtype, device=v.device)
+        work = torch.empty(nbytes, dtype=torch.uint8, device=v.device)
+    _launch(index, q.data_ptr(), k.data_ptr(), v.data_ptr(), dtype, decay.data_ptr(), state.data_ptr(), state.shape[0],
+            fresh, None if slots is None else slots.data_ptr(), None if lengths is None else lengths.data_ptr(),
+            into.data_ptr(), _pack(*q.stride()[:3], *k.stride()[:3], *v.stride()[:3], *sg, *into.stride()[:3], *ss),
+            b, t, h, hq, n, p, n ** -0.5 if scale is None else scale, None if work is None else work.data_ptr(), nbytes)
+    if into is not out:
+        out.copy_(into)
+    return out, state
+
+
+def linear_attention_step(q, k, v, decay, state, *, slots=None, scale=None, out=None):
+    """One token for each row: returns the output [B,H,P] and updates ``state`` in place.
+
+    ``q``, ``k`` [B,Hq,N], ``v`` [B,H,P], BF16 or FP32; ``decay`` FP32 [B,H] or [H]; ``state``,
+    ``slots``, ``scale`` and ``out`` as in :func:`linear_attention` (a batch padded for a
+    captured graph gives its padding rows the slot -1).
+    """
+    op = "linear_attention_step"
+    shape = q.shape
+    if len(shape) != 3 or v.dim() != 3 or k.shape != shape:
+        raise ValueError(f"{op}: q and k must be [B,Hq,N] and v [B,H,P]")
+    b, hq, n = shape
+    vb, h, p = v.shape
+    if vb != b:
+        raise ValueError(f"{op}: q and k must be [B,Hq,N] and v [B,H,P]")
+    dtype, index = _operands(op, q.dtype, q, k, v, decay, hq, h, n, p), q.get_device()
+    sg, shape = decay.stride(), tuple(decay.shape)
+    if shape == (h,) and sg:
+        sg = (0, sg[0])
+    elif shape != (b, h):
+        raise ValueError(f"{op}: decay must be [B,H] or [H]")
+    ss = _check_state(op, state, slots, b, h, n, p)
+    if out is not None:
+        _check_out(op, out, v)
+    _check_device(op, index, k, v, decay, state, slots, out)
+    qb, qh, q1 = q.stride()
+    kb, kh, k1 = k.stride()
+    vb, vh, v1 = v.stride()
+    if q1 != 1:
+        q = q.contiguous()
+        qb, qh, _ = q.stride()
+    if k1 != 1:
+        k = k.contiguous()
+        kb, kh, _ = k.stride()
+    if v1 != 1:
+        v = v.contiguous()
+        vb, vh, _ = v.stride()
+    slot = None
+    if slots is not None:
+        slots = slots.contiguous()
+        slot = slots.data_ptr()
+    if out is None:
+        out, ob, oh = torch.empty_like(v, memory_format=torch.contiguous_format), h * p, p
+    else:
+        ob, oh, _ = out.stride()
+    _launch(index, q.data_ptr(), k.data_ptr(), v.data_ptr(), dtype, decay.data_ptr(), state.data_ptr(), state.shape[0],
+            0, slot, None, out.data_ptr(),
+            _pack(qb, 0, qh, kb, 0, kh, vb, 0, vh, *sg, 0, ob, 0, oh, *ss), b, 1, h, hq, n, p,
+            n ** -0.5 if scale is None else scale, None, 0)
+    return out

@@ -11,12 +11,16 @@ rounding to the tensors' type.
 from __future__ import annotations
 
 import math
+import struct
 
 import torch
 
 from . import _lib
 
-_LAYOUTS = ("half", "interleaved")
+_DTYPES = {torch.float32: _lib.TF_F32, torch.bfloat16: _lib.TF_BF16}
+_LAYOUTS = {"half": 0, "interleaved": 1}
+_launch = _lib.launcher("tf_rotary_positions_fwd")
+_pack = struct.Struct("14q").pack
 
 
 def rotary_frequencies(rotary_dim, base=10000.0, *, scaling=None, factor=1.0, trained_length=None,
@@ -65,39 +69,61 @@ def apply_rotary(q, k, positions, inv_freq, *, layout="half", amplitude=1.0, inp
     x2 sin, x2 cos + x1 sin)``. q and k are FP32 or BF16 with any strides, the last one 1.
     Returns new contiguous tensors, or the arguments themselves when ``inplace``.
     """
-    if layout not in _LAYOUTS:
+    interleaved = _LAYOUTS.get(layout)
+    if interleaved is None:
         raise ValueError(f"apply_rotary: layout must be 'half' or 'interleaved', got {layout!r}")
-    if q.dim() != 4 or (k is not None and (k.dim() != 4 or k.shape[:2] != q.shape[:2] or k.shape[3] != q.shape[3])):
+    shape = q.shape
+    if len(shape) != 4:
         raise ValueError("apply_rotary: q must be [B,T,H,D] and k [B,T,Hk,D]")
-    if k is not None and k.dtype != q.dtype:
-        raise TypeError("apply_rotary: q and k must have one dtype")
-    dtype = _lib.dtype_code(q, "apply_rotary")
-    if inv_freq.dtype != torch.float64 or inv_freq.dim() != 1 or not 2 <= 2 * inv_freq.shape[0] <= q.shape[3]:
+    b, t, h, d = shape
+    dtype, index = _DTYPES.get(q.dtype), q.get_device()
+    if dtype is None:
+        raise TypeError(f"apply_rotary: expected float32 or bfloat16, got {q.dtype}")
+    if k is None:
+        hk, same, grad = 0, True, q.requires_grad
+    else:
+        kb, kt, hk, kd = k.shape if k.dim() == 4 else (-1,) * 4
+        if kb != b or kt != t or kd != d:
+            raise ValueError("apply_rotary: q must be [B,T,H,D] and k [B,T,Hk,D]")
+        if k.dtype != q.dtype:
+            raise TypeError("apply_rotary: q and k must have one dtype")
+        same, grad = k.get_device() == index, q.requires_grad or k.requires_grad
+    half = inv_freq.numel()
+    if inv_freq.dtype != torch.float64 or inv_freq.dim() != 1 or not 2 <= 2 * half <= d:
         raise ValueError("apply_rotary: inv_freq must be float64 [R/2] with 2 <= R <= D")
-    b, t, h, d = q.shape
     if positions.dtype != torch.int64 or tuple(positions.shape) not in ((b, t), (t,)):
         raise ValueError("apply_rotary: positions must be int64 [B,T] or [T]")
-    _lib.no_gradient("apply_rotary", q, k)
-    dev = _lib.require_cuda("apply_rotary", q, q if k is None else k, positions, inv_freq)
+    if grad and torch.is_grad_enabled():
+        raise RuntimeError("apply_rotary: " + _lib.NO_GRADIENT)
+    if index < 0 or not same or positions.get_device() != index or inv_freq.get_device() != index:
+        raise RuntimeError("apply_rotary: all tensors must be CUDA tensors on one device")
+    if not inv_freq.is_contiguous():
+        inv_freq = inv_freq.contiguous()
+    q0, q1, q2, q3 = q.stride()
+    k0 = k1 = k2 = o0 = o1 = o2 = 0
+    k3, kp, kop = 1, None, None
+    if k is not None:
+        k0, k1, k2, k3 = k.stride()
     if inplace:
-        if q.stride(3) != 1 or (k is not None and k.stride(3) != 1):
+        if q3 != 1 or k3 != 1:
             raise ValueError("apply_rotary: in place needs a unit stride in the last dimension")
-        qo, ko = q, k
+        qo, ko, p0, p1, p2, o0, o1, o2 = q, k, q0, q1, q2, k0, k1, k2
     else:
-        q = q if q.stride(3) == 1 else q.contiguous()
-        qo = torch.empty((b, t, h, d), dtype=q.dtype, device=dev)
+        if q3 != 1:
+            q = q.contiguous()
+            q0, q1, q2, _ = q.stride()
+        qo = torch.empty_like(q, memory_format=torch.contiguous_format)
+        p0, p1, p2, ko = t * h * d, h * d, d, None
         if k is not None:
-            k = k if k.stride(3) == 1 else k.contiguous()
-            ko = torch.empty(k.shape, dtype=k.dtype, device=dev)
-        else:
-            ko = None
-    inv_freq = inv_freq.contiguous()
-    none = (0, 0, 0)
-    strides = _lib.int64_array((*q.stride()[:3], *(none if k is None else k.stride()[:3]), *qo.stride()[:3],
-                                *(none if k is None else ko.stride()[:3]),
-                                *(positions.stride() if positions.dim() == 2 else (0, positions.stride(0)))))
-    _lib.launch("tf_rotary_positions_fwd", dev, q.data_ptr(), None if k is None else k.data_ptr(), qo.data_ptr(),
-                None if k is None else ko.data_ptr(), dtype, positions.data_ptr(), inv_freq.data_ptr(),
-                float(amplitude), 1 if layout == "interleaved" else 0, strides, b, t, h,
-                0 if k is None else k.shape[2], d, 2 * inv_freq.shape[0])
-    return (qo, ko) if k is not None else qo
+            if k3 != 1:
+                k = k.contiguous()
+                k0, k1, k2, _ = k.stride()
+            ko = torch.empty_like(k, memory_format=torch.contiguous_format)
+            o0, o1, o2 = t * hk * d, hk * d, d
+    if k is not None:
+        kp, kop = k.data_ptr(), ko.data_ptr()
+    s = positions.stride()
+    _launch(index, q.data_ptr(), kp, qo.data_ptr(), kop, dtype, positions.data_ptr(), inv_freq.data_ptr(), amplitude,
+            interleaved, _pack(q0, q1, q2, k0, k1, k2, p0, p1, p2, o0, o1, o2, 0 if len(s) == 1 else s[0], s[-1]),
+            b, t, h, hk, d, 2 * half)
+    return qo if k is None else (qo, ko)
