@@ -175,7 +175,8 @@ int tf_linear_attention_fwd(const void* q, const void* k, const void* v, int dty
     return TF_ERR_LAYOUT;
   p.B = batch, p.T = seqlen, p.H = heads, p.Hq = groups, p.N = key_dim, p.P = value_dim;
   p.scale = scale;
-  if (static_cast<int64_t>(batch) * heads * ((value_dim + 31) / 32) > 0x7fffffffll) return TF_ERR_SIZE;
+  if (static_cast<int64_t>(batch) * heads * ((value_dim + 31) / 32) > 0x7fffffffll || seqlen > 0x7fffff00)
+    return TF_ERR_SIZE;
   int st = check_device();
   if (st != TF_OK) return st;
   if (linear_chunk_workspace(batch, seqlen, heads, groups, key_dim, value_dim, dtype) > 0) {

@@ -55,9 +55,14 @@ constexpr int kPrepWarp = 4, kScoreWarp = 12, kOutWarp = 20;  // (state: 0)
 // the last quarter's gets the lightest of the single warps.
 constexpr int kSumWarp = 28, kStateMmaWarp = 29, kOutMmaWarp = 30, kLoadWarp = 31;
 constexpr int kThreads = 32 * 32;
-// Registers of a thread: 32 warps have 64 at launch, 2048 together, and share them out again
-// as 4 * 160 + 8 * 56 + 20 * 48 = 2048.
-constexpr int kStateRegs = 160, kOutRegs = 56, kOtherRegs = 48;
+// Registers of a thread: 32 warps have 64 at launch, 2048 together, and share them out again.
+// The state's four warps hold 64 or 128 values a thread.
+template <int NK>
+struct Regs {
+  static constexpr int state = NK == 1 ? 120 : 168, prep = NK == 1 ? 56 : 48, score = NK == 1 ? 56 : 40,
+                       out = 56, single = 56;
+  static_assert(4 * state + 8 * (prep + score + out) + 4 * single == 2048, "what was launched");
+};
 
 __device__ int g_linear_error = 0;    // 1: a bounded wait gave up
 
@@ -73,8 +78,20 @@ struct ChunkParams {
   int* err_host;
 };
 
+// What a CTA works on. Its warps read it from shared memory where they start: few of them
+// have registers for all of it.
+struct alignas(16) Unit {
+  int b, hk, seg;      // row, k head, segment
+  int head0, nheads;   // v heads: one (wide, or without a partner) or two
+  int len;             // the row's length
+  int first, last;     // its chunks with live tokens
+  int64_t slot;        // of the row's state
+  __device__ __forceinline__ int live(int it) const { return min(len - (first + it) * kC, kC); }  // tokens of a chunk
+  __device__ __forceinline__ bool ends_row() const { return last == (len + kC - 1) / kC; }
+};
 template <int STAGES>
 struct alignas(16) Misc {
+  Unit unit;
   uint64_t full[STAGES], empty[STAGES];      // tiles loaded / every product of them done
   uint64_t sums[kSums], sums_free[kSums];    // decay sums written / read
   uint64_t d_full[2];                        // scores there
@@ -83,6 +100,7 @@ struct alignas(16) Misc {
   uint64_t wv_ready[2][2], wv_free[2][2];    // [buffer][half] weighted values written / read
   uint64_t ds_full[2], ds_free[2];           // state product there / read
   uint64_t s_ready, s_free;                  // state operand written / read
+  uint64_t init_full, init_read;             // the state before the first chunk there / read
   uint32_t tmem;
   alignas(16) float row[kSums][2][kC];  // [chunk][head] two factors of scale e^{c_i - c_j}, or c_i and
   float col[kSums][2][kC];              // -c_j (log2) where a factor would leave FP32's range
@@ -108,6 +126,10 @@ struct Layout {
   static constexpr int p = v + (2 * stages + (zero_tile ? 1 : 0)) * kBox;  // [chunk & 1][head]
   static constexpr int o = p + (FULL ? (WIDE ? 2 : 4) * kBox : 0);         // [warp] 32 tokens x 32 columns
   static constexpr int misc = o + (FULL ? 8 * 2048 : 0);
+  // Two areas of up to 32 KB for states: before the first chunk in the stages after its own,
+  // at the end anywhere.
+  static constexpr int init0 = k + NK * kBox, init1 = q + NK * kBox, last0 = 0, last1 = 32768;
+  static_assert(!FULL || (stages - 1) * NK * kBox >= 16384 * NK, "room for the states");
   static constexpr int bytes = misc + static_cast<int>(sizeof(Misc<stages>)) + 1024;
   static_assert(stages >= 3 && bytes <= 232448, "shared memory of a CTA");
   static __device__ __forceinline__ uint32_t va(int stage) {
@@ -180,6 +202,16 @@ __device__ __forceinline__ void tma_store_4d(const void* tmap, uint32_t src, int
                : "memory");
   asm volatile("cp.async.bulk.commit_group;" ::: "memory");
 }
+__device__ __forceinline__ void bulk_load(uint32_t dst, const void* src, uint32_t bytes, uint64_t* bar) {
+  asm volatile("cp.async.bulk.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1], %2, [%3];" ::"r"(dst),
+               "l"(reinterpret_cast<uint64_t>(src)), "r"(bytes), "r"(smem_u32(bar))
+               : "memory");
+}
+__device__ __forceinline__ void bulk_store(void* dst, uint32_t src, uint32_t bytes) {
+  asm volatile("cp.async.bulk.global.shared::cta.bulk_group [%0], [%1], %2;" ::"l"(reinterpret_cast<uint64_t>(dst)),
+               "r"(src), "r"(bytes)
+               : "memory");
+}
 __device__ __forceinline__ void tma_store_wait_read() { asm volatile("cp.async.bulk.wait_group.read 0;" ::: "memory"); }
 // 16 lanes x 8 columns: thread t gives lanes t/4 and t/4 + 8, column 4 x + t % 4, as r[2 x]
 // and r[2 x + 1].
@@ -196,6 +228,11 @@ __device__ __forceinline__ void tmem_st16(uint32_t taddr, const uint32_t (&r)[16
       "r"(r[0]), "r"(r[1]), "r"(r[2]), "r"(r[3]), "r"(r[4]), "r"(r[5]), "r"(r[6]), "r"(r[7]), "r"(r[8]), "r"(r[9]),
       "r"(r[10]), "r"(r[11]), "r"(r[12]), "r"(r[13]), "r"(r[14]), "r"(r[15])
       : "memory");
+}
+__device__ __forceinline__ void tmem_st8(uint32_t taddr, const uint32_t (&r)[8]) {
+  asm volatile("tcgen05.st.sync.aligned.32x32b.x8.b32 [%0], {%1,%2,%3,%4,%5,%6,%7,%8};" ::"r"(taddr), "r"(r[0]),
+               "r"(r[1]), "r"(r[2]), "r"(r[3]), "r"(r[4]), "r"(r[5]), "r"(r[6]), "r"(r[7])
+               : "memory");
 }
 __device__ __forceinline__ void tmem_wait_st() { asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory"); }
 // 16 TMEM lanes x 16 columns as m16n8 fragments: thread t gets lanes t/4 and t/4 + 8,
@@ -261,13 +298,6 @@ __device__ __forceinline__ uint32_t take_bf16(float2& x) {
   return __byte_perm(a, b, 0x7632);
 }
 
-// What a CTA works on.
-struct Unit {
-  int b, hk, seg;     // row, k head, segment
-  int head0, nheads;  // v heads: one (wide, or without a partner) or two
-  int64_t len;        // the row's length
-  int first, last;    // its chunks with live tokens
-};
 template <bool WIDE>
 __device__ __forceinline__ Unit unit_of(const ChunkParams& p, int x) {
   Unit u;
@@ -282,11 +312,27 @@ __device__ __forceinline__ Unit unit_of(const ChunkParams& p, int x) {
   u.head0 = u.hk * share + (WIDE ? pr : 2 * pr);
   u.nheads = WIDE || 2 * pr + 1 >= share ? 1 : 2;
   u.len = l.T;
-  if (l.lengths) u.len = min(max(l.lengths[u.b], static_cast<int64_t>(0)), static_cast<int64_t>(l.T));
-  const int live = static_cast<int>((u.len + kC - 1) / kC);
+  if (l.lengths) u.len = static_cast<int>(min(max(l.lengths[u.b], static_cast<int64_t>(0)), static_cast<int64_t>(l.T)));
   u.first = u.seg * p.seg_chunks;
-  u.last = min(live, u.first + p.seg_chunks);
+  u.last = min((u.len + kC - 1) / kC, u.first + p.seg_chunks);
+  u.slot = l.slots ? l.slots[u.b] : u.b;
   return u;
+}
+
+// Output rows of a CTA from t0 on, as far as its segment goes: zeros, or `word` before the length.
+__device__ __forceinline__ void fill_rows(const ChunkParams& p, const Unit& u, int t0, int thread, int threads,
+                                       uint32_t word) {
+  const LinearParams& l = p.l;
+  const int t1 = static_cast<int>(min(static_cast<int64_t>(l.T), static_cast<int64_t>(u.first + p.seg_chunks) * kC));
+  if (t0 >= t1) return;
+  const int vecs = u.nheads * l.P / 8, rows = threads / vecs;  // 16-byte vectors of a token; tokens at a time
+  const int c = thread % vecs * 8;
+  bf16* o = static_cast<bf16*>(l.out) + u.b * l.so[0] + (u.head0 + c / l.P) * l.so[2] + c % l.P;
+  if (thread < rows * vecs)
+    for (int64_t t = t0 + thread / vecs; t < t1; t += rows) {
+      const uint32_t x = t < u.len ? word : 0u;
+      *reinterpret_cast<uint4*>(o + t * l.so[1]) = make_uint4(x, x, x, x);
+    }
 }
 
 // FULL: the outputs and the final state; otherwise a segment's own state from zero.
@@ -300,45 +346,8 @@ __global__ void __launch_bounds__(kThreads, 1) linear_chunk_kernel(const __grid_
   Misc<kStages>& m = *reinterpret_cast<Misc<kStages>*>(smem_raw + (sb - smem_u32(smem_raw)) + L::misc);
   const LinearParams& l = p.l;
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
-  const Unit u = unit_of<WIDE>(p, blockIdx.x);
-  const int live_chunks = static_cast<int>((u.len + kC - 1) / kC);
-
-  int64_t slot = 0;
-  bool in_pool = false;
-  if (FULL) {
-    slot = l.slots ? l.slots[u.b] : u.b;
-    in_pool = l.state && slot >= 0 && slot < l.nslots;
-    bool taken = false;  // an earlier row has this slot
-    if (l.slots) {
-      for (int i = tid; i < u.b; i += kThreads) taken |= l.slots[i] == slot;
-      taken = __syncthreads_or(taken);
-    }
-    const bool dead = l.state && (!in_pool || taken);
-    // Rows without a state of their own, and chunks past the length: zeros, or NaN for a wrong slot.
-    const int64_t t0 = dead ? static_cast<int64_t>(u.first) * kC
-                            : max(min(static_cast<int64_t>(live_chunks), static_cast<int64_t>(u.first + p.seg_chunks)),
-                                  static_cast<int64_t>(u.first)) * kC;
-    const int64_t t1 = min(static_cast<int64_t>(l.T), static_cast<int64_t>(u.first + p.seg_chunks) * kC);
-    const uint32_t word = dead && slot >= 0 ? 0x7fc07fc0u : 0u;
-    const int vecs = u.nheads * l.P / 8, rows = kThreads / vecs;  // 16-byte vectors of a token; tokens at a time
-    const int c = tid % vecs * 8;
-    bf16* o = static_cast<bf16*>(l.out) + u.b * l.so[0] + (u.head0 + c / l.P) * l.so[2] + c % l.P;
-    if (tid < rows * vecs)
-      for (int64_t t = t0 + tid / vecs; t < t1; t += rows) {
-        const uint32_t x = t < u.len ? word : 0u;
-        *reinterpret_cast<uint4*>(o + t * l.so[1]) = make_uint4(x, x, x, x);
-      }
-    if (dead) return;
-    if (live_chunks == 0 && u.seg == 0 && l.fresh)
-      for (int i = tid; i < u.nheads * l.N * l.P; i += kThreads)
-        l.state[slot * l.ss[0] + (u.head0 + i / (l.N * l.P)) * l.ss[1] + i % (l.N * l.P)] = 0.f;
-    if (u.first >= u.last) return;
-  } else if (u.first + p.seg_chunks >= live_chunks) {
-    return;  // nothing reads this segment's state
-  }
 
   // ---- set-up ------------------------------------------------------------------
-  const bool two = WIDE || u.nheads == 2;  // the second block of value columns is there
   if (warp == kLoadWarp) {
     tmem_alloc(&m.tmem, 512);
     tmem_relinquish();
@@ -367,36 +376,68 @@ __global__ void __launch_bounds__(kThreads, 1) linear_chunk_kernel(const __grid_
     mbar_init(&m.oi_free, 8);
     mbar_init(&m.s_ready, 4);
     mbar_init(&m.s_free, 1);
+    mbar_init(&m.init_full, 1);
+    mbar_init(&m.init_read, 4);
     fence_mbar_init();
   }
-  if (FULL) {  // the zero tile, and P's tiles: what lies above the diagonal is never written
-    if (!WIDE)
-      for (int i = tid; i < kBox / 16; i += kThreads) sts16(sb + L::zero + 16 * i, make_uint4(0, 0, 0, 0));
-    for (int i = tid; i < (WIDE ? 2 : 4) * kBox / 16; i += kThreads) sts16(sb + L::p + 16 * i, make_uint4(0, 0, 0, 0));
+  {
+    const Unit u = unit_of<WIDE>(p, blockIdx.x);
+    if (tid == 0) m.unit = u;
+    bool dead = false;  // no state of its own: padding, a wrong slot, or one that an earlier row has
+    if (FULL) {
+      dead = l.state && (u.slot < 0 || u.slot >= l.nslots);
+      if (l.slots)
+        for (int i = tid; i < u.b; i += kThreads) dead |= l.slots[i] == u.slot;
+    }
+    fence_async_smem();
+    tc_fence_before();
+    dead = __syncthreads_or(dead);
+    tc_fence_after();
+    if (dead || u.first >= u.last || (!FULL && u.ends_row())) {
+      // Nothing to work on, or (a segment's own state) nobody who would read it.
+      if (FULL) fill_rows(p, u, u.first * kC, tid, kThreads, dead && u.slot >= 0 ? 0x7fc07fc0u : 0u);
+      if (FULL && !dead && u.len == 0 && u.seg == 0 && l.fresh && l.state)
+        for (int i = tid; i < u.nheads * l.N * l.P; i += kThreads)
+          l.state[u.slot * l.ss[0] + (u.head0 + i / (l.N * l.P)) * l.ss[1] + i % (l.N * l.P)] = 0.f;
+      if (warp == kLoadWarp) tmem_dealloc(m.tmem, 512);
+      return;
+    }
   }
-  fence_async_smem();
-  tc_fence_before();
-  __syncthreads();
-  tc_fence_after();
+  // The states of this CTA's heads lie in pieces of neighbouring values: 64 rows at a time of
+  // one wide head, or the heads of a pair.
+  auto pieces = [&](const Unit& u) { return WIDE ? NK : u.nheads; };
+  auto piece_bytes = [&](int x) { return static_cast<uint32_t>((WIDE ? min(l.N - 64 * x, 64) : l.N) * l.P * 4); };
+  auto seg_piece = [&](const Unit& u, int seg, int x) {
+    const int64_t row = static_cast<int64_t>(u.b) * l.H + u.head0 + (WIDE ? 0 : x);
+    return p.seg_state + (row * p.segs + seg) * (static_cast<int64_t>(l.N) * l.P) + (WIDE ? x * 64 * l.P : 0);
+  };
+  auto pool_piece = [&](const Unit& u, int x) {
+    return l.state + u.slot * l.ss[0] + (u.head0 + (WIDE ? 0 : x)) * l.ss[1] + (WIDE ? x * 64 * l.P : 0);
+  };
+  const bool has_init = FULL && (p.segs > 1 || (l.state && !l.fresh));
   const uint32_t tm = m.tmem;
-  const int n_chunks = u.last - u.first;
   const int q4 = warp & 3;                  // quarter of the TMEM lanes
   const uint32_t tl = (32u * q4) << 16;
   bool bad = false;  // a bounded wait gave up
-  // Live tokens of a chunk.
-  auto live_of = [&](int it) {
-    return static_cast<int>(min(u.len - static_cast<int64_t>(u.first + it) * kC, static_cast<int64_t>(kC)));
-  };
 
   if (warp >= kSumWarp) {
-    fewer_registers<kOtherRegs>();
+    fewer_registers<Regs<NK>::single>();
+    const Unit u = m.unit;
+    const int n_chunks = u.last - u.first;
     if (warp == kLoadWarp && lane == 0) {
       // ---- loads ----------------------------------------------------------------
+      const bool two = WIDE || u.nheads == 2;  // the second block of value columns is there
       const int boxes = (FULL ? 2 : 1) * NK + (two ? 2 : 1);
       int issued = 0;
       Ring<kStages> ring;
       for (int it = 0; it < n_chunks; ++it, ring.next()) {
         const int st = ring.st, t = (u.first + it) * kC;
+        if (it == 1 && has_init) {  // its stages are free once the state has been taken out
+          if (!mbar_wait(&m.init_read, 0)) {
+            bad = true;
+            break;
+          }
+        }
         if (it >= kStages && !mbar_wait(&m.empty[st], ring.ph ^ 1)) {
           bad = true;
           break;
@@ -410,9 +451,18 @@ __global__ void __launch_bounds__(kThreads, 1) linear_chunk_kernel(const __grid_
         if (two)
           tma_load_4d(sb + L::vb(st), &p.tm_v, &m.full[st], WIDE ? 64 : 0, WIDE ? u.head0 : u.head0 + 1, t, u.b);
         ++issued;
+        if (it == 0 && has_init) {
+          uint32_t bytes = 0;
+          for (int x = 0; x < pieces(u); ++x) bytes += piece_bytes(x);
+          mbar_arrive_expect_tx(&m.init_full, bytes);
+          for (int x = 0; x < pieces(u); ++x)
+            bulk_load(sb + (x ? L::init1 : L::init0), p.segs > 1 ? seg_piece(u, u.seg, x) : pool_piece(u, x),
+                      piece_bytes(x), &m.init_full);
+        }
       }
       // No copy of this CTA may be in flight when it ends (also after a wait that gave up).
       for (int i = max(0, issued - kStages); i < issued; ++i) bad |= !mbar_wait(&m.full[i % kStages], (i / kStages) & 1);
+      if (issued > 0 && has_init) bad |= !mbar_wait(&m.init_full, 0);
     } else if (warp == kStateMmaWarp) {
       // ---- products that need nothing of the state before --------------------------
       // The whole warp runs this, one lane issues: addresses stay in uniform registers.
@@ -521,14 +571,14 @@ __global__ void __launch_bounds__(kThreads, 1) linear_chunk_kernel(const __grid_
       const float* g = l.decay + u.b * l.sg[0] + (u.head0 + (mine ? x : 0)) * l.sg[1];
       float next[kT], seg_total = 0.f;
       auto load_decays = [&](int it) {
-        const int64_t t = static_cast<int64_t>(u.first + it) * kC + tok;
+        const int t = (u.first + it) * kC + tok;
 #pragma unroll
-        for (int j = 0; j < kT; ++j) next[j] = mine && t + j < u.len ? g[(t + j) * l.sg[2]] : 0.f;
+        for (int j = 0; j < kT; ++j) next[j] = mine && t + j < u.len ? g[static_cast<int64_t>(t + j) * l.sg[2]] : 0.f;
       };
       load_decays(0);
 #pragma unroll 1
       for (int it = 0; it < n_chunks; ++it) {
-        const int sl = it % kSums, live = live_of(it);
+        const int sl = it % kSums, live = u.live(it);
         float c[kT], after[kT];
 #pragma unroll
         for (int j = 0; j < kT; ++j) {
@@ -592,13 +642,16 @@ __global__ void __launch_bounds__(kThreads, 1) linear_chunk_kernel(const __grid_
     __syncwarp();
   } else if (warp >= kOutWarp) {
     // ---- outputs ------------------------------------------------------------------------
-    fewer_registers<kOutRegs>();
+    fewer_registers<Regs<NK>::out>();
     if (FULL) {
+      const Unit u = m.unit;
+      const int n_chunks = u.last - u.first;
       const int half = (warp - kOutWarp) >> 2;  // 32 tokens
       const int hd = WIDE ? 0 : q4 >> 1, head = u.head0 + hd;
       const int ocol = WIDE ? 32 * q4 : 32 * (q4 & 1);
       const bool stores = ocol < l.P && hd < u.nheads;
       const uint32_t stage = sb + L::o + (warp - kOutWarp) * 2048u;  // 32 tokens x 32 columns
+      fill_rows(p, u, u.last * kC, tid - 32 * kOutWarp, 256, 0u);  // chunks past the length
       for (int it = 0; it < n_chunks; ++it) {
         const int sl = it % kSums, t0 = (u.first + it) * kC + 32 * half;
         bad |= !mbar_wait(&m.sums[sl], (it / kSums) & 1);
@@ -612,7 +665,7 @@ __global__ void __launch_bounds__(kThreads, 1) linear_chunk_kernel(const __grid_
         __syncwarp();
         const float* ecs = &m.ecs[sl][hd < u.nheads ? hd : 0][32 * half + 2 * (lane & 3)];
         const uint32_t from = tm + 32 * half + tl;
-        const int live = live_of(it);
+        const int live = u.live(it);
         // All of q S first, whose columns the next chunk waits for: [16 tokens][16 lanes].
         float oi[4][8];
 #pragma unroll
@@ -660,14 +713,22 @@ __global__ void __launch_bounds__(kThreads, 1) linear_chunk_kernel(const __grid_
     }
   } else if (warp >= kScoreWarp) {
     // ---- scores to weights: P = D e^{c_i - c_j} for j <= i ------------------------------
-    fewer_registers<kOtherRegs>();
+    fewer_registers<Regs<NK>::score>();
     if (FULL) {
+      const Unit u = m.unit;
+      const int n_chunks = u.last - u.first;
       const int half = (warp - kScoreWarp) >> 2;  // 32 columns
       // Rows i0 and i0 + 8; 16 columns at a time: j0 + 16 z + 8 y + {0, 1}, y < 2. Columns past
       // the warp's last row are left alone.
       const int i0 = 16 * q4 + (lane >> 2), j0 = 32 * half + 2 * (lane & 3);
       const int steps = min(2, max(0, q4 + 1 - 2 * half));
       const int heads = WIDE ? 1 : u.nheads;
+      // The zero tile, and P's tiles: what lies above the diagonal is never written.
+      for (int i = tid - 32 * kScoreWarp; i < (WIDE ? 2 : 4) * kBox / 16; i += 256)
+        sts16(sb + L::p + 16 * i, make_uint4(0, 0, 0, 0));
+      if (!WIDE)
+        for (int i = tid - 32 * kScoreWarp; i < kBox / 16; i += 256) sts16(sb + L::zero + 16 * i, make_uint4(0, 0, 0, 0));
+      bad = bar_or(3, 256, false);
       // Pairs of the last step that lie on or below the diagonal, [y][row group].
       uint32_t keep[4];
 #pragma unroll
@@ -686,7 +747,7 @@ __global__ void __launch_bounds__(kThreads, 1) linear_chunk_kernel(const __grid_
           bad = true;
           break;
         }
-        const int live = live_of(it);
+        const int live = u.live(it);
         if (live < kC) {  // as the prepared values: rows past the length are zero before v is an operand
           const int st = ring.st, vecs = (kC - live) * 8;
           for (int i = tid - 32 * kScoreWarp; i < (WIDE || u.nheads == 2 ? 2 : 1) * vecs; i += 256)
@@ -738,7 +799,10 @@ __global__ void __launch_bounds__(kThreads, 1) linear_chunk_kernel(const __grid_
     }
   } else if (warp >= kPrepWarp) {
     // ---- weighted values, transposed into TMEM -------------------------------------------
-    fewer_registers<kOtherRegs>();
+    fewer_registers<Regs<NK>::prep>();
+    const Unit u = m.unit;
+    const int n_chunks = u.last - u.first;
+    const bool two = WIDE || u.nheads == 2;
     const int pt = tid - 32 * kPrepWarp, half = (warp - kPrepWarp) >> 2;  // 32 tokens
     const int blk = q4 >> 1;                       // block of value columns of this warp's lanes
     const int hd = WIDE ? 0 : blk;
@@ -749,7 +813,7 @@ __global__ void __launch_bounds__(kThreads, 1) linear_chunk_kernel(const __grid_
     }
     Ring<kStages> ring;
     for (int it = 0; it < n_chunks; ++it, ring.next()) {
-      const int st = ring.st, sl = it % kSums, live = live_of(it), wb = it % C::wv_bufs;
+      const int st = ring.st, sl = it % kSums, live = u.live(it), wb = it % C::wv_bufs;
       bad |= !mbar_wait(&m.full[st], ring.ph);
       bad |= !mbar_wait(&m.sums[sl], (it / kSums) & 1);
       if (live < kC) {
@@ -805,39 +869,56 @@ __global__ void __launch_bounds__(kThreads, 1) linear_chunk_kernel(const __grid_
     }
   } else {
     // ---- state ------------------------------------------------------------------------------
-    more_registers<kStateRegs>();
+    more_registers<Regs<NK>::state>();
+    const Unit u = m.unit;
+    const int n_chunks = u.last - u.first;
     const int row = 32 * q4 + lane;              // accumulator lane
     const int blk = row >> 6;                    // block of value columns
     const int hd = WIDE ? 0 : blk;               // head of the CTA
     const int col = WIDE ? row : row & 63;       // value column in the head
     const bool on = col < l.P && hd < u.nheads;
-    const int head = u.head0 + hd;
     constexpr int kNS = 64 * NK;                 // state values of a thread: the key columns of a value
-    const int64_t srow = static_cast<int64_t>(u.b) * l.H + head;
+    // States go between shared memory and registers through TMEM, 16 columns at a time: a loop
+    // over rows can address TMEM, not registers, and unrolled it would be 20 KB of code that
+    // every CTA has to fetch. This lane's value of the first of those rows, in two areas:
+    auto rows_at = [&](uint32_t a0, uint32_t a1, int n) {
+      return sb + (WIDE ? (n < 64 ? a0 : a1) + static_cast<uint32_t>((n & 63) * l.P) * 4 : (blk ? a1 : a0) + n * l.P * 4) +
+             col * 4;
+    };
     float s[kNS];
+    if (!has_init) {
 #pragma unroll
-    for (int i = 0; i < kNS; ++i) s[i] = 0.f;
-    if (FULL) {
-      const float* from = nullptr;
-      if (p.segs > 1)
-        from = p.seg_state + (srow * p.segs + u.seg) * l.N * l.P;
-      else if (l.state && !l.fresh)
-        from = l.state + slot * l.ss[0] + head * l.ss[1];
-      if (from && on) {
+      for (int i = 0; i < kNS; ++i) s[i] = 0.f;
+    } else {
+      bad |= !mbar_wait(&m.init_full, 0);
+      // Columns that nothing uses before the state is there: the second chunk's D, and OI.
+      auto columns = [&](int n) { return tm + (n < 64 ? C::x + 64 + n : C::oi + n - 64) + tl; };
+#pragma unroll 1
+      for (int n = 0; n < kNS; n += 16) {
+        uint32_t r[16], from = rows_at(L::init0, L::init1, n);
 #pragma unroll
-        for (int i = 0; i < kNS; ++i) {
-          if (i < l.N) s[i] = from[i * l.P + col];
+        for (int j = 0; j < 16; ++j, from += l.P * 4) {
+          r[j] = 0;
+          if (on && n + j < l.N) asm volatile("ld.shared.b32 %0, [%1];" : "=r"(r[j]) : "r"(from) : "memory");
         }
+        tmem_st16(columns(n), r);
       }
+      tmem_wait_st();
+#pragma unroll
+      for (int n = 0; n < kNS; n += 16) tmem_ld16(columns(n), *reinterpret_cast<float(*)[16]>(s + n));
+      tmem_wait_ld();
+      tc_fence_before();
+      __syncwarp();
+      if (lane == 0) mbar_arrive(&m.init_read);
     }
     // The state rounded to BF16, as the operand of q S.
     auto put_state = [&]() {
 #pragma unroll
-      for (int i = 0; i < kNS; i += 32) {
-        uint32_t r[16];
+      for (int i = 0; i < kNS; i += 16) {
+        uint32_t r[8];
 #pragma unroll
-        for (int j = 0; j < 16; ++j) r[j] = pack_bf16x2(s[i + 2 * j], s[i + 2 * j + 1]);
-        tmem_st16(tm + C::s + i / 2 + tl, r);
+        for (int j = 0; j < 8; ++j) r[j] = pack_bf16x2(s[i + 2 * j], s[i + 2 * j + 1]);
+        tmem_st8(tm + C::s + i / 2 + tl, r);
       }
       tmem_wait_st();
       tc_fence_before();
@@ -856,14 +937,16 @@ __global__ void __launch_bounds__(kThreads, 1) linear_chunk_kernel(const __grid_
         break;
       }
       const float a = m.total[sl][hd < u.nheads ? hd : 0];
+      constexpr int kBatch = NK == 1 ? 32 : 16;  // columns on their way at a time, as registers allow
 #pragma unroll
-      for (int i = 0; i < kNS; i += 32) {
-        float d[32];
-        tmem_ld16(tm + C::ds + 64 * NK * db + i + tl, *reinterpret_cast<float(*)[16]>(d));
-        tmem_ld16(tm + C::ds + 64 * NK * db + i + 16 + tl, *reinterpret_cast<float(*)[16]>(d + 16));
+      for (int i = 0; i < kNS; i += kBatch) {
+        float d[kBatch];
+#pragma unroll
+        for (int j = 0; j < kBatch; j += 16)
+          tmem_ld16(tm + C::ds + 64 * NK * db + i + j + tl, *reinterpret_cast<float(*)[16]>(d + j));
         tmem_wait_ld();
 #pragma unroll
-        for (int j = 0; j < 32; j += 2) {
+        for (int j = 0; j < kBatch; j += 2) {
           const float2 x = fma2(make_float2(a, a), make_float2(s[i + j], s[i + j + 1]), make_float2(d[j], d[j + 1]));
           s[i + j] = x.x;
           s[i + j + 1] = x.y;
@@ -885,17 +968,36 @@ __global__ void __launch_bounds__(kThreads, 1) linear_chunk_kernel(const __grid_
         put_state();
       }
     }
-    if (on && !bad) {
-      float* to = nullptr;
-      if (!FULL)
-        to = p.seg_state + (srow * p.segs + u.seg + 1) * l.N * l.P;
-      else if (u.last == live_chunks && l.state)
-        to = l.state + slot * l.ss[0] + head * l.ss[1];
-      if (to)
+    // The state after the last chunk, through shared memory: every tile there has been read.
+    if (FULL) bad |= !mbar_wait(&m.o_full[(n_chunks - 1) & 1], ((n_chunks - 1) >> 1) & 1);
+    if (!FULL || (u.ends_row() && l.state)) {
 #pragma unroll
-        for (int i = 0; i < kNS; ++i) {
-          if (i < l.N) to[i * l.P + col] = s[i];
-        }
+      for (int n = 0; n < kNS; n += 8) {
+        uint32_t r[8];
+#pragma unroll
+        for (int j = 0; j < 8; ++j) r[j] = __float_as_uint(s[n + j]);
+        tmem_st8(tm + C::ds + n + tl, r);
+      }
+      tmem_wait_st();
+#pragma unroll 1
+      for (int n = 0; n < kNS; n += 16) {
+        float r[16];
+        tmem_ld16(tm + C::ds + n + tl, r);
+        tmem_wait_ld();
+        uint32_t to = rows_at(L::last0, L::last1, n);
+#pragma unroll
+        for (int j = 0; j < 16; ++j, to += l.P * 4)
+          if (on && n + j < l.N) sts4(to, __float_as_uint(r[j]));
+      }
+      fence_async_smem();
+      bad = bar_or(1, 128, bad);
+      if (tid == 0 && !bad) {
+        for (int x = 0; x < pieces(u); ++x)
+          bulk_store(FULL ? pool_piece(u, x) : seg_piece(u, u.seg + 1, x), sb + (x ? L::last1 : L::last0), piece_bytes(x));
+        asm volatile("cp.async.bulk.commit_group;" ::: "memory");
+        asm volatile("cp.async.bulk.wait_group 0;" ::: "memory");
+      }
+      __syncwarp();
     }
   }
   tc_fence_before();
@@ -936,9 +1038,10 @@ __global__ void __launch_bounds__(256) linear_join_kernel(const __grid_constant_
   if (!l.fresh && l.state && slot >= 0 && slot < l.nslots)
     s = *reinterpret_cast<const float4*>(l.state + slot * l.ss[0] + h * l.ss[1] + e);
   *reinterpret_cast<float4*>(own) = s;
+#pragma unroll 4
   for (int g = 1; g < segs; ++g) {
     const float a = ex2_approx(p.seg_decay[row * p.segs + g - 1]);
-    const float4 d = *reinterpret_cast<const float4*>(own + g * step);
+    const float4 d = __ldcg(reinterpret_cast<const float4*>(own + g * step));
     s.x = fmaf(a, s.x, d.x);
     s.y = fmaf(a, s.y, d.y);
     s.z = fmaf(a, s.z, d.z);
