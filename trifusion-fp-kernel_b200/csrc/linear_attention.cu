@@ -77,25 +77,40 @@ __global__ void __launch_bounds__(kScanThreads) linear_scan_kernel(const __grid_
   const T* k = static_cast<const T*>(p.k) + b * p.sk[0] + hq * p.sk[2];
   const T* v = static_cast<const T*>(p.v) + b * p.sv[0] + h * p.sv[2];
   const float* g = p.decay + b * p.sg[0] + h * p.sg[1];
-  for (int64_t t = 0; t < len; ++t) {
-    const float a = decay_factor(g[t * p.sg[2]]);
-    float vv[4];
+  // One token's operands, loaded while the one before is worked on.
+  float gn = 0.f, vn[4] = {}, kn[NR] = {}, qn[NR] = {};
+  auto load = [&](int64_t t) {
+    if (t >= len) return;
+    gn = g[t * p.sg[2]];
 #pragma unroll
-    for (int j = 0; j < 4; ++j) vv[j] = on ? ld_f(v + t * p.sv[1] + col + j) : 0.f;
-    float4 o = make_float4(0.f, 0.f, 0.f, 0.f);
+    for (int j = 0; j < 4; ++j)
+      if (on) vn[j] = ld_f(v + t * p.sv[1] + col + j);
 #pragma unroll
     for (int i = 0; i < NR; ++i) {
       const int n = r0 + 32 * i;
-      const float kn = n < p.N ? ld_f(k + t * p.sk[1] + n) : 0.f;
-      const float qn = n < p.N ? ld_f(q + t * p.sq[1] + n) : 0.f;
-      s[i].x = fmaf(kn, vv[0], a * s[i].x);
-      s[i].y = fmaf(kn, vv[1], a * s[i].y);
-      s[i].z = fmaf(kn, vv[2], a * s[i].z);
-      s[i].w = fmaf(kn, vv[3], a * s[i].w);
-      o.x = fmaf(qn, s[i].x, o.x);
-      o.y = fmaf(qn, s[i].y, o.y);
-      o.z = fmaf(qn, s[i].z, o.z);
-      o.w = fmaf(qn, s[i].w, o.w);
+      if (n < p.N) kn[i] = ld_f(k + t * p.sk[1] + n), qn[i] = ld_f(q + t * p.sq[1] + n);
+    }
+  };
+  load(0);
+  for (int64_t t = 0; t < len; ++t) {
+    const float a = decay_factor(gn);
+    float vv[4], kk[NR], qq[NR];
+#pragma unroll
+    for (int j = 0; j < 4; ++j) vv[j] = vn[j];
+#pragma unroll
+    for (int i = 0; i < NR; ++i) kk[i] = kn[i], qq[i] = qn[i];
+    load(t + 1);
+    float4 o = make_float4(0.f, 0.f, 0.f, 0.f);
+#pragma unroll
+    for (int i = 0; i < NR; ++i) {
+      s[i].x = fmaf(kk[i], vv[0], a * s[i].x);
+      s[i].y = fmaf(kk[i], vv[1], a * s[i].y);
+      s[i].z = fmaf(kk[i], vv[2], a * s[i].z);
+      s[i].w = fmaf(kk[i], vv[3], a * s[i].w);
+      o.x = fmaf(qq[i], s[i].x, o.x);
+      o.y = fmaf(qq[i], s[i].y, o.y);
+      o.z = fmaf(qq[i], s[i].z, o.z);
+      o.w = fmaf(qq[i], s[i].w, o.w);
     }
 #pragma unroll
     for (int d = 8; d < 32; d <<= 1) {
@@ -125,13 +140,91 @@ __global__ void __launch_bounds__(kScanThreads) linear_scan_kernel(const __grid_
     }
 }
 
+// The same for one token, without what a loop over tokens needs: with NR <= 4 six blocks (96 KB
+// of state on their way) fit an SM instead of three.
+template <typename T, int NR>
+__global__ void __launch_bounds__(kScanThreads, NR <= 4 ? 6 : 3)
+    linear_step_kernel(const __grid_constant__ LinearParams p) {
+  __shared__ float4 partial[8][8];
+  const int slices = (p.P + 31) / 32;
+  const int slice = blockIdx.x % slices;
+  const int row = blockIdx.x / slices;
+  const int h = row % p.H, b = row / p.H;
+  const int w = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const int col = slice * 32 + 4 * (lane & 7);
+  const int r0 = w * 4 + (lane >> 3);
+  const bool on = col < p.P;
+  const int64_t slot = p.slots ? p.slots[b] : b;
+  const bool in_pool = slot >= 0 && slot < p.nslots;
+  float* st = p.state + (in_pool ? slot * p.ss[0] + h * p.ss[1] + static_cast<int64_t>(r0) * p.P + col : 0);
+  float4 s[NR];
+#pragma unroll
+  for (int i = 0; i < NR; ++i)
+    if (in_pool && on && r0 + 32 * i < p.N) s[i] = *reinterpret_cast<const float4*>(st + 32 * i * p.P);
+  const int hq = h / (p.H / p.Hq);
+  const T* q = static_cast<const T*>(p.q) + b * p.sq[0] + hq * p.sq[2] + r0;
+  const T* k = static_cast<const T*>(p.k) + b * p.sk[0] + hq * p.sk[2] + r0;
+  const T* v = static_cast<const T*>(p.v) + b * p.sv[0] + h * p.sv[2] + col;
+  float vv[4] = {};
+#pragma unroll
+  for (int j = 0; j < 4; ++j)
+    if (on) vv[j] = ld_f(v + j);
+  const float a = decay_factor(p.decay[b * p.sg[0] + h * p.sg[1]]);
+  bool dead = !in_pool;  // no state of its own
+  if (p.slots) {
+    for (int i = threadIdx.x; i < b; i += kScanThreads) dead |= p.slots[i] == slot;
+    dead = __syncthreads_or(dead);
+  }
+  float4 o = make_float4(0.f, 0.f, 0.f, 0.f);
+#pragma unroll
+  for (int i = 0; i < NR; ++i)
+    if (!dead && on && r0 + 32 * i < p.N) {
+      const float kn = ld_f(k + 32 * i), qn = ld_f(q + 32 * i);
+      s[i].x = fmaf(kn, vv[0], a * s[i].x);
+      s[i].y = fmaf(kn, vv[1], a * s[i].y);
+      s[i].z = fmaf(kn, vv[2], a * s[i].z);
+      s[i].w = fmaf(kn, vv[3], a * s[i].w);
+      o.x = fmaf(qn, s[i].x, o.x);
+      o.y = fmaf(qn, s[i].y, o.y);
+      o.z = fmaf(qn, s[i].z, o.z);
+      o.w = fmaf(qn, s[i].w, o.w);
+      *reinterpret_cast<float4*>(st + 32 * i * p.P) = s[i];
+    }
+#pragma unroll
+  for (int d = 8; d < 32; d <<= 1) {
+    o.x += __shfl_xor_sync(0xffffffffu, o.x, d);
+    o.y += __shfl_xor_sync(0xffffffffu, o.y, d);
+    o.z += __shfl_xor_sync(0xffffffffu, o.z, d);
+    o.w += __shfl_xor_sync(0xffffffffu, o.w, d);
+  }
+  if (lane < 8) partial[w][lane] = o;
+  __syncthreads();
+  const int c = slice * 32 + lane;
+  if (w == 0 && c < p.P) {
+    const float* f = reinterpret_cast<const float*>(&partial[0][0]);
+    float sum = 0.f;
+#pragma unroll
+    for (int i = 0; i < 8; ++i) sum += f[32 * i + lane];
+    // A row without a state: zero where it is padding, NaN where it names a wrong slot.
+    const float y = dead ? (slot < 0 ? 0.f : __int_as_float(0x7fc00000)) : sum * p.scale;
+    st_f(static_cast<T*>(p.out) + b * p.so[0] + h * p.so[2] + c, y);
+  }
+}
+
+template <typename T, int NR>
+void launch_rows(const LinearParams& p, cudaStream_t stream) {
+  const unsigned grid = static_cast<unsigned>(static_cast<int64_t>(p.B) * p.H * ((p.P + 31) / 32));
+  if (p.T == 1 && p.state && !p.fresh && !p.lengths)
+    linear_step_kernel<T, NR><<<grid, kScanThreads, 0, stream>>>(p);
+  else
+    linear_scan_kernel<T, NR><<<grid, kScanThreads, 0, stream>>>(p);
+}
 template <typename T>
 void launch_scan(const LinearParams& p, cudaStream_t stream) {
-  const unsigned grid = static_cast<unsigned>(static_cast<int64_t>(p.B) * p.H * ((p.P + 31) / 32));
-  if (p.N <= 32) linear_scan_kernel<T, 1><<<grid, kScanThreads, 0, stream>>>(p);
-  else if (p.N <= 64) linear_scan_kernel<T, 2><<<grid, kScanThreads, 0, stream>>>(p);
-  else if (p.N <= 128) linear_scan_kernel<T, 4><<<grid, kScanThreads, 0, stream>>>(p);
-  else linear_scan_kernel<T, 8><<<grid, kScanThreads, 0, stream>>>(p);
+  if (p.N <= 32) launch_rows<T, 1>(p, stream);
+  else if (p.N <= 64) launch_rows<T, 2>(p, stream);
+  else if (p.N <= 128) launch_rows<T, 4>(p, stream);
+  else launch_rows<T, 8>(p, stream);
 }
 
 }  // namespace

@@ -995,7 +995,7 @@ __global__ void __launch_bounds__(kThreads, 1) linear_chunk_kernel(const __grid_
         for (int x = 0; x < pieces(u); ++x)
           bulk_store(FULL ? pool_piece(u, x) : seg_piece(u, u.seg + 1, x), sb + (x ? L::last1 : L::last0), piece_bytes(x));
         asm volatile("cp.async.bulk.commit_group;" ::: "memory");
-        asm volatile("cp.async.bulk.wait_group 0;" ::: "memory");
+        tma_store_wait_read();
       }
       __syncwarp();
     }
@@ -1096,8 +1096,9 @@ struct Plan {
   int64_t rows, state_bytes, bytes;
 };
 
-// A prompt shorter than this runs token by token.
-constexpr int kMinTokens = 32;
+// A prompt shorter than this runs token by token: 7.3 and 9.9 us for 8 tokens (1 and 16 rows of
+// 12 heads, N = 128, P = 64), 33 us for 1024 heads, against 9.4, 9.9 and 31 us in a chunk.
+constexpr int kMinTokens = 8;
 
 bool plan_of(int B, int T, int H, int Hq, int N, int P, int dtype, Plan& x) {
   if (dtype != TF_BF16 || N > 128 || P > 128 || T < kMinTokens) return false;
