@@ -6,6 +6,8 @@
 // q and k heads are shared by H / Hq heads of v. This file holds the recurrent
 // form (one token after another, the state in registers); linear_chunks.cu the
 // chunked form on the tensor cores.
+#include <type_traits>
+
 #include "../../include/trifusion_b200.h"
 #include "linear_attention.cuh"
 #include "tf_common.cuh"
@@ -140,68 +142,94 @@ __global__ void __launch_bounds__(kScanThreads) linear_scan_kernel(const __grid_
     }
 }
 
-// The same for one token, without what a loop over tokens needs: with NR <= 4 six blocks (96 KB
-// of state on their way) fit an SM instead of three.
-template <typename T, int NR>
-__global__ void __launch_bounds__(kScanThreads, NR <= 4 ? 6 : 3)
+// The same for one token, without what a loop over tokens needs, on up to CS times 32 columns,
+// so that a block has 16 KB of state on its way where N <= 128. Bound by HBM: the states are
+// read and written once. They are streamed (evict-first): larger pools than the L2 would only
+// push each other out, smaller ones stay in it all the same. 64 rows of 32 heads, 128 x 128:
+// 43.4 us (268 MB, 94 % of the measured copy rate); 48.0 us with ordinary accesses, 45.1 and
+// 46.6 us with four and six blocks an SM instead of five.
+template <typename T, int NR, int CS>
+__global__ void __launch_bounds__(kScanThreads, NR > 4 ? 3 : NR == 4 ? 5 : CS == 1 ? 6 : 4)
     linear_step_kernel(const __grid_constant__ LinearParams p) {
-  __shared__ float4 partial[8][8];
-  const int slices = (p.P + 31) / 32;
+  __shared__ float4 partial[CS][8][8];
+  const int slices = (p.P + 32 * CS - 1) / (32 * CS);
   const int slice = blockIdx.x % slices;
   const int row = blockIdx.x / slices;
   const int h = row % p.H, b = row / p.H;
   const int w = threadIdx.x >> 5, lane = threadIdx.x & 31;
-  const int col = slice * 32 + 4 * (lane & 7);
+  const int col = slice * 32 * CS + 4 * (lane & 7);  // and 32 columns on, CS - 1 times
   const int r0 = w * 4 + (lane >> 3);
-  const bool on = col < p.P;
   const int64_t slot = p.slots ? p.slots[b] : b;
   const bool in_pool = slot >= 0 && slot < p.nslots;
   float* st = p.state + (in_pool ? slot * p.ss[0] + h * p.ss[1] + static_cast<int64_t>(r0) * p.P + col : 0);
-  float4 s[NR];
+  float4 s[CS][NR];
 #pragma unroll
-  for (int i = 0; i < NR; ++i)
-    if (in_pool && on && r0 + 32 * i < p.N) s[i] = *reinterpret_cast<const float4*>(st + 32 * i * p.P);
+  for (int c = 0; c < CS; ++c)
+#pragma unroll
+    for (int i = 0; i < NR; ++i)
+      if (in_pool && col + 32 * c < p.P && r0 + 32 * i < p.N)
+        s[c][i] = __ldcs(reinterpret_cast<const float4*>(st + 32 * i * p.P + 32 * c));
   const int hq = h / (p.H / p.Hq);
   const T* q = static_cast<const T*>(p.q) + b * p.sq[0] + hq * p.sq[2] + r0;
   const T* k = static_cast<const T*>(p.k) + b * p.sk[0] + hq * p.sk[2] + r0;
   const T* v = static_cast<const T*>(p.v) + b * p.sv[0] + h * p.sv[2] + col;
-  float vv[4] = {};
+  constexpr bool kEarly = NR <= 2;  // k and q on their way with the state, as registers allow
+  float early[2][kEarly ? NR : 1] = {}, vv[CS][4] = {};
+  if (kEarly) {
 #pragma unroll
-  for (int j = 0; j < 4; ++j)
-    if (on) vv[j] = ld_f(v + j);
+    for (int i = 0; i < NR; ++i)
+      if (r0 + 32 * i < p.N) early[0][i % (kEarly ? NR : 1)] = ld_f(k + 32 * i), early[1][i % (kEarly ? NR : 1)] = ld_f(q + 32 * i);
+  }
+#pragma unroll
+  for (int c = 0; c < CS; ++c)
+#pragma unroll
+    for (int j = 0; j < 4; ++j)
+      if (col + 32 * c < p.P) vv[c][j] = ld_f(v + 32 * c + j);
   const float a = decay_factor(p.decay[b * p.sg[0] + h * p.sg[1]]);
   bool dead = !in_pool;  // no state of its own
   if (p.slots) {
     for (int i = threadIdx.x; i < b; i += kScanThreads) dead |= p.slots[i] == slot;
     dead = __syncthreads_or(dead);
   }
-  float4 o = make_float4(0.f, 0.f, 0.f, 0.f);
+  float4 o[CS];
 #pragma unroll
-  for (int i = 0; i < NR; ++i)
-    if (!dead && on && r0 + 32 * i < p.N) {
-      const float kn = ld_f(k + 32 * i), qn = ld_f(q + 32 * i);
-      s[i].x = fmaf(kn, vv[0], a * s[i].x);
-      s[i].y = fmaf(kn, vv[1], a * s[i].y);
-      s[i].z = fmaf(kn, vv[2], a * s[i].z);
-      s[i].w = fmaf(kn, vv[3], a * s[i].w);
-      o.x = fmaf(qn, s[i].x, o.x);
-      o.y = fmaf(qn, s[i].y, o.y);
-      o.z = fmaf(qn, s[i].z, o.z);
-      o.w = fmaf(qn, s[i].w, o.w);
-      *reinterpret_cast<float4*>(st + 32 * i * p.P) = s[i];
+  for (int c = 0; c < CS; ++c) o[c] = make_float4(0.f, 0.f, 0.f, 0.f);
+#pragma unroll
+  for (int i = 0; i < NR; ++i) {
+    if (!dead && (CS > 1 || col < p.P) && r0 + 32 * i < p.N) {
+      const float kn = kEarly ? early[0][i % (kEarly ? NR : 1)] : ld_f(k + 32 * i);
+      const float qn = kEarly ? early[1][i % (kEarly ? NR : 1)] : ld_f(q + 32 * i);
+#pragma unroll
+      for (int c = 0; c < CS; ++c)
+        if (CS == 1 || col + 32 * c < p.P) {
+          float4& x = s[c][i];
+          x.x = fmaf(kn, vv[c][0], a * x.x);
+          x.y = fmaf(kn, vv[c][1], a * x.y);
+          x.z = fmaf(kn, vv[c][2], a * x.z);
+          x.w = fmaf(kn, vv[c][3], a * x.w);
+          o[c].x = fmaf(qn, x.x, o[c].x);
+          o[c].y = fmaf(qn, x.y, o[c].y);
+          o[c].z = fmaf(qn, x.z, o[c].z);
+          o[c].w = fmaf(qn, x.w, o[c].w);
+          __stcs(reinterpret_cast<float4*>(st + 32 * i * p.P + 32 * c), x);
+        }
     }
-#pragma unroll
-  for (int d = 8; d < 32; d <<= 1) {
-    o.x += __shfl_xor_sync(0xffffffffu, o.x, d);
-    o.y += __shfl_xor_sync(0xffffffffu, o.y, d);
-    o.z += __shfl_xor_sync(0xffffffffu, o.z, d);
-    o.w += __shfl_xor_sync(0xffffffffu, o.w, d);
   }
-  if (lane < 8) partial[w][lane] = o;
+#pragma unroll
+  for (int c = 0; c < CS; ++c) {
+#pragma unroll
+    for (int d = 8; d < 32; d <<= 1) {
+      o[c].x += __shfl_xor_sync(0xffffffffu, o[c].x, d);
+      o[c].y += __shfl_xor_sync(0xffffffffu, o[c].y, d);
+      o[c].z += __shfl_xor_sync(0xffffffffu, o[c].z, d);
+      o[c].w += __shfl_xor_sync(0xffffffffu, o[c].w, d);
+    }
+    if (lane < 8) partial[c][w][lane] = o[c];
+  }
   __syncthreads();
-  const int c = slice * 32 + lane;
-  if (w == 0 && c < p.P) {
-    const float* f = reinterpret_cast<const float*>(&partial[0][0]);
+  const int c = (slice * CS + w) * 32 + lane;
+  if (w < CS && c < p.P) {
+    const float* f = reinterpret_cast<const float*>(&partial[w][0][0]);
     float sum = 0.f;
 #pragma unroll
     for (int i = 0; i < 8; ++i) sum += f[32 * i + lane];
@@ -213,11 +241,20 @@ __global__ void __launch_bounds__(kScanThreads, NR <= 4 ? 6 : 3)
 
 template <typename T, int NR>
 void launch_rows(const LinearParams& p, cudaStream_t stream) {
-  const unsigned grid = static_cast<unsigned>(static_cast<int64_t>(p.B) * p.H * ((p.P + 31) / 32));
-  if (p.T == 1 && p.state && !p.fresh && !p.lengths)
-    linear_step_kernel<T, NR><<<grid, kScanThreads, 0, stream>>>(p);
-  else
-    linear_scan_kernel<T, NR><<<grid, kScanThreads, 0, stream>>>(p);
+  const int64_t rows = static_cast<int64_t>(p.B) * p.H;
+  if (p.T == 1 && p.state && !p.fresh && !p.lengths) {
+    // As many columns a block as make up 16 KB, and as there are.
+    auto step = [&](auto cs) {
+      constexpr int CS = decltype(cs)::value;
+      linear_step_kernel<T, NR, CS>
+          <<<static_cast<unsigned>(rows * ((p.P + 32 * CS - 1) / (32 * CS))), kScanThreads, 0, stream>>>(p);
+    };
+    if (NR == 1 && p.P > 64) step(std::integral_constant<int, NR == 1 ? 4 : 1>());
+    else if (NR <= 2 && p.P > 32) step(std::integral_constant<int, NR <= 2 ? 2 : 1>());
+    else step(std::integral_constant<int, 1>());
+  } else {
+    linear_scan_kernel<T, NR><<<static_cast<unsigned>(rows * ((p.P + 31) / 32)), kScanThreads, 0, stream>>>(p);
+  }
 }
 template <typename T>
 void launch_scan(const LinearParams& p, cudaStream_t stream) {
