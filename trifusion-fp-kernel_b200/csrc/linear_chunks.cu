@@ -347,62 +347,6 @@ __global__ void __launch_bounds__(kThreads, 1) linear_chunk_kernel(const __grid_
   const LinearParams& l = p.l;
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
 
-  // ---- set-up ------------------------------------------------------------------
-  if (warp == kLoadWarp) {
-    tmem_alloc(&m.tmem, 512);
-    tmem_relinquish();
-  }
-  if (tid == 0) {
-    for (int i = 0; i < kStages; ++i) {
-      mbar_init(&m.full[i], 1);
-      mbar_init(&m.empty[i], FULL ? 2 : 1);
-    }
-    for (int i = 0; i < kSums; ++i) {
-      mbar_init(&m.sums[i], 1);
-      mbar_init(&m.sums_free[i], FULL ? 12 : 4);
-    }
-    for (int i = 0; i < 2; ++i) {
-      mbar_init(&m.p_ready[i], 8);
-      mbar_init(&m.o_full[i], 1);
-      mbar_init(&m.op_free[i], 8);
-      mbar_init(&m.d_full[i], 1);
-      for (int j = 0; j < 2; ++j) {
-        mbar_init(&m.wv_ready[i][j], 4);
-        mbar_init(&m.wv_free[i][j], 1);
-      }
-      mbar_init(&m.ds_full[i], 1);
-      mbar_init(&m.ds_free[i], 4);
-    }
-    mbar_init(&m.oi_free, 8);
-    mbar_init(&m.s_ready, 4);
-    mbar_init(&m.s_free, 1);
-    mbar_init(&m.init_full, 1);
-    mbar_init(&m.init_read, 4);
-    fence_mbar_init();
-  }
-  {
-    const Unit u = unit_of<WIDE>(p, blockIdx.x);
-    if (tid == 0) m.unit = u;
-    bool dead = false;  // no state of its own: padding, a wrong slot, or one that an earlier row has
-    if (FULL) {
-      dead = l.state && (u.slot < 0 || u.slot >= l.nslots);
-      if (l.slots)
-        for (int i = tid; i < u.b; i += kThreads) dead |= l.slots[i] == u.slot;
-    }
-    fence_async_smem();
-    tc_fence_before();
-    dead = __syncthreads_or(dead);
-    tc_fence_after();
-    if (dead || u.first >= u.last || (!FULL && u.ends_row())) {
-      // Nothing to work on, or (a segment's own state) nobody who would read it.
-      if (FULL) fill_rows(p, u, u.first * kC, tid, kThreads, dead && u.slot >= 0 ? 0x7fc07fc0u : 0u);
-      if (FULL && !dead && u.len == 0 && u.seg == 0 && l.fresh && l.state)
-        for (int i = tid; i < u.nheads * l.N * l.P; i += kThreads)
-          l.state[u.slot * l.ss[0] + (u.head0 + i / (l.N * l.P)) * l.ss[1] + i % (l.N * l.P)] = 0.f;
-      if (warp == kLoadWarp) tmem_dealloc(m.tmem, 512);
-      return;
-    }
-  }
   // The states of this CTA's heads lie in pieces of neighbouring values: 64 rows at a time of
   // one wide head, or the heads of a pair.
   auto pieces = [&](const Unit& u) { return WIDE ? NK : u.nheads; };
@@ -415,6 +359,94 @@ __global__ void __launch_bounds__(kThreads, 1) linear_chunk_kernel(const __grid_
     return l.state + u.slot * l.ss[0] + (u.head0 + (WIDE ? 0 : x)) * l.ss[1] + (WIDE ? x * 64 * l.P : 0);
   };
   const bool has_init = FULL && (p.segs > 1 || (l.state && !l.fresh));
+  // Decays of this lane's tokens of a chunk: a head has all lanes of a warp, or each of two
+  // heads half of them; a lane has kT neighbouring tokens.
+  constexpr int kT = WIDE ? 2 : 4, kLanes = kC / kT;
+  auto load_decays = [&](const Unit& u, int it, float* to) {
+    const int x = lane / kLanes, t = (u.first + it) * kC + lane % kLanes * kT;
+    const float* g = l.decay + u.b * l.sg[0] + (u.head0 + x) * l.sg[1];
+#pragma unroll
+    for (int j = 0; j < kT; ++j)
+      to[j] = x < u.nheads && t + j < u.len ? g[static_cast<int64_t>(t + j) * l.sg[2]] : 0.f;
+  };
+  // One chunk's tiles into a stage.
+  auto load_chunk = [&](const Unit& u, int it, int st) {
+    const bool two = WIDE || u.nheads == 2;  // the second block of value columns is there
+    const int t = (u.first + it) * kC;
+    mbar_arrive_expect_tx(&m.full[st], ((FULL ? 2 : 1) * NK + (two ? 2 : 1)) * kBox);
+    for (int x = 0; x < NK; ++x) {
+      tma_load_4d(sb + L::k + (st * NK + x) * kBox, &p.tm_k, &m.full[st], 64 * x, u.hk, t, u.b);
+      if (FULL) tma_load_4d(sb + L::q + (st * NK + x) * kBox, &p.tm_q, &m.full[st], 64 * x, u.hk, t, u.b);
+    }
+    tma_load_4d(sb + L::va(st), &p.tm_v, &m.full[st], 0, u.head0, t, u.b);
+    if (two)
+      tma_load_4d(sb + L::vb(st), &p.tm_v, &m.full[st], WIDE ? 64 : 0, WIDE ? u.head0 : u.head0 + 1, t, u.b);
+  };
+  // Chunks whose tiles need no waiting for. (The state lies where the second's would.)
+  
+
+  // ---- set-up ------------------------------------------------------------------
+  const Unit first_unit = unit_of<WIDE>(p, blockIdx.x);
+  float decays[4] = {};  // the sum warp's first ones, on their way while the rest is set up
+  {
+    const Unit& u = first_unit;
+    bool dead = false;  // no state of its own: padding, a wrong slot, or one that an earlier row has
+    if (FULL) dead = l.state && (u.slot < 0 || u.slot >= l.nslots);
+    const bool idle = dead || u.first >= u.last || (!FULL && u.ends_row());
+    if (warp == kLoadWarp) {
+      if (lane == 0) {
+        m.unit = u;
+        for (int i = 0; i < kStages; ++i) {
+          mbar_init(&m.full[i], 1);
+          mbar_init(&m.empty[i], FULL ? 2 : 1);
+        }
+        for (int i = 0; i < kSums; ++i) {
+          mbar_init(&m.sums[i], 1);
+          mbar_init(&m.sums_free[i], FULL ? 12 : 4);
+        }
+        for (int i = 0; i < 2; ++i) {
+          mbar_init(&m.p_ready[i], 8);
+          mbar_init(&m.o_full[i], 1);
+          mbar_init(&m.op_free[i], 8);
+          mbar_init(&m.d_full[i], 1);
+          for (int j = 0; j < 2; ++j) {
+            mbar_init(&m.wv_ready[i][j], 4);
+            mbar_init(&m.wv_free[i][j], 1);
+          }
+          mbar_init(&m.ds_full[i], 1);
+          mbar_init(&m.ds_free[i], 4);
+        }
+        mbar_init(&m.oi_free, 8);
+        mbar_init(&m.s_ready, 4);
+        mbar_init(&m.s_free, 1);
+        mbar_init(&m.init_full, 1);
+        mbar_init(&m.init_read, 4);
+        fence_mbar_init();
+      }
+      __syncwarp();
+    } else if (warp == kStateMmaWarp) {
+      tmem_alloc(&m.tmem, 512);
+      tmem_relinquish();
+    }
+    if (warp == kSumWarp && !idle) load_decays(u, 0, decays);
+    if (FULL && l.slots)
+      for (int i = tid; i < u.b; i += kThreads) dead |= l.slots[i] == u.slot;
+    tc_fence_before();
+    dead = __syncthreads_or(dead);
+    tc_fence_after();
+    if (dead || idle) {
+      // Nothing to work on, or (a segment's own state) nobody who would read it.
+      if (FULL) fill_rows(p, u, u.first * kC, tid, kThreads, dead && u.slot >= 0 ? 0x7fc07fc0u : 0u);
+      if (FULL && !dead && u.len == 0 && u.seg == 0 && l.fresh && l.state)
+        for (int i = tid; i < u.nheads * l.N * l.P; i += kThreads)
+          l.state[u.slot * l.ss[0] + (u.head0 + i / (l.N * l.P)) * l.ss[1] + i % (l.N * l.P)] = 0.f;
+      if (warp == kLoadWarp) {
+      } else if (warp == kStateMmaWarp) {
+        tmem_dealloc(m.tmem, 512);
+      }
+      return;
+    }
+  }
   const uint32_t tm = m.tmem;
   const int q4 = warp & 3;                  // quarter of the TMEM lanes
   const uint32_t tl = (32u * q4) << 16;
@@ -426,30 +458,16 @@ __global__ void __launch_bounds__(kThreads, 1) linear_chunk_kernel(const __grid_
     const int n_chunks = u.last - u.first;
     if (warp == kLoadWarp && lane == 0) {
       // ---- loads ----------------------------------------------------------------
-      const bool two = WIDE || u.nheads == 2;  // the second block of value columns is there
-      const int boxes = (FULL ? 2 : 1) * NK + (two ? 2 : 1);
       int issued = 0;
       Ring<kStages> ring;
       for (int it = 0; it < n_chunks; ++it, ring.next()) {
-        const int st = ring.st, t = (u.first + it) * kC;
-        if (it == 1 && has_init) {  // its stages are free once the state has been taken out
-          if (!mbar_wait(&m.init_read, 0)) {
-            bad = true;
-            break;
-          }
-        }
-        if (it >= kStages && !mbar_wait(&m.empty[st], ring.ph ^ 1)) {
+        // The stages after the first are free once the state has been taken out of them.
+        if ((it == 1 && has_init && !mbar_wait(&m.init_read, 0)) ||
+            (it >= kStages && !mbar_wait(&m.empty[ring.st], ring.ph ^ 1))) {
           bad = true;
           break;
         }
-        mbar_arrive_expect_tx(&m.full[st], boxes * kBox);
-        for (int x = 0; x < NK; ++x) {
-          tma_load_4d(sb + L::k + (st * NK + x) * kBox, &p.tm_k, &m.full[st], 64 * x, u.hk, t, u.b);
-          if (FULL) tma_load_4d(sb + L::q + (st * NK + x) * kBox, &p.tm_q, &m.full[st], 64 * x, u.hk, t, u.b);
-        }
-        tma_load_4d(sb + L::va(st), &p.tm_v, &m.full[st], 0, u.head0, t, u.b);
-        if (two)
-          tma_load_4d(sb + L::vb(st), &p.tm_v, &m.full[st], WIDE ? 64 : 0, WIDE ? u.head0 : u.head0 + 1, t, u.b);
+        load_chunk(u, it, ring.st);
         ++issued;
         if (it == 0 && has_init) {
           uint32_t bytes = 0;
@@ -462,7 +480,7 @@ __global__ void __launch_bounds__(kThreads, 1) linear_chunk_kernel(const __grid_
       }
       // No copy of this CTA may be in flight when it ends (also after a wait that gave up).
       for (int i = max(0, issued - kStages); i < issued; ++i) bad |= !mbar_wait(&m.full[i % kStages], (i / kStages) & 1);
-      if (issued > 0 && has_init) bad |= !mbar_wait(&m.init_full, 0);
+      if (has_init) bad |= !mbar_wait(&m.init_full, 0);
     } else if (warp == kStateMmaWarp) {
       // ---- products that need nothing of the state before --------------------------
       // The whole warp runs this, one lane issues: addresses stay in uniform registers.
@@ -564,28 +582,19 @@ __global__ void __launch_bounds__(kThreads, 1) linear_chunk_kernel(const __grid_
       bad = !ok;
     } else if (warp == kSumWarp) {
       // ---- decay sums -------------------------------------------------------------------
-      // A head has all lanes, or each of two heads half of them; a lane has kT neighbouring tokens.
-      constexpr int kT = WIDE ? 2 : 4, kLanes = kC / kT;
       const int x = lane / kLanes, tok = lane % kLanes * kT;
       const bool mine = x < u.nheads;
-      const float* g = l.decay + u.b * l.sg[0] + (u.head0 + (mine ? x : 0)) * l.sg[1];
-      float next[kT], seg_total = 0.f;
-      auto load_decays = [&](int it) {
-        const int t = (u.first + it) * kC + tok;
-#pragma unroll
-        for (int j = 0; j < kT; ++j) next[j] = mine && t + j < u.len ? g[static_cast<int64_t>(t + j) * l.sg[2]] : 0.f;
-      };
-      load_decays(0);
+      float seg_total = 0.f;
 #pragma unroll 1
       for (int it = 0; it < n_chunks; ++it) {
         const int sl = it % kSums, live = u.live(it);
         float c[kT], after[kT];
 #pragma unroll
         for (int j = 0; j < kT; ++j) {
-          const float a = next[j] * kLog2e;
+          const float a = decays[j] * kLog2e;
           c[j] = a < kMinLog2 ? kMinLog2 : a;  // NaN stays
         }
-        if (it + 1 < n_chunks) load_decays(it + 1);
+        if (it + 1 < n_chunks) load_decays(u, it + 1, decays);
         // Sums up to each token, and of those after it, without subtracting large sums.
         after[kT - 1] = 0.f;
 #pragma unroll
@@ -812,6 +821,7 @@ __global__ void __launch_bounds__(kThreads, 1) linear_chunk_kernel(const __grid_
       for (int i = 0; i < 3 * C::wv_bufs; ++i) tmem_st16(tm + C::wv + 32 * i + 16 * half + tl, z);
     }
     Ring<kStages> ring;
+    bool met = u.live(n_chunks - 1) == kC;  // at the barrier of a partial last chunk, if there is one
     for (int it = 0; it < n_chunks; ++it, ring.next()) {
       const int st = ring.st, sl = it % kSums, live = u.live(it), wb = it % C::wv_bufs;
       bad |= !mbar_wait(&m.full[st], ring.ph);
@@ -827,6 +837,7 @@ __global__ void __launch_bounds__(kThreads, 1) linear_chunk_kernel(const __grid_
         }
         fence_async_smem();
         bad = bar_or(2, 256, bad);
+        met = true;
       }
       if (__any_sync(0xffffffffu, bad)) {
         bad = true;
@@ -867,6 +878,7 @@ __global__ void __launch_bounds__(kThreads, 1) linear_chunk_kernel(const __grid_
       __syncwarp();
       if (lane == 0) mbar_arrive(&m.wv_ready[wb][half]);
     }
+    if (!met) bar_or(2, 256, true);
   } else {
     // ---- state ------------------------------------------------------------------------------
     more_registers<Regs<NK>::state>();
@@ -1009,7 +1021,7 @@ __global__ void __launch_bounds__(kThreads, 1) linear_chunk_kernel(const __grid_
       __threadfence_system();
     }
   }
-  if (warp == kLoadWarp) {
+  if (warp == kStateMmaWarp) {
     tc_fence_after();
     tmem_dealloc(tm, 512);
   }
