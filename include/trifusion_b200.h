@@ -541,10 +541,13 @@ int tf_rotary_positions_fwd(const void* q, const void* k, void* q_out, void* k_o
  * their outputs are zero. seqlen 1 is the single-token form.
  * `strides` holds 17 int64 element strides: q, k, v (batch, time, head), decay (batch,
  * head, time), out (batch, time, head), state (slot, head); innermost strides are 1
- * and the state is contiguous over [N,P]. `workspace` holds
- * tf_linear_attention_workspace_size bytes (256-byte aligned, contents irrelevant);
- * where that is not 0 the tokens run in chunks on the tensor cores if q, k, v and out lie on
- * 16-byte boundaries with strides that are multiples of 16 bytes, one by one otherwise. */
+ * and the state is contiguous over [N,P].
+ * BF16 pieces of 8 tokens or more with N and P up to 128 run in chunks of 64 tokens on the
+ * tensor cores (tf_linear_attention_chunked returns 1) if q, k, v and out lie on 16-byte
+ * boundaries with strides that are multiples of 16 bytes; all others token by token. The
+ * chunked form takes tf_linear_attention_workspace_size bytes of `workspace` (256-byte
+ * aligned, contents irrelevant; 0 where there are rows enough for all SMs). */
+int tf_linear_attention_chunked(int batch, int seqlen, int heads, int groups, int key_dim, int value_dim, int dtype);
 int64_t tf_linear_attention_workspace_size(int batch, int seqlen, int heads, int groups, int key_dim, int value_dim,
                                            int dtype);
 int tf_linear_attention_fwd(const void* q, const void* k, const void* v, int dtype, const float* decay, float* state,

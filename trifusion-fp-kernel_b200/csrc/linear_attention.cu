@@ -269,10 +269,15 @@ void launch_scan(const LinearParams& p, cudaStream_t stream) {
 
 extern "C" {
 
-int64_t tf_linear_attention_workspace_size(int batch, int seqlen, int heads, int groups, int key_dim, int value_dim,
-                                           int dtype) {
+int tf_linear_attention_chunked(int batch, int seqlen, int heads, int groups, int key_dim, int value_dim, int dtype) {
   if (batch <= 0 || seqlen <= 0 || heads <= 0 || groups <= 0 || heads % groups || key_dim <= 0 || value_dim <= 0)
     return 0;
+  return tf::linear_chunk_workspace(batch, seqlen, heads, groups, key_dim, value_dim, dtype) >= 0;
+}
+
+int64_t tf_linear_attention_workspace_size(int batch, int seqlen, int heads, int groups, int key_dim, int value_dim,
+                                           int dtype) {
+  if (!tf_linear_attention_chunked(batch, seqlen, heads, groups, key_dim, value_dim, dtype)) return 0;
   return tf::linear_chunk_workspace(batch, seqlen, heads, groups, key_dim, value_dim, dtype);
 }
 
@@ -309,7 +314,7 @@ int tf_linear_attention_fwd(const void* q, const void* k, const void* v, int dty
     return TF_ERR_SIZE;
   int st = check_device();
   if (st != TF_OK) return st;
-  if (linear_chunk_workspace(batch, seqlen, heads, groups, key_dim, value_dim, dtype) > 0) {
+  if (linear_chunk_workspace(batch, seqlen, heads, groups, key_dim, value_dim, dtype) >= 0) {
     st = launch_linear_chunks(p, dtype, workspace, workspace_bytes, static_cast<cudaStream_t>(stream));
     if (st >= 0) return st;
   }

@@ -22,7 +22,7 @@ struct LinearParams {
   float scale;
 };
 
-// The chunked form (linear_chunks.cu): bytes of workspace it takes, 0 where it does not
+// The chunked form (linear_chunks.cu): bytes of workspace it takes, -1 where it does not
 // apply; a launch of it, or -1 where a tensor's layout does not allow it.
 int64_t linear_chunk_workspace(int B, int T, int H, int Hq, int N, int P, int dtype);
 int launch_linear_chunks(const LinearParams& l, int dtype, void* workspace, int64_t workspace_bytes,

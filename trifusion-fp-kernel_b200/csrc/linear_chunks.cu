@@ -1127,7 +1127,7 @@ bool plan_of(int B, int T, int H, int Hq, int N, int P, int dtype, Plan& x) {
   x.seg_chunks = (x.chunks + x.segs - 1) / x.segs;
   x.segs = (x.chunks + x.seg_chunks - 1) / x.seg_chunks;
   x.state_bytes = x.segs > 1 ? static_cast<int64_t>(B) * H * x.segs * N * P * 4 : 0;
-  x.bytes = 256 + x.state_bytes + (x.segs > 1 ? static_cast<int64_t>(B) * H * x.segs * 4 : 0);
+  x.bytes = x.state_bytes + (x.segs > 1 ? static_cast<int64_t>(B) * H * x.segs * 4 : 0);
   return true;
 }
 
@@ -1159,7 +1159,7 @@ void launch_any(const ChunkParams& p, unsigned grid, cudaStream_t stream) {
 
 int64_t linear_chunk_workspace(int B, int T, int H, int Hq, int N, int P, int dtype) {
   Plan x;
-  return plan_of(B, T, H, Hq, N, P, dtype, x) ? x.bytes : 0;
+  return plan_of(B, T, H, Hq, N, P, dtype, x) ? x.bytes : -1;
 }
 
 int launch_linear_chunks(const LinearParams& l, int dtype, void* workspace, int64_t workspace_bytes,
@@ -1171,7 +1171,7 @@ int launch_linear_chunks(const LinearParams& l, int dtype, void* workspace, int6
       !encode(&p.tm_v, l.v, l.P, l.H, l.T, l.B, l.sv) || !encode(&p.tm_o, l.out, l.P, l.H, l.T, l.B, l.so, 32))
     return -1;
   if (x.rows * x.segs > 0x7fffffffll) return TF_ERR_SIZE;
-  if (!workspace || reinterpret_cast<uintptr_t>(workspace) % 256) return TF_ERR_ARG;
+  if (x.bytes > 0 && (!workspace || reinterpret_cast<uintptr_t>(workspace) % 256)) return TF_ERR_ARG;
   if (workspace_bytes < x.bytes) return TF_ERR_SIZE;
   p.l = l;
   p.pairs = x.pairs, p.chunks = x.chunks, p.segs = x.segs, p.seg_chunks = x.seg_chunks;

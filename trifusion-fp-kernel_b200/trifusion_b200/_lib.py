@@ -85,6 +85,7 @@ SIGNATURES = {
     "tf_decoder_heads_fwd": [_p] * 18 + [_q, _p, _i, _p],
     # Streaming operators.
     "tf_rotary_positions_fwd": [_p, _p, _p, _p, _i, _p, _p, _f, _i, _p, _i, _i, _i, _i, _i, _i, _p],
+    "tf_linear_attention_chunked": [_i] * 7,
     "tf_linear_attention_workspace_size": [_i] * 7,
     "tf_linear_attention_fwd": [_p, _p, _p, _i, _p, _p, _q, _i, _p, _p, _p, _p, _i, _i, _i, _i, _i, _i, _f, _p, _q,
                                 _p],

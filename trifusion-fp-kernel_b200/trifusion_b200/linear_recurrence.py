@@ -77,9 +77,12 @@ def _aligned(x):
     return not ((b > 1 and (sb % 8 or sb <= 0)) or (t > 1 and (st % 8 or st <= 0)) or (h > 1 and (sh % 8 or sh <= 0)))
 
 
-@functools.lru_cache(maxsize=1024)
-def _workspace_size(*sizes):
-    return _lib.lib().tf_linear_attention_workspace_size(*sizes)
+@functools.lru_cache(maxsize=4096)
+def _plan(device, *sizes):
+    """Whether a piece of these sizes runs in chunks, and the bytes of workspace it takes then."""
+    with torch.cuda.device(device):
+        lib = _lib.lib()
+        return lib.tf_linear_attention_chunked(*sizes), lib.tf_linear_attention_workspace_size(*sizes)
 
 
 def linear_attention(q, k, v, decay, state=None, *, slots=None, lengths=None, scale=None, out=None):
@@ -140,13 +143,14 @@ def linear_attention(q, k, v, decay, state=None, *, slots=None, lengths=None, sc
         ss = (h * n * p, n * p)
     _lib.error_watch()
     _lib.check_device_error()
-    nbytes = _workspace_size(b, t, h, hq, n, p, dtype)
+    chunked, nbytes = _plan(index, b, t, h, hq, n, p, dtype)
     work, into = None, out
-    if nbytes:  # the chunked form, whose tile loads need 16-byte rows
+    if chunked:  # its tile loads and stores need 16-byte rows
         q, k, v = [x if _aligned(x) else x.clone(memory_format=torch.contiguous_format) for x in (q, k, v)]
         if not _aligned(out):
             into = torch.empty((b, t, h, p), dtype=v.dtype, device=v.device)
-        work = torch.empty(nbytes, dtype=torch.uint8, device=v.device)
+        if nbytes:
+            work = torch.empty(nbytes, dtype=torch.uint8, device=v.device)
     _launch(index, q.data_ptr(), k.data_ptr(), v.data_ptr(), dtype, decay.data_ptr(), state.data_ptr(), state.shape[0],
             fresh, None if slots is None else slots.data_ptr(), None if lengths is None else lengths.data_ptr(),
             into.data_ptr(), _pack(*q.stride()[:3], *k.stride()[:3], *v.stride()[:3], *sg, *into.stride()[:3], *ss),
