@@ -69,6 +69,24 @@ def test_prompt_options_refused():
         linear_attention_step(*step(), STATE, out=torch.zeros(2, 4, 64))
 
 
+def test_written_arguments_refused():
+    """What is written to may not overlap itself, nor hang in a gradient's graph."""
+    out = torch.zeros(2, 1, 4, 64, dtype=torch.bfloat16)
+    with pytest.raises(ValueError, match="overlap"):
+        linear_attention(*prompt(), out=out.expand(2, 5, 4, 64))
+    with pytest.raises(ValueError, match="overlap"):
+        linear_attention_step(*step(), STATE, out=out[:1, 0].expand(2, 4, 64))
+    for kw in (dict(state=STATE.clone().requires_grad_()), dict(state=STATE, out=out[:, 0].clone().requires_grad_())):
+        with pytest.raises(RuntimeError, match="linear_attention_step: .*backward"):
+            linear_attention_step(*step(), **kw)
+    f, _ = rotary_frequencies(32, device="cpu")
+    x = torch.zeros(1, 3, 2, 64)
+    for q, k in ((x.expand(2, 3, 2, 64), x.repeat(2, 1, 1, 1)), (x, x[:, :, :1].expand(1, 3, 2, 64)),
+                 (x[:, :1].expand(1, 3, 2, 64), None)):
+        with pytest.raises(ValueError, match="overlap"):
+            apply_rotary(q, k, torch.arange(3), f, inplace=True)
+
+
 def test_cpu_tensors_fail_loudly():
     with pytest.raises(RuntimeError, match="CUDA tensors"):
         linear_attention(*prompt())
@@ -85,7 +103,7 @@ def test_rotary_refused():
     x = torch.zeros(1, 3, 2, 64)
     pos = torch.arange(3)
     bad = [
-        (ValueError, dict(layout="neox")), (ValueError, dict(q=x[0])), (ValueError, dict(k=x[:, :2])),
+        (ValueError, dict(layout="quarter")), (ValueError, dict(q=x[0])), (ValueError, dict(k=x[:, :2])),
         (TypeError, dict(k=x.bfloat16())), (TypeError, dict(q=x.double(), k=x.double())),
         (ValueError, dict(inv_freq=f.float())), (ValueError, dict(inv_freq=f[:0])),
         (ValueError, dict(q=x[..., :16], k=x[..., :16])), (ValueError, dict(positions=pos.int())),
@@ -97,7 +115,7 @@ def test_rotary_refused():
         with pytest.raises(error, match="apply_rotary"):
             apply_rotary(**args)
     for kw in (dict(rotary_dim=0), dict(rotary_dim=7), dict(rotary_dim=8, base=0.0), dict(rotary_dim=8, factor=0.0),
-               dict(rotary_dim=8, scaling="ntk"), dict(rotary_dim=8, scaling="parts", factor=2.0)):
+               dict(rotary_dim=8, scaling="square"), dict(rotary_dim=8, scaling="parts", factor=2.0)):
         with pytest.raises(ValueError, match="rotary_frequencies"):
             rotary_frequencies(device="cpu", **kw)
 
@@ -141,6 +159,11 @@ def test_c_abi_validates_on_the_host():
     assert attention(state=None, slots=buf) == attention(q=None) == attention(t=-1) == _lib.TF_ERR_ARG
     assert attention(b=0) == attention(h=0, hq=1) == attention(t=0) == _lib.TF_OK
     assert attention(state=ctypes.c_void_p(4100)) == _lib.TF_ERR_LAYOUT
+    sizes = dict(b=2, t=8, h=4, hq=2, n=128, p=64, dtype=1)
+    chunked = lambda **kw: lib.tf_linear_attention_chunked(*(sizes | kw).values())  # noqa: E731
+    assert chunked() == chunked(t=5000) == chunked(n=8, p=128) == 1
+    assert chunked(t=7) == chunked(dtype=0) == chunked(n=136) == chunked(p=136) == chunked(b=0) == chunked(hq=3) == 0
+    assert lib.tf_linear_attention_workspace_size(*(sizes | dict(t=7)).values()) == 0
     assert attention(strides=_lib.int64_array([8] * 15 + [6, 8])) == _lib.TF_ERR_LAYOUT
 
 

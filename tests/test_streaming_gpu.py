@@ -209,6 +209,24 @@ def test_decays_of_all_sizes(time):
     check(args, state)
 
 
+@pytest.mark.parametrize("time", [6, 7, 8, 9, 15, 16])
+@pytest.mark.parametrize("b", [1, 80])
+def test_short_prompts(time, b):
+    """Around the length from which pieces run in chunks."""
+    args, state = inputs(b, time, 6, 2, 64, 64, state=True)
+    check(args, state)
+
+
+@pytest.mark.parametrize("scale", [1e-12, -0.25, 1e12])
+@pytest.mark.parametrize("rate", [-2.4, -3.0])
+@pytest.mark.parametrize("n,p", [(64, 64), (128, 128)])
+def test_scales_with_strong_decays(scale, rate, n, p):
+    """Weights whose factors would leave FP32's range together with the scale."""
+    args, state = inputs(1, 130, 2, 1, n, p, state=True)
+    args[3][:] = rate
+    check(args, state, scale=scale)
+
+
 @pytest.mark.parametrize("time", [5, 300])
 def test_pool_with_slots(time):
     b, h, n, p, pool = 6, 4, 64, 64, 9
@@ -224,6 +242,46 @@ def test_pool_with_slots(time):
     assert (out[1] == 0).all() and out[3].isnan().all() and out[4].isnan().all()
     rest = [1, 2, 3, 5, 6, 7]
     assert torch.equal(big[rest], start[rest]) and torch.equal(big[:, h], start[:, h])
+
+
+@pytest.mark.parametrize("n,p", [(64, 64), (128, 128), (40, 24)])
+def test_long_ragged_rows_of_a_pool(n, p):
+    """Slots, lengths, a pool with a gap between its heads and an output off a 16-byte boundary,
+    on few rows (the time axis is shared out)."""
+    b, t, h, pool = 5, 1400, 2, 6
+    args, _ = inputs(b, t, h, 1, n, p, slow=0.01)
+    big = torch.randn(pool, h + 1, n, p, device=DEV)
+    start = big.clone()
+    slots = torch.tensor([5, 0, -1, 5, 3], device=DEV)
+    lengths = torch.tensor([1400, 0, 900, 300, 577], device=DEV)
+    out = torch.full((b, t, h, p + 4), 7.0, device=DEV, dtype=BF16)
+    linear_attention(*args, big[:, 1:], slots=slots, lengths=lengths, out=out[..., 4:])
+    good = [0, 1, 4]
+    ref, s, mag, smag = recurrence(*[x[good] for x in args], start[slots[good], 1:], lengths[good])
+    check_out(out[good][..., 4:], ref, mag, t, n, True)
+    check_state(big[slots[good], 1:], s, smag, t, n)
+    assert (out[..., :4] == 7).all() and (out[2, :, :, 4:] == 0).all()
+    assert out[3, :300, :, 4:].isnan().all() and (out[3, 300:, :, 4:] == 0).all()
+    rest = [0, 1, 2, 4]
+    assert torch.equal(big[rest], start[rest]) and torch.equal(big[:, 0], start[:, 0])
+
+
+def test_two_streams_at_once():
+    """Calls that share nothing but the device, on two streams without an order between them."""
+    work = [inputs(1, 4000, 4, 1, 128, 64, seed=s, state=True, slow=0.01) for s in (1, 2)]
+    alone = [linear_attention(*args, state.clone()) for args, state in work]
+    states = [[state.clone() for _ in range(6)] for _, state in work]
+    torch.cuda.synchronize()
+    got = [[], []]
+    streams = [torch.cuda.Stream() for _ in work]
+    for i in range(6):
+        for x, stream_ in enumerate(streams):
+            with torch.cuda.stream(stream_):
+                got[x].append(linear_attention(*work[x][0], states[x][i]))
+    torch.cuda.synchronize()
+    for x in range(2):
+        for out, state in got[x]:
+            assert torch.equal(out, alone[x][0]) and torch.equal(state, alone[x][1])
 
 
 @pytest.mark.parametrize("dtype", [BF16, FP32])

@@ -382,9 +382,6 @@ __global__ void __launch_bounds__(kThreads, 1) linear_chunk_kernel(const __grid_
     if (two)
       tma_load_4d(sb + L::vb(st), &p.tm_v, &m.full[st], WIDE ? 64 : 0, WIDE ? u.head0 : u.head0 + 1, t, u.b);
   };
-  // Chunks whose tiles need no waiting for. (The state lies where the second's would.)
-  
-
   // ---- set-up ------------------------------------------------------------------
   const Unit first_unit = unit_of<WIDE>(p, blockIdx.x);
   float decays[4] = {};  // the sum warp's first ones, on their way while the rest is set up
@@ -440,10 +437,7 @@ __global__ void __launch_bounds__(kThreads, 1) linear_chunk_kernel(const __grid_
       if (FULL && !dead && u.len == 0 && u.seg == 0 && l.fresh && l.state)
         for (int i = tid; i < u.nheads * l.N * l.P; i += kThreads)
           l.state[u.slot * l.ss[0] + (u.head0 + i / (l.N * l.P)) * l.ss[1] + i % (l.N * l.P)] = 0.f;
-      if (warp == kLoadWarp) {
-      } else if (warp == kStateMmaWarp) {
-        tmem_dealloc(m.tmem, 512);
-      }
+      if (warp == kStateMmaWarp) tmem_dealloc(m.tmem, 512);
       return;
     }
   }
@@ -613,13 +607,13 @@ __global__ void __launch_bounds__(kThreads, 1) linear_chunk_kernel(const __grid_
         const float total = __shfl_sync(0xffffffffu, r, 0, kLanes), mid = 0.5f * total;
         if (lane % kLanes == 0) before = 0.f;
         if (lane % kLanes == kLanes - 1) behind = 0.f;
-        // e^{c_i - c_j} as a product of two factors, where none leaves 2^+-120.
-        bool near = true;
+        // e^{c_i - c_j} as a product of two factors, where none leaves 2^+-120 (the scale's part: 2^+-20).
+        bool near = l.scale >= 0x1p-20f && l.scale <= 0x1p20f;
 #pragma unroll
         for (int j = 0; j < kT; ++j) {
           c[j] += before;
           after[j] += behind;
-          near = near && fabsf(c[j] - mid) <= 120.f;
+          near = near && fabsf(c[j] - mid) <= 100.f;
         }
         const uint32_t votes = __ballot_sync(0xffffffffu, near);
         const bool factors = WIDE ? votes == 0xffffffffu : (votes >> (16 * x) & 0xffffu) == 0xffffu;
@@ -1063,21 +1057,19 @@ __global__ void __launch_bounds__(256) linear_join_kernel(const __grid_constant_
 }
 
 // ---- host side ---------------------------------------------------------------------
-PFN_cuTensorMapEncodeTiled_v12000 g_encode = nullptr;
-int g_encode_looked = 0;
-
-bool encode_available() {
-  if (!g_encode_looked) {
-    void* fn = nullptr;
+// The driver's encoder of tensor maps, looked up once (also where several threads call first).
+PFN_cuTensorMapEncodeTiled_v12000 encoder() {
+  static const auto fn = [] {
+    void* p = nullptr;
     cudaDriverEntryPointQueryResult q{};
-    if (cudaGetDriverEntryPoint("cuTensorMapEncodeTiled", &fn, cudaEnableDefault, &q) == cudaSuccess &&
-        q == cudaDriverEntryPointSuccess)
-      g_encode = reinterpret_cast<PFN_cuTensorMapEncodeTiled_v12000>(fn);
-    else
+    if (cudaGetDriverEntryPoint("cuTensorMapEncodeTiled", &p, cudaEnableDefault, &q) != cudaSuccess ||
+        q != cudaDriverEntryPointSuccess) {
       (void)cudaGetLastError();
-    g_encode_looked = 1;
-  }
-  return g_encode != nullptr;
+      p = nullptr;
+    }
+    return reinterpret_cast<PFN_cuTensorMapEncodeTiled_v12000>(p);
+  }();
+  return fn;
 }
 
 // [B, T, heads, width] BF16 rows as a map with boxes of `side` tokens x `side` columns of one
@@ -1097,7 +1089,7 @@ bool encode(CUtensorMap* map, const void* base, int width, int heads, int T, int
     strides[i] = static_cast<cuuint64_t>(bytes);
   }
   const cuuint32_t box[4] = {side, 1, side, 1}, one[4] = {1, 1, 1, 1};
-  return g_encode(map, CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, 4, const_cast<void*>(base), dims, strides, box, one,
+  return encoder()(map, CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, 4, const_cast<void*>(base), dims, strides, box, one,
                   CU_TENSOR_MAP_INTERLEAVE_NONE,
                   side == 64 ? CU_TENSOR_MAP_SWIZZLE_128B : CU_TENSOR_MAP_SWIZZLE_64B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
                   CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
@@ -1165,7 +1157,7 @@ int64_t linear_chunk_workspace(int B, int T, int H, int Hq, int N, int P, int dt
 int launch_linear_chunks(const LinearParams& l, int dtype, void* workspace, int64_t workspace_bytes,
                          cudaStream_t stream) {
   Plan x;
-  if (!plan_of(l.B, l.T, l.H, l.Hq, l.N, l.P, dtype, x) || !encode_available()) return -1;
+  if (!plan_of(l.B, l.T, l.H, l.Hq, l.N, l.P, dtype, x) || !encoder()) return -1;
   ChunkParams p{};
   if (!encode(&p.tm_q, l.q, l.N, l.Hq, l.T, l.B, l.sq) || !encode(&p.tm_k, l.k, l.N, l.Hq, l.T, l.B, l.sk) ||
       !encode(&p.tm_v, l.v, l.P, l.H, l.T, l.B, l.sv) || !encode(&p.tm_o, l.out, l.P, l.H, l.T, l.B, l.so, 32))

@@ -51,6 +51,8 @@ def _check_state(op, state, slots, b, h, n, p):
         raise ValueError(f"{op}: state must be contiguous over [N,P], its heads on 16-byte boundaries")
     if (s1 < n * p and h > 1) or (s0 < n * p and state.shape[0] > 1):
         raise ValueError(f"{op}: the states of a pool must not overlap")
+    if state.requires_grad and torch.is_grad_enabled():
+        raise RuntimeError(f"{op}: {_lib.NO_GRADIENT}")
     if slots is None:
         if state.shape[0] != b:
             raise ValueError(f"{op}: without slots, state must have one entry for each row")
@@ -62,6 +64,10 @@ def _check_state(op, state, slots, b, h, n, p):
 def _check_out(op, out, v):
     if out.shape != v.shape or out.dtype != v.dtype or out.stride(-1) != 1:
         raise ValueError(f"{op}: out must be like v with a unit stride in the last dimension")
+    if any(s == 0 and n > 1 for s, n in zip(out.stride(), out.shape)):
+        raise ValueError(f"{op}: out must not overlap itself")
+    if out.requires_grad and torch.is_grad_enabled():
+        raise RuntimeError(f"{op}: {_lib.NO_GRADIENT}")
 
 
 def _check_device(op, index, *tensors):
@@ -100,12 +106,13 @@ def linear_attention(q, k, v, decay, state=None, *, slots=None, lengths=None, sc
     * ``lengths`` (int64 [B], on the device): tokens at or past a row's length are not
       read, and their output is zero.
     * ``scale`` defaults to ``N ** -0.5``; ``out``: a preallocated output like v with a unit
-      stride in the last dimension.
+      stride in the last dimension. ``out`` and ``state`` overlap no other argument.
 
     BF16 operands with N and P up to 128 run on the tensor cores in chunks of 64 tokens
-    (FP32 sums and state); a non-finite value in v or k then also reaches the earlier
-    tokens of its chunk. FP32 operands, wider heads and short pieces run token by token.
-    There is no backward pass.
+    (FP32 sums and state). A non-finite value in v then also reaches the earlier tokens of
+    its chunk, and, with P up to 64, a non-finite weight (a NaN in a head's decays, say) the
+    outputs of the head next to it under the same key head. FP32 operands, wider heads and
+    pieces of fewer than 8 tokens run token by token. There is no backward pass.
     """
     op = "linear_attention"
     shape = q.shape

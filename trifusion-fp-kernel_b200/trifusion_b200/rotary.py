@@ -60,14 +60,19 @@ def rotary_frequencies(rotary_dim, base=10000.0, *, scaling=None, factor=1.0, tr
     return freq.to(device), amplitude
 
 
+def _repeats(x):
+    return any(step == 0 and n > 1 for step, n in zip(x.stride(), x.shape))
+
+
 def apply_rotary(q, k, positions, inv_freq, *, layout="half", amplitude=1.0, inplace=False):
     """Rotate ``q`` ([B, T, H, D]) and ``k`` ([B, T, Hk, D], or None) by ``positions * inv_freq``.
 
-    ``positions`` is int64 [B, T] or [T], any values; ``inv_freq`` FP64 [R/2] with
-    ``R <= D``: elements R.. of each head are copied. Pairs are ``(i, i + R/2)`` (``layout
-    "half"``) or ``(2 i, 2 i + 1)`` (``"interleaved"``); a pair becomes ``amplitude * (x1 cos -
-    x2 sin, x2 cos + x1 sin)``. q and k are FP32 or BF16 with any strides, the last one 1.
-    Returns new contiguous tensors, or the arguments themselves when ``inplace``.
+    ``positions`` is int64 [B, T] or [T], any values (angles at 2^31 are within 1e-7 turns);
+    ``inv_freq`` FP64 [R/2] with ``R <= D``: elements R.. of each head are copied. Pairs are
+    ``(i, i + R/2)`` (``layout "half"``) or ``(2 i, 2 i + 1)`` (``"interleaved"``); a pair becomes ``amplitude * (x1 cos -
+    x2 sin, x2 cos + x1 sin)``. q and k are FP32 or BF16 with any strides; R is at most 1024 and
+    ``(H + Hk) * D`` at most 65535. Returns new contiguous tensors, or the arguments themselves
+    when ``inplace`` (last stride 1, q and k apart from each other). There is no backward pass.
     """
     interleaved = _LAYOUTS.get(layout)
     if interleaved is None:
@@ -93,6 +98,11 @@ def apply_rotary(q, k, positions, inv_freq, *, layout="half", amplitude=1.0, inp
         raise ValueError("apply_rotary: inv_freq must be float64 [R/2] with 2 <= R <= D")
     if positions.dtype != torch.int64 or tuple(positions.shape) not in ((b, t), (t,)):
         raise ValueError("apply_rotary: positions must be int64 [B,T] or [T]")
+    if inplace:
+        if q.stride(3) != 1 or k is not None and k.stride(3) != 1:
+            raise ValueError("apply_rotary: in place needs a unit stride in the last dimension")
+        if _repeats(q) or k is not None and _repeats(k):
+            raise ValueError("apply_rotary: in place needs tensors that do not overlap themselves")
     if grad and torch.is_grad_enabled():
         raise RuntimeError("apply_rotary: " + _lib.NO_GRADIENT)
     if index < 0 or not same or positions.get_device() != index or inv_freq.get_device() != index:
@@ -105,8 +115,6 @@ def apply_rotary(q, k, positions, inv_freq, *, layout="half", amplitude=1.0, inp
     if k is not None:
         k0, k1, k2, k3 = k.stride()
     if inplace:
-        if q3 != 1 or k3 != 1:
-            raise ValueError("apply_rotary: in place needs a unit stride in the last dimension")
         qo, ko, p0, p1, p2, o0, o1, o2 = q, k, q0, q1, q2, k0, k1, k2
     else:
         if q3 != 1:
