@@ -138,30 +138,45 @@ def linear_attention(q, k, v, decay, state=None, *, slots=None, lengths=None, sc
     if out is not None:
         _check_out(op, out, v)
     _check_device(op, index, k, v, decay, state, slots, lengths, out)
-    q, k, v = [x if x.stride(3) == 1 else x.contiguous() for x in (q, k, v)]
-    if slots is not None:
-        slots = slots.contiguous()
-    if lengths is not None:
-        lengths = lengths.contiguous()
+    q0, q1, q2, q3 = q.stride()
+    k0, k1, k2, k3 = k.stride()
+    v0, v1, v2, v3 = v.stride()
+    if q3 != 1 or k3 != 1 or v3 != 1:
+        q, k, v = [x if x.stride(3) == 1 else x.contiguous() for x in (q, k, v)]
+        (q0, q1, q2, _), (k0, k1, k2, _), (v0, v1, v2, _) = q.stride(), k.stride(), v.stride()
     if out is None:
-        out = torch.empty_like(v, memory_format=torch.contiguous_format)
+        out, o0, o1, o2 = torch.empty_like(v, memory_format=torch.contiguous_format), t * h * p, h * p, p
+    else:
+        o0, o1, o2, _ = out.stride()
     if fresh:
         state = torch.empty((b, h, n, p), dtype=torch.float32, device=v.device)
         ss = (h * n * p, n * p)
-    _lib.error_watch()
+    if not _lib._watch["ready"]:
+        _lib.error_watch()
     _lib.check_device_error()
     chunked, nbytes = _plan(index, b, t, h, hq, n, p, dtype)
-    work, into = None, out
+    work, slot, length, into = None, None, None, out
+    qp, kp, vp, outp = q.data_ptr(), k.data_ptr(), v.data_ptr(), out.data_ptr()
     if chunked:  # its tile loads and stores need 16-byte rows
-        q, k, v = [x if _aligned(x) else x.clone(memory_format=torch.contiguous_format) for x in (q, k, v)]
-        if not _aligned(out):
-            into = torch.empty((b, t, h, p), dtype=v.dtype, device=v.device)
+        strides = (q0, q1, q2, k0, k1, k2, v0, v1, v2, o0, o1, o2)
+        if (qp | kp | vp | outp) & 15 or (q0 | q1 | q2 | k0 | k1 | k2 | v0 | v1 | v2 | o0 | o1 | o2) & 7 or min(strides) <= 0:
+            q, k, v = [x if _aligned(x) else x.clone(memory_format=torch.contiguous_format) for x in (q, k, v)]
+            if not _aligned(out):
+                into = torch.empty((b, t, h, p), dtype=v.dtype, device=v.device)
+            (q0, q1, q2, _), (k0, k1, k2, _), (v0, v1, v2, _) = q.stride(), k.stride(), v.stride()
+            o0, o1, o2, _ = into.stride()
+            qp, kp, vp, outp = q.data_ptr(), k.data_ptr(), v.data_ptr(), into.data_ptr()
         if nbytes:
             work = torch.empty(nbytes, dtype=torch.uint8, device=v.device)
-    _launch(index, q.data_ptr(), k.data_ptr(), v.data_ptr(), dtype, decay.data_ptr(), state.data_ptr(), state.shape[0],
-            fresh, None if slots is None else slots.data_ptr(), None if lengths is None else lengths.data_ptr(),
-            into.data_ptr(), _pack(*q.stride()[:3], *k.stride()[:3], *v.stride()[:3], *sg, *into.stride()[:3], *ss),
-            b, t, h, hq, n, p, n ** -0.5 if scale is None else scale, None if work is None else work.data_ptr(), nbytes)
+    if slots is not None:
+        slots = slots.contiguous()
+        slot = slots.data_ptr()
+    if lengths is not None:
+        lengths = lengths.contiguous()
+        length = lengths.data_ptr()
+    _launch(index, qp, kp, vp, dtype, decay.data_ptr(), state.data_ptr(), state.shape[0], fresh, slot, length, outp,
+            _pack(q0, q1, q2, k0, k1, k2, v0, v1, v2, *sg, o0, o1, o2, *ss), b, t, h, hq, n, p,
+            n ** -0.5 if scale is None else scale, None if work is None else work.data_ptr(), nbytes)
     if into is not out:
         out.copy_(into)
     return out, state
