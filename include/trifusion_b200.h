@@ -542,7 +542,7 @@ int tf_rotary_positions_fwd(const void* q, const void* k, void* q_out, void* k_o
  * `strides` holds 17 int64 element strides: q, k, v (batch, time, head), decay (batch,
  * head, time), out (batch, time, head), state (slot, head); innermost strides are 1
  * and the state is contiguous over [N,P].
- * BF16 pieces of 8 tokens or more with N and P up to 128 run in chunks of 64 tokens on the
+ * BF16 pieces of 17 tokens or more with N and P up to 128 run in chunks of 64 tokens on the
  * tensor cores (tf_linear_attention_chunked returns 1) if q, k, v and out lie on 16-byte
  * boundaries with strides that are multiples of 16 bytes; all others token by token. The
  * chunked form takes tf_linear_attention_workspace_size bytes of `workspace` (256-byte

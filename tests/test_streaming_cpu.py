@@ -159,11 +159,11 @@ def test_c_abi_validates_on_the_host():
     assert attention(state=None, slots=buf) == attention(q=None) == attention(t=-1) == _lib.TF_ERR_ARG
     assert attention(b=0) == attention(h=0, hq=1) == attention(t=0) == _lib.TF_OK
     assert attention(state=ctypes.c_void_p(4100)) == _lib.TF_ERR_LAYOUT
-    sizes = dict(b=2, t=8, h=4, hq=2, n=128, p=64, dtype=1)
+    sizes = dict(b=2, t=17, h=4, hq=2, n=128, p=64, dtype=1)
     chunked = lambda **kw: lib.tf_linear_attention_chunked(*(sizes | kw).values())  # noqa: E731
     assert chunked() == chunked(t=5000) == chunked(n=8, p=128) == 1
-    assert chunked(t=7) == chunked(dtype=0) == chunked(n=136) == chunked(p=136) == chunked(b=0) == chunked(hq=3) == 0
-    assert lib.tf_linear_attention_workspace_size(*(sizes | dict(t=7)).values()) == 0
+    assert chunked(t=16) == chunked(dtype=0) == chunked(n=136) == chunked(p=136) == chunked(b=0) == chunked(hq=3) == 0
+    assert lib.tf_linear_attention_workspace_size(*(sizes | dict(t=16)).values()) == 0
     assert attention(strides=_lib.int64_array([8] * 15 + [6, 8])) == _lib.TF_ERR_LAYOUT
 
 

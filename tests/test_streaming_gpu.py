@@ -209,7 +209,7 @@ def test_decays_of_all_sizes(time):
     check(args, state)
 
 
-@pytest.mark.parametrize("time", [6, 7, 8, 9, 15, 16])
+@pytest.mark.parametrize("time", [7, 8, 9, 15, 16, 17, 18])
 @pytest.mark.parametrize("b", [1, 80])
 def test_short_prompts(time, b):
     """Around the length from which pieces run in chunks."""

@@ -25,131 +25,173 @@ __device__ __forceinline__ void st_f(bf16* p, float x) { *p = __float2bfloat16_r
 __device__ __forceinline__ float decay_factor(float g) { return ex2_approx(g * kLog2e); }
 
 // ---- recurrent form ------------------------------------------------------------
-// One block: one row, one head, 32 columns of its state. Thread (warp w, lane l)
-// holds columns 4 (l % 8) .. +3 of state rows w * 4 + l / 8 + 32 i, so a warp reads
-// four 128-byte row segments at a time, and the sum over rows for the output is
-// two shuffles and eight partial sums in shared memory. A single token is bound by
-// the state's bytes (read once, written once); a block has 16 KB of them in flight
-// at N = 128.
-constexpr int kScanThreads = 256;
-
-template <typename T, int NR>
-__global__ void __launch_bounds__(kScanThreads) linear_scan_kernel(const __grid_constant__ LinearParams p) {
-  __shared__ float4 partial[2][8][8];
+// One block: one row, one head, 32 columns of its state. Thread (warp w, lane l) holds columns
+// 4 (l % 8) .. +3 of the NR rows from (4 w + l / 8) NR on: a token's q, k and v are wide reads of
+// shared memory, its output three shuffles (each halves what a lane still sums) and a partial sum
+// of each warp. Tokens come in batches: while one is worked on, the next one's operands are in shared
+// memory and those of the one after it on their way to registers, and a batch takes one barrier,
+// behind which every warp sums up the output of some of its tokens. Bound by issue and, with few blocks, by the latency of a token's chain.
+// Where a block has an SM to itself, or shares it with one other, eight warps with a whole batch
+// unrolled are faster, else four warps with half of it (fewer instructions for a token). FP32, us:
+//   2 x 3600 tokens, 12 heads, N 128, P 64     48 blocks     eight 510   four  724
+//   1 x 7, 12 heads, N 128, P 64               24 blocks     eight 4.6   four  4.7
+//   8 x 4097, 32 heads, N 64, P 64            512 blocks     eight 1435  four 1090
+//   32 x 7, 32 heads, N 128, P 64            2048 blocks     eight 29.2  four 22.4
+// (The first with a barrier for every token: 1058 us; a column a lane: 800 us; the next batch
+// loaded while one is worked on, not two: 694 us.)
+template <typename T, int NR, int WARPS>
+__global__ void __launch_bounds__(32 * WARPS, NR == 8 ? 4 : 2) linear_scan_kernel(const __grid_constant__ LinearParams p) {
+  constexpr int kThreads = 32 * WARPS, kRows = 4 * WARPS * NR;
+  constexpr int kBatch = kRows > 128 ? 4 : 8;  // tokens
+  constexpr int kOwn = kBatch / WARPS;         // of them a warp brings the v, and sums up the output
+  constexpr int kLoads = kBatch * kRows / kThreads;  // of q, and of k, by a thread
+  constexpr int kUnroll = WARPS == 8 ? kBatch : 4;
+  static_assert(kBatch % WARPS == 0 && kBatch * kRows % kThreads == 0, "a batch is shared out evenly");
+  __shared__ alignas(16) float kq[2][kBatch][2][kRows];
+  __shared__ alignas(16) float vs[2][kBatch][32];
+  __shared__ float as[2][kBatch], partial[2][kBatch][WARPS][32];
   const int slices = (p.P + 31) / 32;
   const int slice = blockIdx.x % slices;
   const int row = blockIdx.x / slices;
   const int h = row % p.H, b = row / p.H;
   const int w = threadIdx.x >> 5, lane = threadIdx.x & 31;
-  const int col = slice * 32 + 4 * (lane & 7);
-  const int r0 = w * 4 + (lane >> 3);
+  const int r0 = (4 * w + (lane >> 3)) * NR, c0 = slice * 32 + 4 * (lane & 7);  // of the state
+  const int col = slice * 32 + lane;  // of v and the output
   const bool on = col < p.P;
 
   const int64_t slot = p.slots ? p.slots[b] : b;
   const bool in_pool = p.state && slot >= 0 && slot < p.nslots;
-  float* st = p.state + (in_pool ? slot * p.ss[0] + h * p.ss[1] : 0);
-  float4 s[NR];
+  float* st = p.state + (in_pool ? slot * p.ss[0] + h * p.ss[1] + static_cast<int64_t>(r0) * p.P + c0 : 0);
+  float2 s[4][NR / 2];  // [column][pair of rows]
 #pragma unroll
   for (int i = 0; i < NR; ++i) {
-    const int n = r0 + 32 * i;
-    s[i] = in_pool && !p.fresh && on && n < p.N ? *reinterpret_cast<const float4*>(st + static_cast<int64_t>(n) * p.P + col)
-                                                : make_float4(0.f, 0.f, 0.f, 0.f);
+    const float4 x = in_pool && !p.fresh && c0 < p.P && r0 + i < p.N ? *reinterpret_cast<const float4*>(st + i * p.P)
+                                                                     : make_float4(0.f, 0.f, 0.f, 0.f);
+    (i % 2 ? s[0][i / 2].y : s[0][i / 2].x) = x.x;
+    (i % 2 ? s[1][i / 2].y : s[1][i / 2].x) = x.y;
+    (i % 2 ? s[2][i / 2].y : s[2][i / 2].x) = x.z;
+    (i % 2 ? s[3][i / 2].y : s[3][i / 2].x) = x.w;
   }
   bool taken = false;  // an earlier row has this slot
   if (p.slots) {
     if (in_pool)
-      for (int i = threadIdx.x; i < b; i += kScanThreads) taken |= p.slots[i] == slot;
+      for (int i = threadIdx.x; i < b; i += kThreads) taken |= p.slots[i] == slot;
     taken = __syncthreads_or(taken);
   }
   int64_t len = p.T;
   if (p.lengths) len = min(max(p.lengths[b], static_cast<int64_t>(0)), len);
-  T* out = static_cast<T*>(p.out) + b * p.so[0] + h * p.so[2];
+  T* out = static_cast<T*>(p.out) + b * p.so[0] + h * p.so[2] + col;
   if (p.state && (!in_pool || taken)) {
     // No state of its own: zeros for a row that is padding, NaN for one that names a wrong slot.
-    if (w == 0) {
-      const float fill = slot < 0 ? 0.f : __int_as_float(0x7fc00000);
-      const int c = slice * 32 + lane;
-      if (c < p.P)
-        for (int64_t t = 0; t < p.T; ++t) st_f(out + t * p.so[1] + c, t < len ? fill : 0.f);
-    }
+    const float fill = slot < 0 ? 0.f : __int_as_float(0x7fc00000);
+    if (on)
+      for (int64_t t = w; t < p.T; t += WARPS) st_f(out + t * p.so[1], t < len ? fill : 0.f);
     return;
   }
   const int hq = h / (p.H / p.Hq);
   const T* q = static_cast<const T*>(p.q) + b * p.sq[0] + hq * p.sq[2];
   const T* k = static_cast<const T*>(p.k) + b * p.sk[0] + hq * p.sk[2];
-  const T* v = static_cast<const T*>(p.v) + b * p.sv[0] + h * p.sv[2];
+  const T* v = static_cast<const T*>(p.v) + b * p.sv[0] + h * p.sv[2] + col;
   const float* g = p.decay + b * p.sg[0] + h * p.sg[1];
-  // One token's operands, loaded while the one before is worked on.
-  float gn = 0.f, vn[4] = {}, kn[NR] = {}, qn[NR] = {};
-  auto load = [&](int64_t t) {
-    if (t >= len) return;
-    gn = g[t * p.sg[2]];
+  // What a thread brings of the batch from t0 on. Tokens past the length change nothing: zeros, and
+  // no decay.
+  float kn[kLoads], qn[kLoads], vn[kOwn], gn;
+  auto load = [&](int64_t t0) {
 #pragma unroll
-    for (int j = 0; j < 4; ++j)
-      if (on) vn[j] = ld_f(v + t * p.sv[1] + col + j);
-#pragma unroll
-    for (int i = 0; i < NR; ++i) {
-      const int n = r0 + 32 * i;
-      if (n < p.N) kn[i] = ld_f(k + t * p.sk[1] + n), qn[i] = ld_f(q + t * p.sq[1] + n);
+    for (int j = 0; j < kLoads; ++j) {
+      const int i = threadIdx.x + j * kThreads, n = i % kRows;
+      const int64_t t = t0 + i / kRows;
+      const bool live = t < len && n < p.N;
+      kn[j] = live ? ld_f(k + t * p.sk[1] + n) : 0.f;
+      qn[j] = live ? ld_f(q + t * p.sq[1] + n) : 0.f;
     }
+#pragma unroll
+    for (int j = 0; j < kOwn; ++j) {
+      const int64_t t = t0 + w * kOwn + j;
+      vn[j] = t < len && on ? ld_f(v + t * p.sv[1]) : 0.f;
+    }
+    gn = threadIdx.x < kBatch && t0 + threadIdx.x < len ? g[(t0 + threadIdx.x) * p.sg[2]] : 0.f;
+  };
+  auto store = [&](int x) {
+#pragma unroll
+    for (int j = 0; j < kLoads; ++j) {
+      const int i = threadIdx.x + j * kThreads;
+      kq[x][i / kRows][0][i % kRows] = kn[j], kq[x][i / kRows][1][i % kRows] = qn[j];
+    }
+#pragma unroll
+    for (int j = 0; j < kOwn; ++j) vs[x][w * kOwn + j][lane] = vn[j];
+    if (threadIdx.x < kBatch) as[x][threadIdx.x] = decay_factor(gn);
   };
   load(0);
-  for (int64_t t = 0; t < len; ++t) {
-    const float a = decay_factor(gn);
-    float vv[4], kk[NR], qq[NR];
+  store(0);
+  load(kBatch);
+  __syncthreads();
+  int x = 0;
+  for (int64_t t0 = 0; t0 < len; t0 += kBatch, x ^= 1) {
+    store(x ^ 1);
+    load(t0 + 2 * kBatch);
+#pragma unroll (kUnroll)
+    for (int t = 0; t < kBatch; ++t) {
+      const float2 a = make_float2(as[x][t], as[x][t]);
+      const float4 vr = *reinterpret_cast<const float4*>(&vs[x][t][4 * (lane & 7)]);
+      const float2 vv[4] = {make_float2(vr.x, vr.x), make_float2(vr.y, vr.y), make_float2(vr.z, vr.z),
+                            make_float2(vr.w, vr.w)};
+      float2 o[4] = {};
 #pragma unroll
-    for (int j = 0; j < 4; ++j) vv[j] = vn[j];
+      for (int i = 0; i < NR / 2; ++i) {
+        const float2 kk = *reinterpret_cast<const float2*>(&kq[x][t][0][r0 + 2 * i]);
+        const float2 qq = *reinterpret_cast<const float2*>(&kq[x][t][1][r0 + 2 * i]);
 #pragma unroll
-    for (int i = 0; i < NR; ++i) kk[i] = kn[i], qq[i] = qn[i];
-    load(t + 1);
-    float4 o = make_float4(0.f, 0.f, 0.f, 0.f);
+        for (int c = 0; c < 4; ++c) {
+          s[c][i] = fma2(kk, vv[c], mul2(a, s[c][i]));
+          o[c] = fma2(qq, s[c][i], o[c]);
+        }
+      }
+      const bool hi = lane & 8, top = lane & 16;
+      float y[4];
 #pragma unroll
-    for (int i = 0; i < NR; ++i) {
-      s[i].x = fmaf(kk[i], vv[0], a * s[i].x);
-      s[i].y = fmaf(kk[i], vv[1], a * s[i].y);
-      s[i].z = fmaf(kk[i], vv[2], a * s[i].z);
-      s[i].w = fmaf(kk[i], vv[3], a * s[i].w);
-      o.x = fmaf(qq[i], s[i].x, o.x);
-      o.y = fmaf(qq[i], s[i].y, o.y);
-      o.z = fmaf(qq[i], s[i].z, o.z);
-      o.w = fmaf(qq[i], s[i].w, o.w);
+      for (int c = 0; c < 4; ++c) y[c] = o[c].x + o[c].y;
+      float y0 = hi ? y[2] : y[0], y1 = hi ? y[3] : y[1];
+      y0 += __shfl_xor_sync(0xffffffffu, hi ? y[0] : y[2], 8);
+      y1 += __shfl_xor_sync(0xffffffffu, hi ? y[1] : y[3], 8);
+      const float z = __shfl_xor_sync(0xffffffffu, top ? y0 : y1, 16) + (top ? y1 : y0);
+      partial[x][t][w][4 * (lane & 7) + (hi ? 2 : 0) + (top ? 1 : 0)] = z;
     }
-#pragma unroll
-    for (int d = 8; d < 32; d <<= 1) {
-      o.x += __shfl_xor_sync(0xffffffffu, o.x, d);
-      o.y += __shfl_xor_sync(0xffffffffu, o.y, d);
-      o.z += __shfl_xor_sync(0xffffffffu, o.z, d);
-      o.w += __shfl_xor_sync(0xffffffffu, o.w, d);
-    }
-    if (lane < 8) partial[t & 1][w][lane] = o;
     __syncthreads();
-    if (w == 0) {
-      const float* f = reinterpret_cast<const float*>(&partial[t & 1][0][0]);
-      float sum = 0.f;
+    if (on) {
 #pragma unroll
-      for (int i = 0; i < 8; ++i) sum += f[32 * i + lane];
-      const int c = slice * 32 + lane;
-      if (c < p.P) st_f(out + t * p.so[1] + c, sum * p.scale);
+      for (int j = 0; j < kOwn; ++j) {
+        const int t = w * kOwn + j;
+        float sum = 0.f;
+#pragma unroll
+        for (int i = 0; i < WARPS; ++i) sum += partial[x][t][i][lane];
+        if (t0 + t < len) st_f(out + (t0 + t) * p.so[1], sum * p.scale);
+      }
     }
   }
-  if (w == 0 && slice * 32 + lane < p.P)
-    for (int64_t t = len; t < p.T; ++t) st_f(out + t * p.so[1] + slice * 32 + lane, 0.f);
-  if (p.state && on && (len > 0 || p.fresh))
+  if (on)
+    for (int64_t t = len + w; t < p.T; t += WARPS) st_f(out + t * p.so[1], 0.f);
+  if (p.state && c0 < p.P && (len > 0 || p.fresh))
 #pragma unroll
-    for (int i = 0; i < NR; ++i) {
-      const int n = r0 + 32 * i;
-      if (n < p.N) *reinterpret_cast<float4*>(st + static_cast<int64_t>(n) * p.P + col) = s[i];
-    }
+    for (int i = 0; i < NR; ++i)
+      if (r0 + i < p.N) {
+        auto at = [&](int c) { return i % 2 ? s[c][i / 2].y : s[c][i / 2].x; };
+        *reinterpret_cast<float4*>(st + i * p.P) = make_float4(at(0), at(1), at(2), at(3));
+      }
 }
 
-// The same for one token, without what a loop over tokens needs, on up to CS times 32 columns,
-// so that a block has 16 KB of state on its way where N <= 128. Bound by HBM: the states are
+constexpr int kStepThreads = 256;
+
+// One token. Thread (warp w, lane l) holds columns 4 (l % 8) .. +3 of state rows w * 4 + l / 8 +
+// 32 i, on up to CS times 32 columns, so that a warp reads four 128-byte row segments at a time, a
+// block has 16 KB of state on its way where N <= 128, and the sum over rows for the output is two
+// shuffles and eight partial sums in shared memory. Bound by HBM: the states are
 // read and written once. They are streamed (evict-first): larger pools than the L2 would only
 // push each other out, smaller ones stay in it all the same. 64 rows of 32 heads, 128 x 128:
 // 43.4 us (268 MB, 94 % of the measured copy rate); 48.0 us with ordinary accesses, 45.1 and
 // 46.6 us with four and six blocks an SM instead of five.
 template <typename T, int NR, int CS>
-__global__ void __launch_bounds__(kScanThreads, NR > 4 ? 3 : NR == 4 ? 5 : CS == 1 ? 6 : 4)
+__global__ void __launch_bounds__(kStepThreads, NR > 4 ? 3 : NR == 4 ? 5 : CS == 1 ? 6 : 4)
     linear_step_kernel(const __grid_constant__ LinearParams p) {
   __shared__ float4 partial[CS][8][8];
   const int slices = (p.P + 32 * CS - 1) / (32 * CS);
@@ -188,7 +230,7 @@ __global__ void __launch_bounds__(kScanThreads, NR > 4 ? 3 : NR == 4 ? 5 : CS ==
   const float a = decay_factor(p.decay[b * p.sg[0] + h * p.sg[1]]);
   bool dead = !in_pool;  // no state of its own
   if (p.slots) {
-    for (int i = threadIdx.x; i < b; i += kScanThreads) dead |= p.slots[i] == slot;
+    for (int i = threadIdx.x; i < b; i += kStepThreads) dead |= p.slots[i] == slot;
     dead = __syncthreads_or(dead);
   }
   float4 o[CS];
@@ -239,7 +281,7 @@ __global__ void __launch_bounds__(kScanThreads, NR > 4 ? 3 : NR == 4 ? 5 : CS ==
   }
 }
 
-template <typename T, int NR>
+template <typename T, int NR>  // N <= 32 NR
 void launch_rows(const LinearParams& p, cudaStream_t stream) {
   const int64_t rows = static_cast<int64_t>(p.B) * p.H;
   if (p.T == 1 && p.state && !p.fresh && !p.lengths) {
@@ -247,13 +289,18 @@ void launch_rows(const LinearParams& p, cudaStream_t stream) {
     auto step = [&](auto cs) {
       constexpr int CS = decltype(cs)::value;
       linear_step_kernel<T, NR, CS>
-          <<<static_cast<unsigned>(rows * ((p.P + 32 * CS - 1) / (32 * CS))), kScanThreads, 0, stream>>>(p);
+          <<<static_cast<unsigned>(rows * ((p.P + 32 * CS - 1) / (32 * CS))), kStepThreads, 0, stream>>>(p);
     };
     if (NR == 1 && p.P > 64) step(std::integral_constant<int, NR == 1 ? 4 : 1>());
     else if (NR <= 2 && p.P > 32) step(std::integral_constant<int, NR <= 2 ? 2 : 1>());
     else step(std::integral_constant<int, 1>());
   } else {
-    linear_scan_kernel<T, NR><<<static_cast<unsigned>(rows * ((p.P + 31) / 32)), kScanThreads, 0, stream>>>(p);
+    auto scan = [&](auto warps) {
+      constexpr int W = decltype(warps)::value, R = 8 * NR / W < 2 ? 2 : 8 * NR / W;
+      linear_scan_kernel<T, R, W><<<static_cast<unsigned>(rows * ((p.P + 31) / 32)), 32 * W, 0, stream>>>(p);
+    };
+    if (NR <= 4 && rows * ((p.P + 31) / 32) <= 2 * sm_count()) scan(std::integral_constant<int, NR <= 4 ? 8 : 4>());
+    else scan(std::integral_constant<int, 4>());
   }
 }
 template <typename T>

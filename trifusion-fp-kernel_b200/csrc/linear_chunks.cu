@@ -29,6 +29,19 @@
 // Long rows on few heads: the time axis is cut into segments. One launch forms every
 // segment's own state from zero, one joins them (S_in of each segment), and the main
 // launch runs all segments side by side.
+//
+// One CTA of 32 warps an SM, a warp for each step and mbarriers between the steps, so that
+// several chunks are in work at once: loads (TMA), decay sums, weighted values, scores to P,
+// outputs, the state, and one warp each for the products that need the state before and those
+// that do not. What decides: 64 registers a thread (shared out again by setmaxnreg) and code that
+// stays in the instruction cache - loops are kept rolled where unrolling them cost a fetch a pass.
+// Measured on a B200 (device time; copy rate 6552 GB/s):
+//   2 x 26 tokens, 4 heads, N 128, P 64        8.7 us   launch, set-up and two memory latencies
+//   16 x 200 ragged, 12 heads, N 128, P 64    14.3 us   four chunks in a row of about 2400 cycles
+//   2 x 3600 ragged, 12 heads, N 128, P 64    34 us     5 chunks a segment, twice, and a join
+//   1 x 32768, 16 + 16 heads, 128 x 128      168 us     102 us at 5.2 TB/s, 58 us for the
+//                                                       segments' states (4.2 TB/s), join 8 us
+//   8 x 4097 ragged, 32 + 8 heads, 64 x 64    88 us     issue: 71 % of the slots of 128 SMs
 #include <cuda.h>
 #include <cudaTypedefs.h>
 
@@ -46,13 +59,16 @@ using namespace sm100;
 constexpr int kC = 64;                // tokens of a chunk
 constexpr int kBox = 8192;            // bytes of a 64 x 64 BF16 tile
 constexpr int kSums = 4;              // chunks whose decay sums are kept
-constexpr float kMinLog2 = -256.f;    // a decay below it is zero in FP32 against any state
+// A decay below it is zero in FP32 against any state. (64 of them in a chunk add up to 2^14,
+// where the sums' steps are 2^-10: weights within 2^-10 or so, less than P's rounding.)
+constexpr float kMinLog2 = -256.f;
 
 // Warps, by what they do; groups of four have the four quarters of the TMEM lanes, pairs of
 // groups the two halves of a chunk's tokens.
 constexpr int kPrepWarp = 4, kScoreWarp = 12, kOutWarp = 20;  // (state: 0)
 // A quarter's warps share a scheduler, and the later a chunk's rows the more scores they have:
-// the last quarter's gets the lightest of the single warps.
+// the last quarter's gets the lightest of the single warps (100 -> 92 us for 8 x 4097 tokens,
+// with the sums of both heads in one pass).
 constexpr int kSumWarp = 28, kStateMmaWarp = 29, kOutMmaWarp = 30, kLoadWarp = 31;
 constexpr int kThreads = 32 * 32;
 // Registers of a thread: 32 warps have 64 at launch, 2048 together, and share them out again.
@@ -264,23 +280,6 @@ __device__ __forceinline__ bool elect_one() {
   uint32_t x;
   asm volatile("{\n .reg .pred p;\n elect.sync _|p, 0xffffffff;\n selp.u32 %0, 1, 0, p;\n}\n" : "=r"(x));
   return x != 0;
-}
-// Two FP32 products or differences in one instruction.
-__device__ __forceinline__ float2 mul2(float2 a, float2 b) {
-  float2 r;
-  asm("{\n .reg .b64 x, y, z;\n mov.b64 x, {%2, %3};\n mov.b64 y, {%4, %5};\n mul.rn.f32x2 z, x, y;\n"
-      " mov.b64 {%0, %1}, z;\n}\n"
-      : "=f"(r.x), "=f"(r.y)
-      : "f"(a.x), "f"(a.y), "f"(b.x), "f"(b.y));
-  return r;
-}
-__device__ __forceinline__ float2 fma2(float2 a, float2 b, float2 c) {
-  float2 r;
-  asm("{\n .reg .b64 x, y, z, w;\n mov.b64 x, {%2, %3};\n mov.b64 y, {%4, %5};\n mov.b64 w, {%6, %7};\n"
-      " fma.rn.f32x2 z, x, y, w;\n mov.b64 {%0, %1}, z;\n}\n"
-      : "=f"(r.x), "=f"(r.y)
-      : "f"(a.x), "f"(a.y), "f"(b.x), "f"(b.y), "f"(c.x), "f"(c.y));
-  return r;
 }
 template <int N>
 __device__ __forceinline__ void more_registers() {
@@ -1100,9 +1099,10 @@ struct Plan {
   int64_t rows, state_bytes, bytes;
 };
 
-// A prompt shorter than this runs token by token: 7.3 and 9.9 us for 8 tokens (1 and 16 rows of
-// 12 heads, N = 128, P = 64), 33 us for 1024 heads, against 9.4, 9.9 and 31 us in a chunk.
-constexpr int kMinTokens = 8;
+// A prompt shorter than this runs token by token: 6.2, 10.8 and 38 us for 16 tokens (1, 16 and 32
+// rows of 12, 12 and 32 heads, N = 128, P = 64) against 9.5, 9.9 and 37 us in a chunk; 17 tokens take
+// 7, 12 and 44 us.
+constexpr int kMinTokens = 17;
 
 bool plan_of(int B, int T, int H, int Hq, int N, int P, int dtype, Plan& x) {
   if (dtype != TF_BF16 || N > 128 || P > 128 || T < kMinTokens) return false;

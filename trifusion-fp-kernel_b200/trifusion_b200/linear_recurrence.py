@@ -112,7 +112,7 @@ def linear_attention(q, k, v, decay, state=None, *, slots=None, lengths=None, sc
     (FP32 sums and state). A non-finite value in v then also reaches the earlier tokens of
     its chunk, and, with P up to 64, a non-finite weight (a NaN in a head's decays, say) the
     outputs of the head next to it under the same key head. FP32 operands, wider heads and
-    pieces of fewer than 8 tokens run token by token. There is no backward pass.
+    pieces of up to 16 tokens run token by token. There is no backward pass.
     """
     op = "linear_attention"
     shape = q.shape
