@@ -521,13 +521,23 @@ int tf_ragged_copy_fwd(void* packed, void* const* dense, const int64_t* groups, 
  * theta = positions[b,t] * inv_freq[i] for i < R/2 (FP64 angles), pair (x1, x2) ->
  * amplitude * (x1 cos - x2 sin, x2 cos + x1 sin) in FP32 with one rounding; pairs are
  * (i, i + R/2), or (2i, 2i + 1) with `interleaved`; elements R..D-1 are copied.
- * q_out/k_out may be q/k themselves. `strides` holds 14 int64 element strides: q, k,
- * q_out, k_out (batch, time, head each; innermost stride 1), positions (batch, time).
+ * q_out/k_out may be q/k themselves. `strides` are in elements: q, k, q_out, k_out (batch,
+ * time, head each; innermost stride 1), positions (batch, time).
  * R/2 <= 512, D * (Hq + Hk) <= 65535 and B * T < 2^31 (else TF_ERR_SIZE). */
-int tf_rotary_positions_fwd(const void* q, const void* k, void* q_out, void* k_out, int dtype,
-                            const int64_t* positions, const double* inv_freq, float amplitude, int interleaved,
-                            const int64_t* strides, int batch, int seqlen, int q_heads, int k_heads, int head_dim,
-                            int rotary_dim, void* stream);
+typedef struct tf_rotary_io {
+  const void* q;
+  const void* k;
+  void* q_out;
+  void* k_out;
+  const int64_t* positions;
+  const double* inv_freq;
+  int64_t strides[14];
+  double amplitude;
+  int32_t dtype, interleaved;
+  int32_t batch, seqlen, q_heads, k_heads, head_dim, rotary_dim;
+} tf_rotary_io;
+
+int tf_rotary_positions_fwd(const tf_rotary_io* io, void* stream);
 
 /* Linear attention with a decay for each head:
  *   S_t = e^decay[b,h,t] S_(t-1) + k_t v_t^T (key_dim x value_dim, FP32),
@@ -539,21 +549,35 @@ int tf_rotary_positions_fwd(const void* q, const void* k, void* q_out, void* k_o
  * changes; a slot >= state_slots or one that an earlier row has: NaN outputs, no
  * state changes. Tokens at or past lengths[b] (nullable int64 [B]) are not read and
  * their outputs are zero. seqlen 1 is the single-token form.
- * `strides` holds 17 int64 element strides: q, k, v (batch, time, head), decay (batch,
- * head, time), out (batch, time, head), state (slot, head); innermost strides are 1
- * and the state is contiguous over [N,P].
+ * `strides` are in elements: q, k, v (batch, time, head), decay (batch, head, time), out
+ * (batch, time, head), state (slot, head); innermost strides are 1 and the state is
+ * contiguous over [N,P].
  * BF16 pieces of 17 tokens or more with N and P up to 128 run in chunks of 64 tokens on the
  * tensor cores (tf_linear_attention_chunked returns 1) if q, k, v and out lie on 16-byte
  * boundaries with strides that are multiples of 16 bytes; all others token by token. The
  * chunked form takes tf_linear_attention_workspace_size bytes of `workspace` (256-byte
  * aligned, contents irrelevant; 0 where there are rows enough for all SMs). */
+typedef struct tf_linear_attention_io {
+  const void* q;
+  const void* k;
+  const void* v;
+  void* out;
+  const float* decay;
+  float* state;
+  const int64_t* slots;
+  const int64_t* lengths;
+  void* workspace;
+  int64_t workspace_bytes, state_slots;
+  int64_t strides[17];
+  double scale;
+  int32_t dtype, fresh;
+  int32_t batch, seqlen, heads, groups, key_dim, value_dim;
+} tf_linear_attention_io;
+
 int tf_linear_attention_chunked(int batch, int seqlen, int heads, int groups, int key_dim, int value_dim, int dtype);
 int64_t tf_linear_attention_workspace_size(int batch, int seqlen, int heads, int groups, int key_dim, int value_dim,
                                            int dtype);
-int tf_linear_attention_fwd(const void* q, const void* k, const void* v, int dtype, const float* decay, float* state,
-                            int64_t state_slots, int fresh, const int64_t* slots, const int64_t* lengths, void* out,
-                            const int64_t* strides, int batch, int seqlen, int heads, int groups, int key_dim,
-                            int value_dim, float scale, void* workspace, int64_t workspace_bytes, void* stream);
+int tf_linear_attention_fwd(const tf_linear_attention_io* io, void* stream);
 
 #ifdef __cplusplus
 }

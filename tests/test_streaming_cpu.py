@@ -1,7 +1,7 @@
 """Host side of the streaming operators: refusals, frequencies and the C ABI's checks (no GPU)."""
 
-import ctypes
 import math
+import struct
 
 import pytest
 import torch
@@ -139,32 +139,32 @@ def test_frequencies():
 
 def test_c_abi_validates_on_the_host():
     lib = _lib.lib()
-    buf = ctypes.c_void_p(4096)
-    st14, st17 = _lib.int64_array([8] * 14), _lib.int64_array([8] * 17)
+    buf = 4096
 
-    def rotary(dtype=1, strides=st14, b=1, t=1, h=1, hk=1, d=8, r=8, q=buf):
-        return lib.tf_rotary_positions_fwd(q, buf, buf, buf, dtype, buf, buf, 1.0, 0, strides, b, t, h, hk, d, r, None)
+    def rotary(dtype=1, b=1, t=1, h=1, hk=1, d=8, r=8, q=buf):
+        return lib.tf_rotary_positions_fwd(struct.pack("6Q14qd8i", q, buf, buf, buf, buf, buf, *[8] * 14, 1.0, dtype, 0,
+                                                       b, t, h, hk, d, r), None)
 
-    assert rotary(dtype=2) == rotary(strides=None) == rotary(b=-1) == rotary(r=7) == rotary(r=10) == _lib.TF_ERR_ARG
-    assert rotary(q=None) == _lib.TF_ERR_ARG
+    assert lib.tf_rotary_positions_fwd(None, None) == rotary(dtype=2) == rotary(b=-1) == rotary(r=7) == rotary(r=10) == _lib.TF_ERR_ARG
+    assert rotary(q=0) == _lib.TF_ERR_ARG
     assert rotary(b=0) == rotary(t=0) == rotary(h=0, hk=0) == _lib.TF_OK
     assert rotary(d=2048, r=2048) == rotary(d=256, h=256) == rotary(b=1 << 16, t=1 << 16) == _lib.TF_ERR_SIZE
 
-    def attention(dtype=1, state=buf, slots_n=4, fresh=0, slots=None, strides=st17, b=2, t=3, h=4, hq=2, n=64, p=64, q=buf):
-        return lib.tf_linear_attention_fwd(q, buf, buf, dtype, buf, state, slots_n, fresh, slots, None, buf, strides,
-                                           b, t, h, hq, n, p, 1.0, None, 0, None)
+    def attention(dtype=1, state=buf, slots_n=4, fresh=0, slots=0, strides=(8,) * 17, b=2, t=3, h=4, hq=2, n=64, p=64, q=buf):
+        return lib.tf_linear_attention_fwd(struct.pack("9Q2q17qd8i", q, buf, buf, buf, buf, state, slots, 0, 0, 0, slots_n,
+                                                       *strides, 1.0, dtype, fresh, b, t, h, hq, n, p), None)
 
-    assert attention(dtype=3) == attention(strides=None) == attention(h=5) == attention(hq=0) == _lib.TF_ERR_ARG
+    assert lib.tf_linear_attention_fwd(None, None) == attention(dtype=3) == attention(h=5) == attention(hq=0) == _lib.TF_ERR_ARG
     assert attention(n=60) == attention(p=264) == attention(n=0) == attention(slots_n=1) == _lib.TF_ERR_ARG
-    assert attention(state=None, slots=buf) == attention(q=None) == attention(t=-1) == _lib.TF_ERR_ARG
+    assert attention(state=0, slots=buf) == attention(q=0) == attention(t=-1) == _lib.TF_ERR_ARG
     assert attention(b=0) == attention(h=0, hq=1) == attention(t=0) == _lib.TF_OK
-    assert attention(state=ctypes.c_void_p(4100)) == _lib.TF_ERR_LAYOUT
+    assert attention(state=4100) == _lib.TF_ERR_LAYOUT
     sizes = dict(b=2, t=17, h=4, hq=2, n=128, p=64, dtype=1)
     chunked = lambda **kw: lib.tf_linear_attention_chunked(*(sizes | kw).values())  # noqa: E731
     assert chunked() == chunked(t=5000) == chunked(n=8, p=128) == 1
     assert chunked(t=16) == chunked(dtype=0) == chunked(n=136) == chunked(p=136) == chunked(b=0) == chunked(hq=3) == 0
     assert lib.tf_linear_attention_workspace_size(*(sizes | dict(t=16)).values()) == 0
-    assert attention(strides=_lib.int64_array([8] * 15 + [6, 8])) == _lib.TF_ERR_LAYOUT
+    assert attention(strides=[8] * 15 + [6, 8]) == _lib.TF_ERR_LAYOUT
 
 
 @pytest.mark.parametrize("first", ["linear_attention_step", "linear_attention", "apply_rotary", "linear_recurrence"])

@@ -328,41 +328,42 @@ int64_t tf_linear_attention_workspace_size(int batch, int seqlen, int heads, int
   return tf::linear_chunk_workspace(batch, seqlen, heads, groups, key_dim, value_dim, dtype);
 }
 
-int tf_linear_attention_fwd(const void* q, const void* k, const void* v, int dtype, const float* decay, float* state,
-                            int64_t state_slots, int fresh, const int64_t* slots, const int64_t* lengths, void* out,
-                            const int64_t* strides, int batch, int seqlen, int heads, int groups, int key_dim,
-                            int value_dim, float scale, void* workspace, int64_t workspace_bytes, void* stream) {
+int tf_linear_attention_fwd(const tf_linear_attention_io* io, void* stream) {
   using namespace tf;
+  if (!io) return TF_ERR_ARG;
+  const int dtype = io->dtype, batch = io->batch, seqlen = io->seqlen, heads = io->heads, groups = io->groups,
+            key_dim = io->key_dim, value_dim = io->value_dim;
+  const int64_t state_slots = io->state_slots;
+  float* state = io->state;
   if (dtype != TF_F32 && dtype != TF_BF16) return TF_ERR_ARG;
-  if (!strides || batch < 0 || seqlen < 0 || heads < 0 || groups < 1 || heads % groups || state_slots < 0)
-    return TF_ERR_ARG;
+  if (batch < 0 || seqlen < 0 || heads < 0 || groups < 1 || heads % groups || state_slots < 0) return TF_ERR_ARG;
   if (key_dim < 8 || value_dim < 8 || key_dim % 8 || value_dim % 8 || key_dim > 256 || value_dim > 256)
     return TF_ERR_ARG;
-  if (slots && !state) return TF_ERR_ARG;
-  if (!slots && state && state_slots < batch) return TF_ERR_ARG;
-  if (batch == 0 || heads == 0 || (seqlen == 0 && !(state && fresh))) return TF_OK;
-  if (seqlen > 0 && (!q || !k || !v || !decay || !out)) return TF_ERR_ARG;
+  if (io->slots && !state) return TF_ERR_ARG;
+  if (!io->slots && state && state_slots < batch) return TF_ERR_ARG;
+  if (batch == 0 || heads == 0 || (seqlen == 0 && !(state && io->fresh))) return TF_OK;
+  if (seqlen > 0 && (!io->q || !io->k || !io->v || !io->decay || !io->out)) return TF_ERR_ARG;
   LinearParams p{};
-  p.q = q, p.k = k, p.v = v, p.out = out;
-  p.decay = decay;
+  p.q = io->q, p.k = io->k, p.v = io->v, p.out = io->out;
+  p.decay = io->decay;
   p.state = state;
   p.nslots = state_slots;
-  p.fresh = fresh != 0;
-  p.slots = slots;
-  p.lengths = lengths;
-  const int64_t* s = strides;
+  p.fresh = io->fresh != 0;
+  p.slots = io->slots;
+  p.lengths = io->lengths;
+  const int64_t* s = io->strides;
   for (int i = 0; i < 3; ++i) p.sq[i] = s[i], p.sk[i] = s[3 + i], p.sv[i] = s[6 + i], p.sg[i] = s[9 + i], p.so[i] = s[12 + i];
   p.ss[0] = s[15], p.ss[1] = s[16];
   if (state && (reinterpret_cast<uintptr_t>(state) % 16 || (state_slots > 1 && p.ss[0] % 4) || (heads > 1 && p.ss[1] % 4)))
     return TF_ERR_LAYOUT;
   p.B = batch, p.T = seqlen, p.H = heads, p.Hq = groups, p.N = key_dim, p.P = value_dim;
-  p.scale = scale;
+  p.scale = static_cast<float>(io->scale);
   if (static_cast<int64_t>(batch) * heads * ((value_dim + 31) / 32) > 0x7fffffffll || seqlen > 0x7fffff00)
     return TF_ERR_SIZE;
   int st = check_device();
   if (st != TF_OK) return st;
   if (linear_chunk_workspace(batch, seqlen, heads, groups, key_dim, value_dim, dtype) >= 0) {
-    st = launch_linear_chunks(p, dtype, workspace, workspace_bytes, static_cast<cudaStream_t>(stream));
+    st = launch_linear_chunks(p, dtype, io->workspace, io->workspace_bytes, static_cast<cudaStream_t>(stream));
     if (st >= 0) return st;
   }
   if (dtype == TF_F32) launch_scan<float>(p, static_cast<cudaStream_t>(stream));

@@ -149,27 +149,31 @@ void launch(const RotaryParams& p, bool interleaved, cudaStream_t stream) {
 }  // namespace
 }  // namespace tf
 
-extern "C" int tf_rotary_positions_fwd(const void* q, const void* k, void* q_out, void* k_out, int dtype,
-                                       const int64_t* positions, const double* inv_freq, float amplitude,
-                                       int interleaved, const int64_t* strides, int batch, int seqlen, int q_heads,
-                                       int k_heads, int head_dim, int rotary_dim, void* stream) {
+extern "C" int tf_rotary_positions_fwd(const tf_rotary_io* io, void* stream) {
   using namespace tf;
+  if (!io) return TF_ERR_ARG;
+  const int dtype = io->dtype, batch = io->batch, seqlen = io->seqlen, q_heads = io->q_heads, k_heads = io->k_heads,
+            head_dim = io->head_dim, rotary_dim = io->rotary_dim;
+  const bool interleaved = io->interleaved != 0;
+  const void *q = io->q, *k = io->k;
+  void *q_out = io->q_out, *k_out = io->k_out;
+  const int64_t* strides = io->strides;
   if (dtype != TF_F32 && dtype != TF_BF16) return TF_ERR_ARG;
   if (batch < 0 || seqlen < 0 || q_heads < 0 || k_heads < 0 || head_dim < 1 || rotary_dim < 2 || rotary_dim % 2 ||
-      rotary_dim > head_dim || !strides)
+      rotary_dim > head_dim)
     return TF_ERR_ARG;
   if (batch == 0 || seqlen == 0 || q_heads + k_heads == 0) return TF_OK;
-  if (!positions || !inv_freq || (q_heads && (!q || !q_out)) || (k_heads && (!k || !k_out))) return TF_ERR_ARG;
+  if (!io->positions || !io->inv_freq || (q_heads && (!q || !q_out)) || (k_heads && (!k || !k_out))) return TF_ERR_ARG;
   if (rotary_dim / 2 > kMaxPairs || static_cast<int64_t>(head_dim) * (q_heads + k_heads) > 65535) return TF_ERR_SIZE;
   RotaryParams p{};
   p.q = q, p.k = k, p.qo = q_out, p.ko = k_out;
   for (int i = 0; i < 3; ++i) {
     p.sq[i] = strides[i], p.sk[i] = strides[3 + i], p.soq[i] = strides[6 + i], p.sok[i] = strides[9 + i];
   }
-  p.positions = positions;
+  p.positions = io->positions;
   p.sp[0] = strides[12], p.sp[1] = strides[13];
-  p.inv_freq = inv_freq;
-  p.amplitude = amplitude;
+  p.inv_freq = io->inv_freq;
+  p.amplitude = static_cast<float>(io->amplitude);
   p.T = seqlen;
   p.tokens = static_cast<int64_t>(batch) * seqlen;
   if (p.tokens > 0x7fffffffll) return TF_ERR_SIZE;

@@ -84,11 +84,10 @@ SIGNATURES = {
     "tf_decoder_heads_scratch_bytes": [_i],
     "tf_decoder_heads_fwd": [_p] * 18 + [_q, _p, _i, _p],
     # Streaming operators.
-    "tf_rotary_positions_fwd": [_p, _p, _p, _p, _i, _p, _p, _f, _i, _p, _i, _i, _i, _i, _i, _i, _p],
+    "tf_rotary_positions_fwd": [_p, _p],
     "tf_linear_attention_chunked": [_i] * 7,
     "tf_linear_attention_workspace_size": [_i] * 7,
-    "tf_linear_attention_fwd": [_p, _p, _p, _i, _p, _p, _q, _i, _p, _p, _p, _p, _i, _i, _i, _i, _i, _i, _f, _p, _q,
-                                _p],
+    "tf_linear_attention_fwd": [_p, _p],
 }
 _RESTYPES = {"tf_status_string": ctypes.c_char_p, "tf_last_cuda_error": ctypes.c_char_p,
              "tf_recurrence_workspace_size": ctypes.c_size_t,
@@ -210,10 +209,13 @@ def launch(fn, device, *args):
         check(getattr(lib(), fn)(*args, stream))
 
 
-def launcher(fn):
-    """As :func:`launch` for one entry point, for operators whose kernels are shorter than the
-    host's work around them: ``launcher(fn)(device_index, *args)`` changes the current device
-    only where it has to and asks for the stream's handle alone."""
+def launcher(fn, layout):
+    """As :func:`launch` for one entry point that takes a record, for operators whose kernels are
+    shorter than the host's work around them: ``launcher(fn, layout)(device_index, *fields)`` packs
+    the record (``layout`` is its :mod:`struct` format), changes the current device only where it
+    has to and asks for the stream's handle alone."""
+    import struct
+
     import torch
 
     raw_stream = getattr(torch._C, "_cuda_getCurrentRawStream", None)
@@ -221,17 +223,18 @@ def launcher(fn):
         def raw_stream(index):
             return torch.cuda.current_stream(index).cuda_stream
     current = torch.cuda.current_device
+    pack = struct.Struct(layout).pack
     call = None
 
-    def run(index, *args):
+    def run(index, *fields):
         nonlocal call
         if call is None:
             call = getattr(lib(), fn)
         if current() == index:
-            status = call(*args, raw_stream(index))
+            status = call(pack(*fields), raw_stream(index))
         else:
             with torch.cuda.device(index):
-                status = call(*args, raw_stream(index))
+                status = call(pack(*fields), raw_stream(index))
         if status != TF_OK:
             check(status)
 

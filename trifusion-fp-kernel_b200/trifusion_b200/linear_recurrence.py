@@ -13,14 +13,12 @@ tensor or as a pool with a slot for each row.
 from __future__ import annotations
 
 import functools
-import struct
 
 import torch
 
 from . import _lib
 
-_launch = _lib.launcher("tf_linear_attention_fwd")
-_pack = struct.Struct("17q").pack
+_launch = _lib.launcher("tf_linear_attention_fwd", "9Q2q17qd8i")  # tf_linear_attention_io
 _DTYPES = {torch.float32: _lib.TF_F32, torch.bfloat16: _lib.TF_BF16}
 
 
@@ -44,19 +42,20 @@ def _operands(op, dtype, q, k, v, decay, hq, h, n, p):
 
 def _check_state(op, state, slots, b, h, n, p):
     """Checks a state and its slots; returns the state's strides over slots and heads."""
-    if state.dtype != torch.float32 or state.dim() != 4 or tuple(state.shape[1:]) != (h, n, p):
+    shape = state.shape
+    if state.dtype != torch.float32 or len(shape) != 4 or shape[1:] != (h, n, p):
         raise ValueError(f"{op}: state must be float32 [slots,H,N,P]")
     s0, s1, s2, s3 = state.stride()
     if s3 != 1 or s2 != p or s0 % 4 or s1 % 4 or state.data_ptr() % 16:
         raise ValueError(f"{op}: state must be contiguous over [N,P], its heads on 16-byte boundaries")
-    if (s1 < n * p and h > 1) or (s0 < n * p and state.shape[0] > 1):
+    if (s1 < n * p and h > 1) or (s0 < n * p and shape[0] > 1):
         raise ValueError(f"{op}: the states of a pool must not overlap")
     if state.requires_grad and torch.is_grad_enabled():
         raise RuntimeError(f"{op}: {_lib.NO_GRADIENT}")
     if slots is None:
-        if state.shape[0] != b:
+        if shape[0] != b:
             raise ValueError(f"{op}: without slots, state must have one entry for each row")
-    elif slots.dtype != torch.int64 or tuple(slots.shape) != (b,):
+    elif slots.dtype != torch.int64 or slots.shape != (b,):
         raise ValueError(f"{op}: slots must be int64 [B]")
     return s0, s1
 
@@ -70,9 +69,8 @@ def _check_out(op, out, v):
         raise RuntimeError(f"{op}: {_lib.NO_GRADIENT}")
 
 
-def _check_device(op, index, *tensors):
-    if index < 0 or any(t is not None and t.get_device() != index for t in tensors):
-        raise RuntimeError(f"{op}: all tensors must be CUDA tensors on one device")
+def _on(index, x):
+    return x is None or x.get_device() == index
 
 
 def _aligned(x):
@@ -123,7 +121,7 @@ def linear_attention(q, k, v, decay, state=None, *, slots=None, lengths=None, sc
     if vb != b or vt != t:
         raise ValueError(f"{op}: q and k must be [B,T,Hq,N] and v [B,T,H,P]")
     dtype, index = _operands(op, q.dtype, q, k, v, decay, hq, h, n, p), q.get_device()
-    sg, shape = decay.stride(), tuple(decay.shape)
+    sg, shape = decay.stride(), decay.shape
     if shape == (h,) and sg:
         sg = (0, sg[0], 0)
     elif shape != (b, h, t):
@@ -133,11 +131,13 @@ def linear_attention(q, k, v, decay, state=None, *, slots=None, lengths=None, sc
         ss = _check_state(op, state, slots, b, h, n, p)
     elif slots is not None:
         raise ValueError(f"{op}: slots need a state")
-    if lengths is not None and (lengths.dtype != torch.int64 or tuple(lengths.shape) != (b,)):
+    if lengths is not None and (lengths.dtype != torch.int64 or lengths.shape != (b,)):
         raise ValueError(f"{op}: lengths must be int64 [B]")
     if out is not None:
         _check_out(op, out, v)
-    _check_device(op, index, k, v, decay, state, slots, lengths, out)
+    if (index < 0 or k.get_device() != index or v.get_device() != index or decay.get_device() != index
+            or not (_on(index, state) and _on(index, slots) and _on(index, lengths) and _on(index, out))):
+        raise RuntimeError(f"{op}: all tensors must be CUDA tensors on one device")
     q0, q1, q2, q3 = q.stride()
     k0, k1, k2, k3 = k.stride()
     v0, v1, v2, v3 = v.stride()
@@ -155,7 +155,7 @@ def linear_attention(q, k, v, decay, state=None, *, slots=None, lengths=None, sc
         _lib.error_watch()
     _lib.check_device_error()
     chunked, nbytes = _plan(index, b, t, h, hq, n, p, dtype)
-    work, slot, length, into = None, None, None, out
+    slot, length, work, wp, into = 0, 0, None, 0, out
     qp, kp, vp, outp = q.data_ptr(), k.data_ptr(), v.data_ptr(), out.data_ptr()
     if chunked:  # its tile loads and stores need 16-byte rows
         strides = (q0, q1, q2, k0, k1, k2, v0, v1, v2, o0, o1, o2)
@@ -168,15 +168,16 @@ def linear_attention(q, k, v, decay, state=None, *, slots=None, lengths=None, sc
             qp, kp, vp, outp = q.data_ptr(), k.data_ptr(), v.data_ptr(), into.data_ptr()
         if nbytes:
             work = torch.empty(nbytes, dtype=torch.uint8, device=v.device)
+            wp = work.data_ptr()
     if slots is not None:
         slots = slots.contiguous()
         slot = slots.data_ptr()
     if lengths is not None:
         lengths = lengths.contiguous()
         length = lengths.data_ptr()
-    _launch(index, qp, kp, vp, dtype, decay.data_ptr(), state.data_ptr(), state.shape[0], fresh, slot, length, outp,
-            _pack(q0, q1, q2, k0, k1, k2, v0, v1, v2, *sg, o0, o1, o2, *ss), b, t, h, hq, n, p,
-            n ** -0.5 if scale is None else scale, None if work is None else work.data_ptr(), nbytes)
+    _launch(index, qp, kp, vp, outp, decay.data_ptr(), state.data_ptr(), slot, length, wp, nbytes, state.shape[0],
+            q0, q1, q2, k0, k1, k2, v0, v1, v2, *sg, o0, o1, o2, *ss, n ** -0.5 if scale is None else scale,
+            dtype, fresh, b, t, h, hq, n, p)
     if into is not out:
         out.copy_(into)
     return out, state
@@ -198,7 +199,7 @@ def linear_attention_step(q, k, v, decay, state, *, slots=None, scale=None, out=
     if vb != b:
         raise ValueError(f"{op}: q and k must be [B,Hq,N] and v [B,H,P]")
     dtype, index = _operands(op, q.dtype, q, k, v, decay, hq, h, n, p), q.get_device()
-    sg, shape = decay.stride(), tuple(decay.shape)
+    sg, shape = decay.stride(), decay.shape
     if shape == (h,) and sg:
         sg = (0, sg[0])
     elif shape != (b, h):
@@ -206,7 +207,9 @@ def linear_attention_step(q, k, v, decay, state, *, slots=None, scale=None, out=
     ss = _check_state(op, state, slots, b, h, n, p)
     if out is not None:
         _check_out(op, out, v)
-    _check_device(op, index, k, v, decay, state, slots, out)
+    if (index < 0 or k.get_device() != index or v.get_device() != index or decay.get_device() != index
+            or state.get_device() != index or not (_on(index, slots) and _on(index, out))):
+        raise RuntimeError(f"{op}: all tensors must be CUDA tensors on one device")
     qb, qh, q1 = q.stride()
     kb, kh, k1 = k.stride()
     vb, vh, v1 = v.stride()
@@ -219,7 +222,7 @@ def linear_attention_step(q, k, v, decay, state, *, slots=None, scale=None, out=
     if v1 != 1:
         v = v.contiguous()
         vb, vh, _ = v.stride()
-    slot = None
+    slot = 0
     if slots is not None:
         slots = slots.contiguous()
         slot = slots.data_ptr()
@@ -227,8 +230,7 @@ def linear_attention_step(q, k, v, decay, state, *, slots=None, scale=None, out=
         out, ob, oh = torch.empty_like(v, memory_format=torch.contiguous_format), h * p, p
     else:
         ob, oh, _ = out.stride()
-    _launch(index, q.data_ptr(), k.data_ptr(), v.data_ptr(), dtype, decay.data_ptr(), state.data_ptr(), state.shape[0],
-            0, slot, None, out.data_ptr(),
-            _pack(qb, 0, qh, kb, 0, kh, vb, 0, vh, *sg, 0, ob, 0, oh, *ss), b, 1, h, hq, n, p,
-            n ** -0.5 if scale is None else scale, None, 0)
+    _launch(index, q.data_ptr(), k.data_ptr(), v.data_ptr(), out.data_ptr(), decay.data_ptr(), state.data_ptr(), slot, 0,
+            0, 0, state.shape[0], qb, 0, qh, kb, 0, kh, vb, 0, vh, *sg, 0, ob, 0, oh, *ss,
+            n ** -0.5 if scale is None else scale, dtype, 0, b, 1, h, hq, n, p)
     return out

@@ -11,7 +11,6 @@ rounding to the tensors' type.
 from __future__ import annotations
 
 import math
-import struct
 
 import torch
 
@@ -19,8 +18,7 @@ from . import _lib
 
 _DTYPES = {torch.float32: _lib.TF_F32, torch.bfloat16: _lib.TF_BF16}
 _LAYOUTS = {"half": 0, "interleaved": 1}
-_launch = _lib.launcher("tf_rotary_positions_fwd")
-_pack = struct.Struct("14q").pack
+_launch = _lib.launcher("tf_rotary_positions_fwd", "6Q14qd8i")  # tf_rotary_io
 
 
 def rotary_frequencies(rotary_dim, base=10000.0, *, scaling=None, factor=1.0, trained_length=None,
@@ -111,7 +109,7 @@ def apply_rotary(q, k, positions, inv_freq, *, layout="half", amplitude=1.0, inp
         inv_freq = inv_freq.contiguous()
     q0, q1, q2, q3 = q.stride()
     k0 = k1 = k2 = o0 = o1 = o2 = 0
-    k3, kp, kop = 1, None, None
+    k3, kp, kop = 1, 0, 0
     if k is not None:
         k0, k1, k2, k3 = k.stride()
     if inplace:
@@ -131,7 +129,7 @@ def apply_rotary(q, k, positions, inv_freq, *, layout="half", amplitude=1.0, inp
     if k is not None:
         kp, kop = k.data_ptr(), ko.data_ptr()
     s = positions.stride()
-    _launch(index, q.data_ptr(), kp, qo.data_ptr(), kop, dtype, positions.data_ptr(), inv_freq.data_ptr(), amplitude,
-            interleaved, _pack(q0, q1, q2, k0, k1, k2, p0, p1, p2, o0, o1, o2, 0 if len(s) == 1 else s[0], s[-1]),
-            b, t, h, hk, d, 2 * half)
+    _launch(index, q.data_ptr(), kp, qo.data_ptr(), kop, positions.data_ptr(), inv_freq.data_ptr(), q0, q1, q2, k0, k1, k2,
+            p0, p1, p2, o0, o1, o2, 0 if len(s) == 1 else s[0], s[-1], amplitude, dtype, interleaved, b, t, h, hk, d,
+            2 * half)
     return qo if k is None else (qo, ko)
