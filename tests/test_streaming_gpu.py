@@ -227,6 +227,40 @@ def test_scales_with_strong_decays(scale, rate, n, p):
     check(args, state, scale=scale)
 
 
+@pytest.mark.parametrize("dtype", [BF16, FP32])
+@pytest.mark.parametrize("n,p", [(64, 64), (128, 128), (128, 64)])
+@pytest.mark.parametrize("bad", [float("nan"), float("inf")])
+def test_where_non_finite_values_reach(dtype, n, p, bad):
+    """A query's reaches its token, a key's its heads from its token on, a value's its column of its
+    head (in the chunked form from the start of its chunk of 64 tokens on), a state's its column."""
+    b, t, h, hq, at = 2, 200, 4, 2, 100
+    args, state = inputs(b, t, h, hq, n, p, dtype, state=True)
+    start = 64 if dtype == BF16 else at
+
+    def run(i, *where):
+        mine = [x.clone() for x in args] + [state.clone()]
+        mine[i][where] = bad
+        out, new = linear_attention(*mine)
+        return out.isfinite(), new.isfinite()
+
+    out, new = run(0, 0, at, 1)                     # heads 2 and 3 read key head 1
+    assert new.all() and not out[0, at, 2:].any()
+    out[0, at, 2:] = True
+    assert out.all()
+    out, new = run(1, 0, at, 1)
+    assert not out[0, at:, 2:].any() and not new[0, 2:].any()
+    out[0, at:, 2:] = new[0, 2:] = True
+    assert out.all() and new.all()
+    out, new = run(2, 0, at, 1, 5)
+    assert not out[0, at:, 1, 5].any() and not new[0, 1, :, 5].any()
+    out[0, start:, 1, 5] = new[0, 1, :, 5] = True
+    assert out.all() and new.all()
+    out, new = run(4, 0, 3, 7, 5)
+    assert not out[0, :, 3, 5].any() and not new[0, 3, 7, 5]
+    out[0, :, 3, 5] = new[0, 3, 7, 5] = True
+    assert out.all() and new.all()
+
+
 @pytest.mark.parametrize("time", [5, 300])
 def test_pool_with_slots(time):
     b, h, n, p, pool = 6, 4, 64, 64, 9
