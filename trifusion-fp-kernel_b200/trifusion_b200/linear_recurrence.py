@@ -149,8 +149,8 @@ def linear_attention(q, k, v, decay, state=None, *, slots=None, lengths=None, sc
     else:
         o0, o1, o2, _ = out.stride()
     if fresh:
-        state = torch.empty((b, h, n, p), dtype=torch.float32, device=v.device)
-        ss = (h * n * p, n * p)
+        ss = (h * n * p, n * p)  # (the strided form is the faster call)
+        state = torch.empty_strided((b, h, n, p), (*ss, p, 1), dtype=torch.float32, device=v.device)
     if not _lib._watch["ready"]:
         _lib.error_watch()
     _lib.check_device_error()
@@ -167,7 +167,7 @@ def linear_attention(q, k, v, decay, state=None, *, slots=None, lengths=None, sc
             o0, o1, o2, _ = into.stride()
             qp, kp, vp, outp = q.data_ptr(), k.data_ptr(), v.data_ptr(), into.data_ptr()
         if nbytes:
-            work = torch.empty(nbytes, dtype=torch.uint8, device=v.device)
+            work = torch.empty_strided((nbytes,), (1,), dtype=torch.uint8, device=v.device)
             wp = work.data_ptr()
     if slots is not None:
         slots = slots.contiguous()
