@@ -227,6 +227,27 @@ def test_scales_with_strong_decays(scale, rate, n, p):
     check(args, state, scale=scale)
 
 
+@pytest.mark.parametrize("form", ["chunks", "tokens", "steps"])
+def test_slow_decays_over_a_long_memory(form):
+    """Roundings of the state go both ways: 2^-24 r.m.s. at most for each of the two or three of a token,
+    added up like a random walk, and no more than 2^-29 a token that go one way."""
+    t, h, n, p = 2000, 2, 64, 64
+    args, _ = inputs(1, t, h, 1, n, p, slow=1e-4)
+    _, s, _, _ = recurrence(*args)
+    if form == "chunks":
+        _, new = linear_attention(*args)
+    elif form == "tokens":
+        _, new = linear_attention(*[x.float() for x in args])
+    else:
+        new = torch.zeros(1, h, n, p, device=DEV)
+        for i in range(t):
+            linear_attention_step(args[0][:, i], args[1][:, i], args[2][:, i], args[3][:, :, i], new)
+    err = new.double() - s
+    bias = abs(((new.double() * s).sum() / (s * s).sum() - 1).item())
+    assert err.norm() <= 2.0 ** -24 * (3 * t) ** 0.5 * s.norm()
+    assert bias <= t * 2.0 ** -29
+
+
 @pytest.mark.parametrize("dtype", [BF16, FP32])
 @pytest.mark.parametrize("n,p", [(64, 64), (128, 128), (128, 64)])
 @pytest.mark.parametrize("bad", [float("nan"), float("inf")])

@@ -21,8 +21,22 @@ __device__ __forceinline__ float ld_f(const bf16* p) { return bf2f(__ldg(p)); }
 __device__ __forceinline__ void st_f(float* p, float x) { *p = x; }
 __device__ __forceinline__ void st_f(bf16* p, float x) { *p = __float2bfloat16_rn(x); }
 
-// e^g for a log decay g. -inf (a reset) gives exactly 0; NaN stays NaN.
-__device__ __forceinline__ float decay_factor(float g) { return ex2_approx(g * kLog2e); }
+// The factor e^g of a log decay g; near 1 (its sign bit is set then) e^g - 1, to which the state
+// itself is added: with e^g errors of the factor add up over a long memory (3e-9 a token, all one
+// way, 1.7e-5 of the state after 4680 tokens of slow decay; now 1.3e-6). -inf (a reset) gives
+// exactly 0; NaN stays NaN.
+__device__ __forceinline__ float decay_factor(float g) {
+  // The Taylor series of e^g - 1 to g^7: the rest is below 2^-25 of it for |g| < 0.35.
+  float x = 1.f / 5040.f;
+  x = fmaf(x, g, 1.f / 720.f);
+  x = fmaf(x, g, 1.f / 120.f);
+  x = fmaf(x, g, 1.f / 24.f);
+  x = fmaf(x, g, 1.f / 6.f);
+  x = fmaf(x, g, 0.5f);
+  x = fmaf(x, g * g, g);
+  return g <= 0.f && g > -0.35f ? -fabsf(x) : ex2_approx(g * kLog2e);
+}
+__device__ __forceinline__ bool near_one(float factor) { return __float_as_int(factor) < 0; }
 
 // ---- recurrent form ------------------------------------------------------------
 // One block: one row, one head, 32 columns of its state. Thread (warp w, lane l) holds columns
@@ -30,15 +44,18 @@ __device__ __forceinline__ float decay_factor(float g) { return ex2_approx(g * k
 // shared memory, its output three shuffles (each halves what a lane still sums) and a partial sum
 // of each warp. Tokens come in batches: while one is worked on, the next one's operands are in shared
 // memory and those of the one after it on their way to registers, and a batch takes one barrier,
-// behind which every warp sums up the output of some of its tokens. Bound by issue and, with few blocks, by the latency of a token's chain.
-// Where a block has an SM to itself, or shares it with one other, eight warps with a whole batch
+// behind which every warp sums up the output of some of its tokens. Bound by issue and, with few
+// blocks, by the latency of a token's chain. Up to two blocks an SM, eight warps with a whole batch
 // unrolled are faster, else four warps with half of it (fewer instructions for a token). FP32, us:
-//   2 x 3600 tokens, 12 heads, N 128, P 64     48 blocks     eight 510   four  724
-//   1 x 7, 12 heads, N 128, P 64               24 blocks     eight 4.6   four  4.7
-//   8 x 4097, 32 heads, N 64, P 64            512 blocks     eight 1435  four 1090
-//   32 x 7, 32 heads, N 128, P 64            2048 blocks     eight 29.2  four 22.4
-// (The first with a barrier for every token: 1058 us; a column a lane: 800 us; the next batch
-// loaded while one is worked on, not two: 694 us.)
+//   1 x 7 tokens, 12 heads, N 128, P 64        24 blocks     eight 4.4   four  4.7
+//   2 x 3600, 12 heads, N 128, P 64            48 blocks     eight 510   four  639
+//   12 x 200, 12 heads, N 128, P 64           288 blocks     eight 49.4  four 54.7
+//   16 x 200, 12 heads, N 128, P 64           384 blocks     eight 74.1  four 72.0
+//   8 x 4097, 32 heads, N 64, P 64            512 blocks     eight 1356  four 1091
+//   32 x 7, 32 heads, N 128, P 64            2048 blocks     eight 30.1  four 22.2
+// (All with the rounded factor e^g; decay_factor's two forms take these to 4.6, 604 and, the larger
+// ones with four warps, 1137 and 23.1. 2 x 3600 with a barrier for every token: 1058 us; with a column
+// a lane: 800 us; the next batch loaded while one is worked on, not two: 694 us.)
 template <typename T, int NR, int WARPS>
 __global__ void __launch_bounds__(32 * WARPS, NR == 8 ? 4 : 2) linear_scan_kernel(const __grid_constant__ LinearParams p) {
   constexpr int kThreads = 32 * WARPS, kRows = 4 * WARPS * NR;
@@ -132,7 +149,9 @@ __global__ void __launch_bounds__(32 * WARPS, NR == 8 ? 4 : 2) linear_scan_kerne
     load(t0 + 2 * kBatch);
 #pragma unroll (kUnroll)
     for (int t = 0; t < kBatch; ++t) {
-      const float2 a = make_float2(as[x][t], as[x][t]);
+      const float a = as[x][t];
+      const float2 factor = make_float2(a, a);
+      const bool keep = near_one(a);
       const float4 vr = *reinterpret_cast<const float4*>(&vs[x][t][4 * (lane & 7)]);
       const float2 vv[4] = {make_float2(vr.x, vr.x), make_float2(vr.y, vr.y), make_float2(vr.z, vr.z),
                             make_float2(vr.w, vr.w)};
@@ -143,7 +162,7 @@ __global__ void __launch_bounds__(32 * WARPS, NR == 8 ? 4 : 2) linear_scan_kerne
         const float2 qq = *reinterpret_cast<const float2*>(&kq[x][t][1][r0 + 2 * i]);
 #pragma unroll
         for (int c = 0; c < 4; ++c) {
-          s[c][i] = fma2(kk, vv[c], mul2(a, s[c][i]));
+          s[c][i] = fma2(kk, vv[c], fma2(factor, s[c][i], keep ? s[c][i] : make_float2(0.f, 0.f)));
           o[c] = fma2(qq, s[c][i], o[c]);
         }
       }
@@ -227,11 +246,18 @@ __global__ void __launch_bounds__(kStepThreads, NR > 4 ? 3 : NR == 4 ? 5 : CS ==
 #pragma unroll
     for (int j = 0; j < 4; ++j)
       if (col + 32 * c < p.P) vv[c][j] = ld_f(v + 32 * c + j);
-  const float a = decay_factor(p.decay[b * p.sg[0] + h * p.sg[1]]);
+  float a = decay_factor(p.decay[b * p.sg[0] + h * p.sg[1]]);
   bool dead = !in_pool;  // no state of its own
   if (p.slots) {
     for (int i = threadIdx.x; i < b; i += kStepThreads) dead |= p.slots[i] == slot;
     dead = __syncthreads_or(dead);
+  }
+  if (!near_one(a)) {  // apart, so that the usual case stays at two operations a value
+#pragma unroll
+    for (int c = 0; c < CS; ++c)
+#pragma unroll
+      for (int i = 0; i < NR; ++i) s[c][i] = make_float4(a * s[c][i].x, a * s[c][i].y, a * s[c][i].z, a * s[c][i].w);
+    a = 0.f;
   }
   float4 o[CS];
 #pragma unroll
@@ -245,10 +271,10 @@ __global__ void __launch_bounds__(kStepThreads, NR > 4 ? 3 : NR == 4 ? 5 : CS ==
       for (int c = 0; c < CS; ++c)
         if (CS == 1 || col + 32 * c < p.P) {
           float4& x = s[c][i];
-          x.x = fmaf(kn, vv[c][0], a * x.x);
-          x.y = fmaf(kn, vv[c][1], a * x.y);
-          x.z = fmaf(kn, vv[c][2], a * x.z);
-          x.w = fmaf(kn, vv[c][3], a * x.w);
+          x.x = fmaf(kn, vv[c][0], fmaf(a, x.x, x.x));
+          x.y = fmaf(kn, vv[c][1], fmaf(a, x.y, x.y));
+          x.z = fmaf(kn, vv[c][2], fmaf(a, x.z, x.z));
+          x.w = fmaf(kn, vv[c][3], fmaf(a, x.w, x.w));
           o[c].x = fmaf(qn, x.x, o[c].x);
           o[c].y = fmaf(qn, x.y, o[c].y);
           o[c].z = fmaf(qn, x.z, o[c].z);
