@@ -54,7 +54,7 @@ int tf_version(void);
 const char* tf_last_cuda_error(void);
 
 /* Device-side error word of the current device: non-zero after one of a
- * recurrence kernel's bounded waits gave up (on the tensor core, on the other
+ * recurrence or chunked linear-attention kernel's bounded waits gave up (on the tensor core, on the other
  * warps of its CTA, or on another CTA's chunk flag); the kernel then finishes
  * instead of hanging, and the outputs of that launch are invalid. Synchronous;
  * `reset` != 0 clears it (and the host-mapped word below). */
@@ -71,9 +71,11 @@ int tf_error_watch_init(void);
 int tf_device_error_pending(void);
 
 /* Limit, in nanoseconds, of a recurrence kernel's waits on other CTAs' chunk
- * flags in later launches (0 restores the default of 2 s). A diagnostic
+ * flags, and of the waits in a chunked linear-attention kernel (4.2 s at most), in
+ * later launches (0 restores the default of 2 s). A diagnostic
  * control: a launch whose wait runs out records the error above and completes
- * with invalid outputs. Waits inside a CTA keep their fixed 2 s limit. */
+ * with invalid outputs. Waits inside a recurrence kernel's CTA, and those for copies
+ * and products in flight before a CTA ends, keep their fixed 2 s limit. */
 int tf_set_flag_wait_ns(long long ns);
 
 /* Bytes of workspace the recurrence needs for [batch, seqlen, heads]

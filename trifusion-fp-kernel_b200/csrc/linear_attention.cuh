@@ -29,6 +29,7 @@ int launch_linear_chunks(const LinearParams& l, int dtype, void* workspace, int6
                          cudaStream_t stream);
 int read_linear_error(int reset);
 int* host_error_word();
+unsigned long long flag_wait_limit_ns();
 
 // Two FP32 products, or products and sums, in one instruction.
 __device__ __forceinline__ float2 mul2(float2 a, float2 b) {

@@ -45,6 +45,7 @@
 #include <cuda.h>
 #include <cudaTypedefs.h>
 
+#include <algorithm>
 #include <atomic>
 
 #include "../../include/trifusion_b200.h"
@@ -92,6 +93,7 @@ struct ChunkParams {
   float* seg_state;   // [B*H][segs][N][P]: the state before each segment
   float* seg_decay;   // [B*H][segs]: log2 decay over the segment
   int* err_host;
+  uint32_t wait_ns;   // limit of the kernel's waits
 };
 
 // What a CTA works on. Its warps read it from shared memory where they start: few of them
@@ -117,6 +119,7 @@ struct alignas(16) Misc {
   uint64_t ds_full[2], ds_free[2];           // state product there / read
   uint64_t s_ready, s_free;                  // state operand written / read
   uint64_t init_full, init_read;             // the state before the first chunk there / read
+  uint64_t drained[2];                       // a product warp's last product and arrivals are done
   uint32_t tmem;
   alignas(16) float row[kSums][2][kC];  // [chunk][head] two factors of scale e^{c_i - c_j}, or c_i and
   float col[kSums][2][kC];              // -c_j (log2) where a factor would leave FP32's range
@@ -195,6 +198,26 @@ __device__ __forceinline__ bool bar_or(int id, int n, bool x) {
       : "r"(static_cast<uint32_t>(x)), "r"(id), "r"(n)
       : "memory");
   return r != 0;
+}
+// Waits for the phase with `parity` to complete; false after `limit` ns. Its first try suspends the
+// thread for longer than an ordinary wait takes, so that the limit is looked at only in a wait for
+// something that does not come.
+__device__ __forceinline__ bool wait_within(uint64_t* bar, uint32_t parity, uint32_t limit) {
+  if (mbar_try_wait(bar, parity)) return true;
+  const uint64_t t0 = global_timer_ns();
+  for (;;) {
+    if (mbar_try_wait(bar, parity)) return true;
+    if (global_timer_ns() - t0 > limit) return false;
+  }
+}
+// With a limit below a millisecond the thread is not suspended: the limit is kept from the first
+// moment on, and ordinary waits can run out. (Polling always cost 8 x 4097 tokens 3 %.)
+__device__ __forceinline__ bool wait_or_poll(uint64_t* bar, uint32_t parity, uint32_t limit) {
+  if (limit >= 1000000u) return wait_within(bar, parity, limit);
+  const uint64_t t0 = global_timer_ns();
+  while (!mbar_test_wait(bar, parity))
+    if (global_timer_ns() - t0 > limit) return false;
+  return true;
 }
 __device__ __forceinline__ void mbar_arrive(uint64_t* bar) {
   asm volatile("{\n .reg .b64 st;\n mbarrier.arrive.shared::cta.b64 st, [%0];\n}\n" ::"r"(smem_u32(bar)) : "memory");
@@ -346,6 +369,10 @@ __global__ void __launch_bounds__(kThreads, 1) linear_chunk_kernel(const __grid_
   const LinearParams& l = p.l;
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
 
+  // Waits of the kernel's steps for one another. One that gives up ends its warp's work: the warps
+  // behind it give up too, the copies and products already issued are waited for (mbar_wait, whose
+  // limit is fixed), TMEM is freed, and the launch leaves an error and invalid outputs and states.
+  auto wait_for = [&](uint64_t* bar, uint32_t parity) { return wait_within(bar, parity, p.wait_ns); };
   // The states of this CTA's heads lie in pieces of neighbouring values: 64 rows at a time of
   // one wide head, or the heads of a pair.
   auto pieces = [&](const Unit& u) { return WIDE ? NK : u.nheads; };
@@ -412,6 +439,8 @@ __global__ void __launch_bounds__(kThreads, 1) linear_chunk_kernel(const __grid_
           mbar_init(&m.ds_full[i], 1);
           mbar_init(&m.ds_free[i], 4);
         }
+        mbar_init(&m.drained[0], 1);
+        mbar_init(&m.drained[1], 1);
         mbar_init(&m.oi_free, 8);
         mbar_init(&m.s_ready, 4);
         mbar_init(&m.s_free, 1);
@@ -449,14 +478,21 @@ __global__ void __launch_bounds__(kThreads, 1) linear_chunk_kernel(const __grid_
     fewer_registers<Regs<NK>::single>();
     const Unit u = m.unit;
     const int n_chunks = u.last - u.first;
+    // A product warp ends when its products and their arrivals at barriers are done: none may still
+    // be on its way into shared memory or TMEM when the CTA gives them up.
+    auto drain = [&](int x) {
+      if (elect_one()) umma_commit(&m.drained[x]);
+      __syncwarp();
+      return __all_sync(0xffffffffu, mbar_wait(&m.drained[x], 0)) != 0;
+    };
     if (warp == kLoadWarp && lane == 0) {
       // ---- loads ----------------------------------------------------------------
       int issued = 0;
       Ring<kStages> ring;
       for (int it = 0; it < n_chunks; ++it, ring.next()) {
         // The stages after the first are free once the state has been taken out of them.
-        if ((it == 1 && has_init && !mbar_wait(&m.init_read, 0)) ||
-            (it >= kStages && !mbar_wait(&m.empty[ring.st], ring.ph ^ 1))) {
+        if ((it == 1 && has_init && !wait_or_poll(&m.init_read, 0, p.wait_ns)) ||
+            (it >= kStages && !wait_or_poll(&m.empty[ring.st], ring.ph ^ 1, p.wait_ns))) {
           bad = true;
           break;
         }
@@ -478,11 +514,15 @@ __global__ void __launch_bounds__(kThreads, 1) linear_chunk_kernel(const __grid_
       // ---- products that need nothing of the state before --------------------------
       // The whole warp runs this, one lane issues: addresses stay in uniform registers.
       // (Two warps for the products: with one, its waits and issue were the longest path.)
+      // The lanes wait for themselves, and stopping is one decision of the warp, once a chunk: lanes that
+      // left alone would keep the others at elect for good. Until then the products run on whatever
+      // is there; the launch's results are invalid then anyway.
       Ring<kStages> ring;
+      bool ok = true;
       auto scores = [&](int it) {  // D
         const int st = ring.st;
-        if (!mbar_wait(&m.full[st], ring.ph)) return false;
-        if (it >= 2 && !mbar_wait(&m.op_free[it & 1], ((it >> 1) - 1) & 1)) return false;
+        ok &= wait_for(&m.full[st], ring.ph);
+        if (it >= 2) ok &= wait_for(&m.op_free[it & 1], ((it >> 1) - 1) & 1);
         tc_fence_after();
         const uint32_t qd = desc_lo(sb + L::q + st * NK * kBox, 0), kd = desc_lo(sb + L::k + st * NK * kBox, 0);
         if (elect_one()) {
@@ -494,15 +534,14 @@ __global__ void __launch_bounds__(kThreads, 1) linear_chunk_kernel(const __grid_
           umma_commit(&m.d_full[it & 1]);
         }
         __syncwarp();
-        return true;
       };
       auto state = [&](int it) {  // dS^T
         const int st = ring.st, wb = it % C::wv_bufs, db = it % C::ds_bufs;
         const uint32_t kd = desc_lo(sb + L::k + st * NK * kBox, kBox);
-        if (it >= C::ds_bufs && !mbar_wait(&m.ds_free[db], (it / C::ds_bufs - 1) & 1)) return false;
+        if (it >= C::ds_bufs) ok &= wait_for(&m.ds_free[db], (it / C::ds_bufs - 1) & 1);
 #pragma unroll 1
         for (int half = 0; half < 2; ++half) {
-          if (!mbar_wait(&m.wv_ready[wb][half], (it / C::wv_bufs) & 1)) return false;
+          ok &= wait_for(&m.wv_ready[wb][half], (it / C::wv_bufs) & 1);
           tc_fence_after();
           if (elect_one()) {
 #pragma unroll
@@ -518,20 +557,23 @@ __global__ void __launch_bounds__(kThreads, 1) linear_chunk_kernel(const __grid_
           }
           __syncwarp();
         }
-        return true;
       };
-      bool ok = true;
 #pragma unroll 1
-      for (int it = 0; it < n_chunks && ok; ++it, ring.next()) ok = (!FULL || scores(it)) && state(it);
-      bad = !ok;
+      for (int it = 0; it < n_chunks && !bad; ++it, ring.next()) {
+        if (FULL) scores(it);
+        state(it);
+        bad = __any_sync(0xffffffffu, !ok);
+      }
+      bad |= !drain(0);
     } else if (FULL && warp == kOutMmaWarp) {
       // ---- the output's products ------------------------------------------------------
       Ring<kStages> ring;
+      bool ok = true;
       auto inter = [&](int it) {  // OI^T
         const int st = ring.st;
-        if (!mbar_wait(&m.full[st], ring.ph)) return false;
-        if (!mbar_wait(&m.s_ready, it & 1)) return false;
-        if (it > 0 && !mbar_wait(&m.oi_free, (it - 1) & 1)) return false;
+        ok &= wait_for(&m.full[st], ring.ph);
+        ok &= wait_for(&m.s_ready, it & 1);
+        if (it > 0) ok &= wait_for(&m.oi_free, (it - 1) & 1);
         tc_fence_after();
         const uint32_t qd = desc_lo(sb + L::q + st * NK * kBox, 0);
         if (elect_one()) {
@@ -542,11 +584,10 @@ __global__ void __launch_bounds__(kThreads, 1) linear_chunk_kernel(const __grid_
           umma_commit(&m.s_free);
         }
         __syncwarp();
-        return true;
       };
       auto within = [&](int it) {  // OP^T
         const int st = ring.st;
-        if (!mbar_wait(&m.p_ready[it & 1], (it >> 1) & 1)) return false;
+        ok &= wait_for(&m.p_ready[it & 1], (it >> 1) & 1);
         tc_fence_after();
         // Wide: both tiles of v. Head x of a pair: its tile and the zero tile, in the order of the blocks.
         const uint32_t step = WIDE ? kBox : (st + 1) * kBox;
@@ -567,12 +608,14 @@ __global__ void __launch_bounds__(kThreads, 1) linear_chunk_kernel(const __grid_
           umma_commit(&m.empty[st]);
         }
         __syncwarp();
-        return true;
       };
-      bool ok = true;
 #pragma unroll 1
-      for (int it = 0; it < n_chunks && ok; ++it, ring.next()) ok = inter(it) && within(it);
-      bad = !ok;
+      for (int it = 0; it < n_chunks && !bad; ++it, ring.next()) {
+        inter(it);
+        within(it);
+        bad = __any_sync(0xffffffffu, !ok);
+      }
+      bad |= !drain(1);
     } else if (warp == kSumWarp) {
       // ---- decay sums -------------------------------------------------------------------
       const int x = lane / kLanes, tok = lane % kLanes * kT;
@@ -616,7 +659,7 @@ __global__ void __launch_bounds__(kThreads, 1) linear_chunk_kernel(const __grid_
         }
         const uint32_t votes = __ballot_sync(0xffffffffu, near);
         const bool factors = WIDE ? votes == 0xffffffffu : (votes >> (16 * x) & 0xffffu) == 0xffffu;
-        bad |= it >= kSums && !mbar_wait(&m.sums_free[sl], (it / kSums - 1) & 1);
+        bad |= it >= kSums && !wait_for(&m.sums_free[sl], (it / kSums - 1) & 1);
         if (__any_sync(0xffffffffu, bad)) {
           bad = true;
           break;
@@ -656,8 +699,8 @@ __global__ void __launch_bounds__(kThreads, 1) linear_chunk_kernel(const __grid_
       fill_rows(p, u, u.last * kC, tid - 32 * kOutWarp, 256, 0u);  // chunks past the length
       for (int it = 0; it < n_chunks; ++it) {
         const int sl = it % kSums, t0 = (u.first + it) * kC + 32 * half;
-        bad |= !mbar_wait(&m.sums[sl], (it / kSums) & 1);
-        bad |= !mbar_wait(&m.o_full[it & 1], (it >> 1) & 1);
+        bad |= !wait_for(&m.sums[sl], (it / kSums) & 1);
+        bad |= !wait_for(&m.o_full[it & 1], (it >> 1) & 1);
         tc_fence_after();
         if (__any_sync(0xffffffffu, bad)) {
           bad = true;
@@ -741,9 +784,9 @@ __global__ void __launch_bounds__(kThreads, 1) linear_chunk_kernel(const __grid_
       Ring<kStages> ring;
       for (int it = 0; it < n_chunks; ++it, ring.next()) {
         const int sl = it % kSums;
-        bad |= !mbar_wait(&m.sums[sl], (it / kSums) & 1);
-        bad |= it >= 2 && !mbar_wait(&m.o_full[it & 1], ((it >> 1) - 1) & 1);  // P's tiles have been read
-        bad |= !mbar_wait(&m.d_full[it & 1], (it >> 1) & 1);
+        bad |= !wait_for(&m.sums[sl], (it / kSums) & 1);
+        bad |= it >= 2 && !wait_for(&m.o_full[it & 1], ((it >> 1) - 1) & 1);  // P's tiles have been read
+        bad |= !wait_for(&m.d_full[it & 1], (it >> 1) & 1);
         tc_fence_after();
         if (__any_sync(0xffffffffu, bad)) {
           bad = true;
@@ -817,8 +860,8 @@ __global__ void __launch_bounds__(kThreads, 1) linear_chunk_kernel(const __grid_
     bool met = u.live(n_chunks - 1) == kC;  // at the barrier of a partial last chunk, if there is one
     for (int it = 0; it < n_chunks; ++it, ring.next()) {
       const int st = ring.st, sl = it % kSums, live = u.live(it), wb = it % C::wv_bufs;
-      bad |= !mbar_wait(&m.full[st], ring.ph);
-      bad |= !mbar_wait(&m.sums[sl], (it / kSums) & 1);
+      bad |= !wait_for(&m.full[st], ring.ph);
+      bad |= !wait_for(&m.sums[sl], (it / kSums) & 1);
       if (live < kC) {
         // Rows past the length hold anything: as operands they must be zero. (The scores may
         // read k before or after: those columns are masked.)
@@ -837,7 +880,7 @@ __global__ void __launch_bounds__(kThreads, 1) linear_chunk_kernel(const __grid_
         break;
       }
       // The operand is free once the state product before has read it.
-      if (it >= C::wv_bufs) bad |= !mbar_wait(&m.wv_free[wb][half], (it / C::wv_bufs - 1) & 1);
+      if (it >= C::wv_bufs) bad |= !wait_for(&m.wv_free[wb][half], (it / C::wv_bufs - 1) & 1);
       tc_fence_after();
       if (mine) {
         const float* w = &m.w[sl][hd][32 * half + 2 * (lane & 3)];
@@ -895,7 +938,7 @@ __global__ void __launch_bounds__(kThreads, 1) linear_chunk_kernel(const __grid_
 #pragma unroll
       for (int i = 0; i < kNS; ++i) s[i] = 0.f;
     } else {
-      bad |= !mbar_wait(&m.init_full, 0);
+      bad |= !wait_for(&m.init_full, 0);
       // Columns that nothing uses before the state is there: the second chunk's D, and OI.
       auto columns = [&](int n) { return tm + (n < 64 ? C::x + 64 + n : C::oi + n - 64) + tl; };
 #pragma unroll 1
@@ -934,8 +977,8 @@ __global__ void __launch_bounds__(kThreads, 1) linear_chunk_kernel(const __grid_
     for (int it = 0; it < n_chunks; ++it) {
       const int sl = it % kSums, db = it % C::ds_bufs;
       // S = e^{c_C} S + dS.
-      bad |= !mbar_wait(&m.sums[sl], (it / kSums) & 1);
-      bad |= !mbar_wait(&m.ds_full[db], (it / C::ds_bufs) & 1);
+      bad |= !wait_for(&m.sums[sl], (it / kSums) & 1);
+      bad |= !wait_for(&m.ds_full[db], (it / C::ds_bufs) & 1);
       tc_fence_after();
       if (__any_sync(0xffffffffu, bad)) {
         bad = true;
@@ -964,7 +1007,7 @@ __global__ void __launch_bounds__(kThreads, 1) linear_chunk_kernel(const __grid_
         mbar_arrive(&m.sums_free[sl]);
       }
       if (FULL && it + 1 < n_chunks) {
-        bad |= !mbar_wait(&m.s_free, it & 1);  // the operand has been read
+        bad |= !wait_for(&m.s_free, it & 1);  // the operand has been read
         tc_fence_after();
         if (__any_sync(0xffffffffu, bad)) {
           bad = true;
@@ -974,7 +1017,7 @@ __global__ void __launch_bounds__(kThreads, 1) linear_chunk_kernel(const __grid_
       }
     }
     // The state after the last chunk, through shared memory: every tile there has been read.
-    if (FULL) bad |= !mbar_wait(&m.o_full[(n_chunks - 1) & 1], ((n_chunks - 1) >> 1) & 1);
+    if (FULL) bad |= !wait_for(&m.o_full[(n_chunks - 1) & 1], ((n_chunks - 1) >> 1) & 1);
     if (!FULL || (u.ends_row() && l.state)) {
 #pragma unroll
       for (int n = 0; n < kNS; n += 8) {
@@ -1170,6 +1213,7 @@ int launch_linear_chunks(const LinearParams& l, int dtype, void* workspace, int6
   p.seg_state = static_cast<float*>(workspace);
   p.seg_decay = reinterpret_cast<float*>(static_cast<char*>(workspace) + x.state_bytes);
   p.err_host = host_error_word();
+  p.wait_ns = static_cast<uint32_t>(std::min(flag_wait_limit_ns(), 0xffffffffull));
   const unsigned grid = static_cast<unsigned>(x.rows * x.segs);
   if (x.segs > 1) {
     launch_any<false>(p, grid, stream);

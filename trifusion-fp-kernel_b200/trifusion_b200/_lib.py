@@ -168,8 +168,9 @@ def check_device_error():
 
 
 def set_flag_wait_ns(ns):
-    """Limit of the kernels' waits on other CTAs' chunk flags in later launches, in
-    nanoseconds (0: the default 2 s). A diagnostic control for tests."""
+    """Limit of the recurrence kernels' waits on other CTAs' chunk flags, and of the chunked
+    linear attention's waits, in later launches, in nanoseconds (0: the default 2 s). A
+    diagnostic control for tests."""
     check(lib().tf_set_flag_wait_ns(int(ns)))
 
 
