@@ -21,22 +21,33 @@ __device__ __forceinline__ float ld_f(const bf16* p) { return bf2f(__ldg(p)); }
 __device__ __forceinline__ void st_f(float* p, float x) { *p = x; }
 __device__ __forceinline__ void st_f(bf16* p, float x) { *p = __float2bfloat16_rn(x); }
 
-// The factor e^g of a log decay g; near 1 (its sign bit is set then) e^g - 1, to which the state
-// itself is added: with e^g errors of the factor add up over a long memory (3e-9 a token, all one
-// way, 1.7e-5 of the state after 4680 tokens of slow decay; now 1.3e-6). -inf (a reset) gives
-// exactly 0; NaN stays NaN.
-__device__ __forceinline__ float decay_factor(float g) {
-  // The Taylor series of e^g - 1 to g^7: the rest is below 2^-25 of it for |g| < 0.35.
+// The factor e^g of a log decay g. Rounded to FP32, errors of the factor add up over a long memory
+// (3e-9 a token, all one way: 1.7e-5 of the state after 4680 tokens of slow decay, now 1.1e-6). So
+// near 1 it is e^g rounded down, and what that leaves is applied too: with the factor of a next token,
+// or as a second factor. Both are above zero for every finite g, so that an infinite state stays
+// what it is (S + (e^g - 1) S would be inf - inf). 0 gives exactly 1, -inf exactly 0, NaN stays.
+constexpr float kTiny = 0x1p-149f;  // FP32's smallest number
+__device__ __forceinline__ bool near_one(float g) { return g <= 0.f && g > -0.35f; }
+// e^g - 1 by its Taylor series to g^7: the rest is below 2^-25 of it where near_one(g).
+__device__ __forceinline__ float decay_less_one(float g) {
   float x = 1.f / 5040.f;
   x = fmaf(x, g, 1.f / 720.f);
   x = fmaf(x, g, 1.f / 120.f);
   x = fmaf(x, g, 1.f / 24.f);
   x = fmaf(x, g, 1.f / 6.f);
   x = fmaf(x, g, 0.5f);
-  x = fmaf(x, g * g, g);
-  return g <= 0.f && g > -0.35f ? -fabsf(x) : ex2_approx(g * kLog2e);
+  return fmaf(x, g * g, g);
 }
-__device__ __forceinline__ bool near_one(float factor) { return __float_as_int(factor) < 0; }
+// 1 + x for -0.35 < x < 2^-24, rounded down; x is left with the rest (both differences are exact).
+__device__ __forceinline__ float take_factor(float& x) {
+  const float down = __fadd_rd(1.f, x);
+  x = (1.f - down) + x;
+  return down;
+}
+__device__ __forceinline__ float far_factor(float g) {
+  const float e = ex2_approx(g * kLog2e);
+  return e == 0.f && g > -INFINITY ? kTiny : e;
+}
 
 // ---- recurrent form ------------------------------------------------------------
 // One block: one row, one head, 32 columns of its state. Thread (warp w, lane l) holds columns
@@ -66,7 +77,7 @@ __global__ void __launch_bounds__(32 * WARPS, NR == 8 ? 4 : 2) linear_scan_kerne
   static_assert(kBatch % WARPS == 0 && kBatch * kRows % kThreads == 0, "a batch is shared out evenly");
   __shared__ alignas(16) float kq[2][kBatch][2][kRows];
   __shared__ alignas(16) float vs[2][kBatch][32];
-  __shared__ float as[2][kBatch], partial[2][kBatch][WARPS][32];
+  __shared__ float as[2][kBatch], rest, partial[2][kBatch][WARPS][32];
   const int slices = (p.P + 31) / 32;
   const int slice = blockIdx.x % slices;
   const int row = blockIdx.x / slices;
@@ -112,7 +123,7 @@ __global__ void __launch_bounds__(32 * WARPS, NR == 8 ? 4 : 2) linear_scan_kerne
   const float* g = p.decay + b * p.sg[0] + h * p.sg[1];
   // What a thread brings of the batch from t0 on. Tokens past the length change nothing: zeros, and
   // no decay.
-  float kn[kLoads], qn[kLoads], vn[kOwn], gn;
+  float kn[kLoads], qn[kLoads], vn[kOwn], gn, left = 0.f;
   auto load = [&](int64_t t0) {
 #pragma unroll
     for (int j = 0; j < kLoads; ++j) {
@@ -137,7 +148,18 @@ __global__ void __launch_bounds__(32 * WARPS, NR == 8 ? 4 : 2) linear_scan_kerne
     }
 #pragma unroll
     for (int j = 0; j < kOwn; ++j) vs[x][w * kOwn + j][lane] = vn[j];
-    if (threadIdx.x < kBatch) as[x][threadIdx.x] = decay_factor(gn);
+    if (w == 0) {  // token after token, each with what the factors before it left
+      const float own = near_one(gn) ? decay_less_one(gn) : 0.f;
+      float factor = far_factor(gn);
+#pragma unroll
+      for (int j = 0; j < kBatch; ++j) {
+        left += __shfl_sync(0xffffffffu, own, j);
+        const float near = take_factor(left);
+        if (lane == j && near_one(gn)) factor = near;
+      }
+      if (lane < kBatch) as[x][lane] = factor;
+      if (lane == 0) rest = left;
+    }
   };
   load(0);
   store(0);
@@ -151,7 +173,6 @@ __global__ void __launch_bounds__(32 * WARPS, NR == 8 ? 4 : 2) linear_scan_kerne
     for (int t = 0; t < kBatch; ++t) {
       const float a = as[x][t];
       const float2 factor = make_float2(a, a);
-      const bool keep = near_one(a);
       const float4 vr = *reinterpret_cast<const float4*>(&vs[x][t][4 * (lane & 7)]);
       const float2 vv[4] = {make_float2(vr.x, vr.x), make_float2(vr.y, vr.y), make_float2(vr.z, vr.z),
                             make_float2(vr.w, vr.w)};
@@ -162,7 +183,7 @@ __global__ void __launch_bounds__(32 * WARPS, NR == 8 ? 4 : 2) linear_scan_kerne
         const float2 qq = *reinterpret_cast<const float2*>(&kq[x][t][1][r0 + 2 * i]);
 #pragma unroll
         for (int c = 0; c < 4; ++c) {
-          s[c][i] = fma2(kk, vv[c], fma2(factor, s[c][i], keep ? s[c][i] : make_float2(0.f, 0.f)));
+          s[c][i] = fma2(factor, s[c][i], mul2(kk, vv[c]));
           o[c] = fma2(qq, s[c][i], o[c]);
         }
       }
@@ -190,13 +211,18 @@ __global__ void __launch_bounds__(32 * WARPS, NR == 8 ? 4 : 2) linear_scan_kerne
   }
   if (on)
     for (int64_t t = len + w; t < p.T; t += WARPS) st_f(out + t * p.so[1], 0.f);
-  if (p.state && c0 < p.P && (len > 0 || p.fresh))
+  if (p.state && c0 < p.P && (len > 0 || p.fresh)) {
+    const float more = fmaxf(rest, kTiny);  // what the factors left
 #pragma unroll
     for (int i = 0; i < NR; ++i)
       if (r0 + i < p.N) {
-        auto at = [&](int c) { return i % 2 ? s[c][i / 2].y : s[c][i / 2].x; };
+        auto at = [&](int c) {
+          const float y = i % 2 ? s[c][i / 2].y : s[c][i / 2].x;
+          return fmaf(more, y, y);
+        };
         *reinterpret_cast<float4*>(st + i * p.P) = make_float4(at(0), at(1), at(2), at(3));
       }
+  }
 }
 
 constexpr int kStepThreads = 256;
@@ -246,19 +272,15 @@ __global__ void __launch_bounds__(kStepThreads, NR > 4 ? 3 : NR == 4 ? 5 : CS ==
 #pragma unroll
     for (int j = 0; j < 4; ++j)
       if (col + 32 * c < p.P) vv[c][j] = ld_f(v + 32 * c + j);
-  float a = decay_factor(p.decay[b * p.sg[0] + h * p.sg[1]]);
+  const float g = p.decay[b * p.sg[0] + h * p.sg[1]];
+  float more = near_one(g) ? decay_less_one(g) : 0.f, a = take_factor(more);
+  if (!near_one(g)) a = far_factor(g);
   bool dead = !in_pool;  // no state of its own
   if (p.slots) {
     for (int i = threadIdx.x; i < b; i += kStepThreads) dead |= p.slots[i] == slot;
     dead = __syncthreads_or(dead);
   }
-  if (!near_one(a)) {  // apart, so that the usual case stays at two operations a value
-#pragma unroll
-    for (int c = 0; c < CS; ++c)
-#pragma unroll
-      for (int i = 0; i < NR; ++i) s[c][i] = make_float4(a * s[c][i].x, a * s[c][i].y, a * s[c][i].z, a * s[c][i].w);
-    a = 0.f;
-  }
+  const float2 a0 = make_float2(a, a), a1 = make_float2(fmaxf(more, kTiny), fmaxf(more, kTiny));
   float4 o[CS];
 #pragma unroll
   for (int c = 0; c < CS; ++c) o[c] = make_float4(0.f, 0.f, 0.f, 0.f);
@@ -271,14 +293,13 @@ __global__ void __launch_bounds__(kStepThreads, NR > 4 ? 3 : NR == 4 ? 5 : CS ==
       for (int c = 0; c < CS; ++c)
         if (CS == 1 || col + 32 * c < p.P) {
           float4& x = s[c][i];
-          x.x = fmaf(kn, vv[c][0], fmaf(a, x.x, x.x));
-          x.y = fmaf(kn, vv[c][1], fmaf(a, x.y, x.y));
-          x.z = fmaf(kn, vv[c][2], fmaf(a, x.z, x.z));
-          x.w = fmaf(kn, vv[c][3], fmaf(a, x.w, x.w));
-          o[c].x = fmaf(qn, x.x, o[c].x);
-          o[c].y = fmaf(qn, x.y, o[c].y);
-          o[c].z = fmaf(qn, x.z, o[c].z);
-          o[c].w = fmaf(qn, x.w, o[c].w);
+          const float2 k2 = make_float2(kn, kn), q2 = make_float2(qn, qn);
+          const float2 lo = make_float2(x.x, x.y), hi = make_float2(x.z, x.w);
+          const float2 y = fma2(a0, lo, fma2(a1, lo, mul2(k2, make_float2(vv[c][0], vv[c][1]))));
+          const float2 z = fma2(a0, hi, fma2(a1, hi, mul2(k2, make_float2(vv[c][2], vv[c][3]))));
+          x = make_float4(y.x, y.y, z.x, z.y);
+          const float2 oy = fma2(q2, y, make_float2(o[c].x, o[c].y)), oz = fma2(q2, z, make_float2(o[c].z, o[c].w));
+          o[c] = make_float4(oy.x, oy.y, oz.x, oz.y);
           __stcs(reinterpret_cast<float4*>(st + 32 * i * p.P + 32 * c), x);
         }
     }

@@ -63,6 +63,8 @@ constexpr int kSums = 4;              // chunks whose decay sums are kept
 // A decay below it is zero in FP32 against any state. (64 of them in a chunk add up to 2^14,
 // where the sums' steps are 2^-10: weights within 2^-10 or so, less than P's rounding.)
 constexpr float kMinLog2 = -256.f;
+// In place of a state's factor that is zero in FP32, so that an infinite state stays infinite.
+constexpr float kTiny = 0x1p-149f;
 
 // Warps, by what they do; groups of four have the four quarters of the TMEM lanes, pairs of
 // groups the two halves of a chunk's tokens.
@@ -674,7 +676,8 @@ __global__ void __launch_bounds__(kThreads, 1) linear_chunk_kernel(const __grid_
           put(m.w[sl][x], tok + j < live ? ex2_approx(after[j]) : 0.f, tok + j + 1 < live ? ex2_approx(after[j + 1]) : 0.f);
         }
         if (lane % kLanes == 0) {
-          m.total[sl][x] = ex2_approx(total);
+          const float e = ex2_approx(total);
+          m.total[sl][x] = e == 0.f ? kTiny : e;
           m.factors[sl][x] = factors;
         }
         seg_total += total;
@@ -1088,7 +1091,7 @@ __global__ void __launch_bounds__(256) linear_join_kernel(const __grid_constant_
   *reinterpret_cast<float4*>(own) = s;
 #pragma unroll 4
   for (int g = 1; g < segs; ++g) {
-    const float a = ex2_approx(p.seg_decay[row * p.segs + g - 1]);
+    const float e = ex2_approx(p.seg_decay[row * p.segs + g - 1]), a = e == 0.f ? kTiny : e;
     const float4 d = __ldcg(reinterpret_cast<const float4*>(own + g * step));
     s.x = fmaf(a, s.x, d.x);
     s.y = fmaf(a, s.y, d.y);
