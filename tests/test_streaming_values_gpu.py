@@ -3,7 +3,7 @@
 import pytest
 import torch
 
-from streaming_reference import check_state, recurrence
+from streaming_reference import check_out, check_state, recurrence
 
 pytestmark = pytest.mark.gpu
 
@@ -13,6 +13,7 @@ if not torch.cuda.is_available():
 from trifusion_b200 import linear_attention, linear_attention_step  # noqa: E402
 
 DEV = "cuda"
+CHUNKED = ("chunks", "pair", "segments")
 INF, NAN = float("inf"), float("nan")
 FORMS = ["step", "tokens", "wide", "chunks", "pair", "segments"]
 
@@ -74,3 +75,22 @@ def test_infinite_states_stay_infinite(form):
     share = out.shape[2] // q.shape[2]
     sign = q[:, :, :, 3].sign().repeat_interleave(share, dim=2)[live][:, :2]
     assert (out[live][:, :2, 5].float() == sign * INF).all()
+
+
+@pytest.mark.parametrize("form", FORMS)
+@pytest.mark.parametrize("bad", [NAN, INF])
+def test_resets_forget_states_that_are_not_finite(form, bad):
+    """A decay of -inf on the first token, inside, on the last, on none and behind a length."""
+    q, k, v, decay, state, lengths = operands(form, 1)
+    t, n = q.shape[1], q.shape[3]
+    first = t if lengths is None else int(lengths.min())
+    decay[:, 0, 0] = decay[:, 1, first // 2] = decay[:, 2, t - 1] = -INF
+    state[0] = bad
+    state[1, :, 3, 5] = bad
+    out, new = run(form, q, k, v, decay, state, lengths)
+    ref, s, mag, smag = recurrence(q, k, v, decay, state, lengths)
+    check_finite_part(new, s, smag, t, n)
+    good = ref.isfinite() & mag.isfinite()
+    assert torch.equal(out.isfinite(), good) and good[:, :, 0].all() and good[0, first // 2:, 1].all()
+    keep = lambda x: torch.where(good, x, torch.zeros_like(x))  # noqa: E731
+    check_out(keep(out), keep(ref), keep(mag), t, n, form in CHUNKED)

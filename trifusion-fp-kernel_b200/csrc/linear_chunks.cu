@@ -78,7 +78,7 @@ constexpr int kThreads = 32 * 32;
 // The state's four warps hold 64 or 128 values a thread.
 template <int NK>
 struct Regs {
-  static constexpr int state = NK == 1 ? 120 : 168, prep = NK == 1 ? 56 : 48, score = NK == 1 ? 56 : 40,
+  static constexpr int state = NK == 1 ? 120 : 152, prep = NK == 1 ? 56 : 48, score = NK == 1 ? 56 : 48,
                        out = 56, single = 56;
   static_assert(4 * state + 8 * (prep + score + out) + 4 * single == 2048, "what was launched");
 };
@@ -127,8 +127,9 @@ struct alignas(16) Misc {
   float col[kSums][2][kC];              // -c_j (log2) where a factor would leave FP32's range
   float ecs[kSums][2][kC];              // scale e^{c_i}
   float w[kSums][2][kC];                // e^{c_C - c_j}, 0 past the length
-  float total[kSums][2];                // e^{c_C}
+  float total[kSums][2];                // e^{c_C}, below zero where a decay is -inf
   int factors[kSums][2];                // row and col hold factors
+  int reset[kSums][2];                  // the first token with a decay of -inf, where there is one
 };
 // Shared memory, in bytes from a 1024-byte boundary: as many stages (chunks) as fit, up to
 // six. The value tiles of a pair of heads lie around one zero tile, .. a1 a0 zero b0 b1 ..: a
@@ -274,6 +275,9 @@ __device__ __forceinline__ void tmem_st8(uint32_t taddr, const uint32_t (&r)[8])
   asm volatile("tcgen05.st.sync.aligned.32x32b.x8.b32 [%0], {%1,%2,%3,%4,%5,%6,%7,%8};" ::"r"(taddr), "r"(r[0]),
                "r"(r[1]), "r"(r[2]), "r"(r[3]), "r"(r[4]), "r"(r[5]), "r"(r[6]), "r"(r[7])
                : "memory");
+}
+__device__ __forceinline__ void tmem_st1(uint32_t taddr, uint32_t r) {
+  asm volatile("tcgen05.st.sync.aligned.32x32b.x1.b32 [%0], {%1};" ::"r"(taddr), "r"(r) : "memory");
 }
 __device__ __forceinline__ void tmem_wait_st() { asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory"); }
 // 16 TMEM lanes x 16 columns as m16n8 fragments: thread t gets lanes t/4 and t/4 + 8,
@@ -623,6 +627,9 @@ __global__ void __launch_bounds__(kThreads, 1) linear_chunk_kernel(const __grid_
       const int x = lane / kLanes, tok = lane % kLanes * kT;
       const bool mine = x < u.nheads;
       float seg_total = 0.f;
+      // This lane's decays of the chunk that is loaded next, and how many are before the length.
+      const float* ahead = l.decay + u.b * l.sg[0] + (u.head0 + x) * l.sg[1] + (u.first * kC + tok) * l.sg[2];
+      int left = mine ? u.len - u.first * kC - tok : 0;
 #pragma unroll 1
       for (int it = 0; it < n_chunks; ++it) {
         const int sl = it % kSums, live = u.live(it);
@@ -632,7 +639,14 @@ __global__ void __launch_bounds__(kThreads, 1) linear_chunk_kernel(const __grid_
           const float a = decays[j] * kLog2e;
           c[j] = a < kMinLog2 ? kMinLog2 : a;  // NaN stays
         }
-        if (it + 1 < n_chunks) load_decays(u, it + 1, decays);
+        float was[kT];
+#pragma unroll
+        for (int j = 0; j < kT; ++j) was[j] = decays[j];
+        ahead += kC * l.sg[2], left -= kC;
+        if (it + 1 < n_chunks) {
+#pragma unroll
+          for (int j = 0; j < kT; ++j) decays[j] = j < left ? ahead[j * l.sg[2]] : 0.f;
+        }
         // Sums up to each token, and of those after it, without subtracting large sums.
         after[kT - 1] = 0.f;
 #pragma unroll
@@ -681,6 +695,19 @@ __global__ void __launch_bounds__(kThreads, 1) linear_chunk_kernel(const __grid_
           m.factors[sl][x] = factors;
         }
         seg_total += total;
+        // A decay of -inf, after which nothing of the state before may be left, also where that is not
+        // finite. (Such a chunk's sum is kMinLog2 or less.)
+        if (__builtin_expect(__any_sync(0xffffffffu, total <= kMinLog2), 0)) {
+          int reset = kC;
+#pragma unroll
+          for (int j = kT - 1; j >= 0; --j) reset = was[j] == -INFINITY ? tok + j : reset;
+#pragma unroll 1
+          for (int o = 1; o < kLanes; o <<= 1) reset = min(reset, __shfl_xor_sync(0xffffffffu, reset, o, kLanes));
+          if (reset < kC) {
+            if (lane % kLanes == 0) m.total[sl][x] = -1.f, m.reset[sl][x] = reset;
+            seg_total = -INFINITY;
+          }
+        }
         __syncwarp();
         if (lane == 0) mbar_arrive(&m.sums[sl]);
       }
@@ -703,11 +730,20 @@ __global__ void __launch_bounds__(kThreads, 1) linear_chunk_kernel(const __grid_
       for (int it = 0; it < n_chunks; ++it) {
         const int sl = it % kSums, t0 = (u.first + it) * kC + 32 * half;
         bad |= !wait_for(&m.sums[sl], (it / kSums) & 1);
+        const bool resets = m.total[sl][hd < u.nheads ? hd : 0] < 0.f;
         bad |= !wait_for(&m.o_full[it & 1], (it >> 1) & 1);
         tc_fence_after();
-        if (__any_sync(0xffffffffu, bad)) {
-          bad = true;
-          break;
+        if (__any_sync(0xffffffffu, bad || resets)) {
+          if (__any_sync(0xffffffffu, bad)) {
+            bad = true;
+            break;
+          }
+          // From a decay of -inf on, tokens have nothing of the state: their columns of OI are zero, also
+          // where the state is not finite. (One branch for the two rare cases: of its own it cost 2 %.)
+#pragma unroll 1
+          for (int t = max(m.reset[sl][hd < u.nheads ? hd : 0] - 32 * half, 0); t < 32; ++t)
+            tmem_st1(tm + C::oi + 32 * half + t + tl, 0u);
+          tmem_wait_st();
         }
         if (lane == 0) tma_store_wait_read();
         __syncwarp();
@@ -981,13 +1017,17 @@ __global__ void __launch_bounds__(kThreads, 1) linear_chunk_kernel(const __grid_
       const int sl = it % kSums, db = it % C::ds_bufs;
       // S = e^{c_C} S + dS.
       bad |= !wait_for(&m.sums[sl], (it / kSums) & 1);
+      const float a = m.total[sl][hd < u.nheads ? hd : 0];
       bad |= !wait_for(&m.ds_full[db], (it / C::ds_bufs) & 1);
       tc_fence_after();
       if (__any_sync(0xffffffffu, bad)) {
         bad = true;
         break;
       }
-      const float a = m.total[sl][hd < u.nheads ? hd : 0];
+      if (__builtin_expect(a < 0.f, 0)) {
+#pragma unroll
+        for (int i = 0; i < kNS; ++i) s[i] = 0.f;  // a decay of -inf: nothing of S, also where it is not finite
+      }
       constexpr int kBatch = NK == 1 ? 32 : 16;  // columns on their way at a time, as registers allow
 #pragma unroll
       for (int i = 0; i < kNS; i += kBatch) {
@@ -1091,7 +1131,8 @@ __global__ void __launch_bounds__(256) linear_join_kernel(const __grid_constant_
   *reinterpret_cast<float4*>(own) = s;
 #pragma unroll 4
   for (int g = 1; g < segs; ++g) {
-    const float e = ex2_approx(p.seg_decay[row * p.segs + g - 1]), a = e == 0.f ? kTiny : e;
+    const float total = p.seg_decay[row * p.segs + g - 1], e = ex2_approx(total), a = e == 0.f ? kTiny : e;
+    if (total == -INFINITY) s = make_float4(0.f, 0.f, 0.f, 0.f);  // a decay of -inf in the segment
     const float4 d = __ldcg(reinterpret_cast<const float4*>(own + g * step));
     s.x = fmaf(a, s.x, d.x);
     s.y = fmaf(a, s.y, d.y);

@@ -94,7 +94,8 @@ def linear_attention(q, k, v, decay, state=None, *, slots=None, lengths=None, sc
 
     * ``q``, ``k`` [B,T,Hq,N], ``v`` [B,T,H,P], BF16 or FP32, H a multiple of Hq, N and P
       multiples of 8 up to 256; ``decay`` FP32 [B,H,T], or [H] for one decay a head: natural
-      logs, at most 0 in use; ``-inf`` forgets everything before.
+      logs, at most 0 in use; ``-inf`` forgets everything before, states that are not finite
+      included (an entry of a pool needs no clearing where its first decay is ``-inf``).
     * ``state`` FP32 [B,H,N,P] is the state before the first token and is overwritten by
       the state after the last. With ``slots`` (int64 [B]) it is a pool [slots,H,N,P] and row
       b works on entry ``slots[b]``. A row with a negative slot is padding: its output is
@@ -109,7 +110,8 @@ def linear_attention(q, k, v, decay, state=None, *, slots=None, lengths=None, sc
     BF16 operands with N and P up to 128 run on the tensor cores in chunks of 64 tokens
     (FP32 sums and state). A non-finite value in v then also reaches the earlier tokens of
     its chunk, and, with P up to 64, a non-finite weight (a NaN in a head's decays, say) the
-    outputs of the head next to it under the same key head. FP32 operands, wider heads and
+    outputs of the head next to it under the same key head; a decay of ``-inf`` does not stop
+    what is not finite in the tokens of its own chunk. FP32 operands, wider heads and
     pieces of up to 16 tokens run token by token. There is no backward pass.
     """
     op = "linear_attention"
