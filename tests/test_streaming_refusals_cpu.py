@@ -1,0 +1,46 @@
+"""Arguments of the streaming operators that are refused before anything is launched (no GPU)."""
+
+import itertools
+
+import pytest
+import torch
+
+from trifusion_b200 import linear_attention, linear_attention_step
+
+
+def prompt(b=2, t=5, h=4, hq=2, n=64, p=64):
+    z = lambda *s: torch.zeros(*s, dtype=torch.bfloat16)  # noqa: E731
+    return [z(b, t, hq, n), z(b, t, hq, n), z(b, t, h, p), torch.zeros(b, h, t)]
+
+
+def step(b=2, h=4, hq=2, n=64, p=64):
+    z = lambda *s: torch.zeros(*s, dtype=torch.bfloat16)  # noqa: E731
+    return [z(b, hq, n), z(b, hq, n), z(b, h, p), torch.zeros(b, h)]
+
+
+SIZE = 64 * 64
+
+
+@pytest.mark.parametrize("strides", [(SIZE, SIZE), (2 * SIZE, SIZE), (SIZE, 2 * SIZE), (3 * SIZE, 2 * SIZE + 4),
+                                     (5 * SIZE, 2 * SIZE + 4)])
+def test_pools_whose_entries_meet_are_refused(strides):
+    """Head 0 of one entry in head 1 (2, 3) of another, wholly or in part."""
+    state = torch.zeros(40 * SIZE).as_strided((3, 4, 64, 64), (*strides, 64, 1))
+    with pytest.raises(ValueError, match="linear_attention: .*overlap"):
+        linear_attention(*prompt(b=3), state)
+    with pytest.raises(ValueError, match="linear_attention_step: .*overlap"):
+        linear_attention_step(*step(b=3), state)
+
+
+def test_which_pools_meet():
+    """The rule against every pair of entries, and pools that only look as if they met."""
+    from trifusion_b200.linear_recurrence import _meet
+
+    for s0, n0, s1, n1 in itertools.product(range(4, 30), (2, 3, 5), range(4, 30), (2, 4)):
+        at = sorted(i * s0 + j * s1 for i in range(n0) for j in range(n1))
+        assert _meet(s0, n0, s1, n1, 4) == any(b - a < 4 for a, b in zip(at, at[1:])), (s0, n0, s1, n1)
+    for strides in ((4 * SIZE, SIZE), (SIZE, 3 * SIZE), (3 * SIZE, 5 * SIZE)):  # (nested, transposed, interleaved)
+        state = torch.zeros(40 * SIZE).as_strided((3, 4 if strides[0] != 3 * SIZE else 2, 64, 64), (*strides, 64, 1))
+        h = state.shape[1]
+        with pytest.raises(RuntimeError, match="CUDA tensors"):
+            linear_attention(*prompt(b=3, h=h), state)

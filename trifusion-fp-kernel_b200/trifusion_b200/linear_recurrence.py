@@ -40,6 +40,14 @@ def _operands(op, dtype, q, k, v, decay, hq, h, n, p):
     return code
 
 
+def _meet(s0, n0, s1, n1, size):
+    """Whether two of the n0 x n1 pieces of ``size`` values at i * s0 + j * s1 overlap (neither stride
+    being below ``size``)."""
+    if s0 >= s1 * (n1 - 1) + size or s1 >= s0 * (n0 - 1) + size:
+        return False
+    return any(0 < i < n0 and abs(j * s1 - i * s0) < size for j in range(1, n1) for i in (j * s1 // s0, j * s1 // s0 + 1))
+
+
 def _check_state(op, state, slots, b, h, n, p):
     """Checks a state and its slots; returns the state's strides over slots and heads."""
     shape = state.shape
@@ -48,7 +56,8 @@ def _check_state(op, state, slots, b, h, n, p):
     s0, s1, s2, s3 = state.stride()
     if s3 != 1 or s2 != p or s0 % 4 or s1 % 4 or state.data_ptr() % 16:
         raise ValueError(f"{op}: state must be contiguous over [N,P], its heads on 16-byte boundaries")
-    if (s1 < n * p and h > 1) or (s0 < n * p and shape[0] > 1):
+    size, pool = n * p, shape[0]
+    if (s1 < size and h > 1) or (s0 < size and pool > 1) or (h > 1 and pool > 1 and _meet(s0, pool, s1, h, size)):
         raise ValueError(f"{op}: the states of a pool must not overlap")
     if state.requires_grad and torch.is_grad_enabled():
         raise RuntimeError(f"{op}: {_lib.NO_GRADIENT}")
