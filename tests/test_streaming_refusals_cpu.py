@@ -5,7 +5,7 @@ import itertools
 import pytest
 import torch
 
-from trifusion_b200 import linear_attention, linear_attention_step
+from trifusion_b200 import apply_rotary, linear_attention, linear_attention_step, rotary_frequencies
 
 
 def prompt(b=2, t=5, h=4, hq=2, n=64, p=64):
@@ -44,3 +44,24 @@ def test_which_pools_meet():
         h = state.shape[1]
         with pytest.raises(RuntimeError, match="CUDA tensors"):
             linear_attention(*prompt(b=3, h=h), state)
+
+
+def test_written_tensors_that_overlap_in_part_are_refused():
+    """Windows that slide by less than they hold: two tokens, or two heads, share elements."""
+    f, _ = rotary_frequencies(32, device="cpu")
+    row = torch.zeros(4096, dtype=torch.bfloat16)
+    for strides in ((1280, 256, 32, 1), (1280, 192, 64, 1), (640, 256, 64, 1), (1280, 2, 512, 1)):
+        x = row.as_strided((2, 5, 4, 64), strides)
+        with pytest.raises(ValueError, match="linear_attention: .*overlap"):
+            linear_attention(*prompt(), out=x)
+        with pytest.raises(ValueError, match="apply_rotary: .*overlap"):
+            apply_rotary(x, None, torch.arange(5), f, inplace=True)
+        with pytest.raises(ValueError, match="apply_rotary: .*overlap"):
+            apply_rotary(torch.zeros(2, 5, 4, 64, dtype=torch.bfloat16), x, torch.arange(5), f, inplace=True)
+    # Slices, transposed views and rows with a gap between them are apart.
+    wide = torch.zeros(2, 4, 7, 80, dtype=torch.bfloat16)
+    for x in (wide[:, :, 1:6, 8:72].transpose(1, 2), wide.transpose(1, 2)[:, :5, :, :64], wide[:, :1, :5, :64].transpose(1, 2)):
+        with pytest.raises(RuntimeError, match="CUDA tensors"):
+            linear_attention(*prompt(h=x.shape[2], hq=1), out=x)
+        with pytest.raises(RuntimeError, match="CUDA tensors"):
+            apply_rotary(x, None, torch.arange(5), f, inplace=True)

@@ -198,6 +198,18 @@ def require_cuda(op, *tensors):
     return dev
 
 
+def overlaps_itself(x):
+    """Whether elements of ``x`` may lie on one another: some stride does not span what the smaller ones
+    reach. (Slices and transposed views of a tensor always pass.)"""
+    reach = 1
+    for step, n in sorted(zip(x.stride(), x.shape)):
+        if n > 1:
+            if step < reach:
+                return True
+            reach += step * (n - 1)
+    return False
+
+
 NO_GRADIENT = "no backward pass; detach the operands or call it under torch.no_grad()"
 
 

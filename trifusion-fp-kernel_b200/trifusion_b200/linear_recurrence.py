@@ -72,7 +72,7 @@ def _check_state(op, state, slots, b, h, n, p):
 def _check_out(op, out, v):
     if out.shape != v.shape or out.dtype != v.dtype or out.stride(-1) != 1:
         raise ValueError(f"{op}: out must be like v with a unit stride in the last dimension")
-    if any(s == 0 and n > 1 for s, n in zip(out.stride(), out.shape)):
+    if out.numel() and not out.is_contiguous() and _lib.overlaps_itself(out):
         raise ValueError(f"{op}: out must not overlap itself")
     if out.requires_grad and torch.is_grad_enabled():
         raise RuntimeError(f"{op}: {_lib.NO_GRADIENT}")

@@ -58,10 +58,6 @@ def rotary_frequencies(rotary_dim, base=10000.0, *, scaling=None, factor=1.0, tr
     return freq.to(device), amplitude
 
 
-def _repeats(x):
-    return any(step == 0 and n > 1 for step, n in zip(x.stride(), x.shape))
-
-
 def apply_rotary(q, k, positions, inv_freq, *, layout="half", amplitude=1.0, inplace=False):
     """Rotate ``q`` ([B, T, H, D]) and ``k`` ([B, T, Hk, D], or None) by ``positions * inv_freq``.
 
@@ -99,8 +95,9 @@ def apply_rotary(q, k, positions, inv_freq, *, layout="half", amplitude=1.0, inp
     if inplace:
         if q.stride(3) != 1 or k is not None and k.stride(3) != 1:
             raise ValueError("apply_rotary: in place needs a unit stride in the last dimension")
-        if _repeats(q) or k is not None and _repeats(k):
-            raise ValueError("apply_rotary: in place needs tensors that do not overlap themselves")
+        for x in (q, k):
+            if x is not None and not x.is_contiguous() and _lib.overlaps_itself(x):
+                raise ValueError("apply_rotary: in place needs tensors that do not overlap themselves")
     if grad and torch.is_grad_enabled():
         raise RuntimeError("apply_rotary: " + _lib.NO_GRADIENT)
     if index < 0 or not same or positions.get_device() != index or inv_freq.get_device() != index:
