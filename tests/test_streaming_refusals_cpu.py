@@ -65,3 +65,15 @@ def test_written_tensors_that_overlap_in_part_are_refused():
             linear_attention(*prompt(h=x.shape[2], hq=1), out=x)
         with pytest.raises(RuntimeError, match="CUDA tensors"):
             apply_rotary(x, None, torch.arange(5), f, inplace=True)
+
+
+def test_rotating_one_tensor_twice_in_place_is_refused():
+    f, _ = rotary_frequencies(32, device="cpu")
+    x = torch.zeros(2, 5, 4, 64)
+    for q, k in ((x, x), (x, x[:, :, :1]), (x[:, :, :2], x)):
+        with pytest.raises(ValueError, match="apart"):
+            apply_rotary(q, k, torch.arange(5), f, inplace=True)
+        with pytest.raises(RuntimeError, match="CUDA tensors"):
+            apply_rotary(q, k, torch.arange(5), f)
+    with pytest.raises(RuntimeError, match="CUDA tensors"):
+        apply_rotary(x[:, :, :2], x[:, :, 2:], torch.arange(5), f, inplace=True)

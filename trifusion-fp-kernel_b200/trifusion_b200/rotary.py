@@ -98,6 +98,8 @@ def apply_rotary(q, k, positions, inv_freq, *, layout="half", amplitude=1.0, inp
         for x in (q, k):
             if x is not None and not x.is_contiguous() and _lib.overlaps_itself(x):
                 raise ValueError("apply_rotary: in place needs tensors that do not overlap themselves")
+        if k is not None and q.data_ptr() == k.data_ptr() and q.numel() and k.numel():
+            raise ValueError("apply_rotary: in place needs q and k apart from each other")
     if grad and torch.is_grad_enabled():
         raise RuntimeError("apply_rotary: " + _lib.NO_GRADIENT)
     if index < 0 or not same or positions.get_device() != index or inv_freq.get_device() != index:
