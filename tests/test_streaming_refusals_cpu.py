@@ -77,3 +77,30 @@ def test_rotating_one_tensor_twice_in_place_is_refused():
             apply_rotary(q, k, torch.arange(5), f)
     with pytest.raises(RuntimeError, match="CUDA tensors"):
         apply_rotary(x[:, :, :2], x[:, :, 2:], torch.arange(5), f, inplace=True)
+
+
+@pytest.mark.parametrize("grad", [True, False])
+def test_tangents_are_refused(grad):
+    """A dual tensor's tangent would be dropped; torch.no_grad() does not turn forward mode off."""
+    import torch.autograd.forward_ad as fw
+
+    f, _ = rotary_frequencies(32, device="cpu")
+    x = torch.zeros(1, 5, 2, 64)
+    state = torch.zeros(2, 4, 64, 64)
+    with torch.set_grad_enabled(grad), fw.dual_level():
+        dual = lambda y: fw.make_dual(y, torch.ones_like(y))  # noqa: E731
+        for i in range(4):
+            for make, call in ((prompt, linear_attention), (step, linear_attention_step)):
+                args = make()
+                args[i] = dual(args[i])
+                with pytest.raises(RuntimeError, match=f"{call.__name__}: .*forward mode"):
+                    call(*args, state)
+        with pytest.raises(RuntimeError, match="linear_attention_step: .*forward mode"):
+            linear_attention_step(*step(), dual(state))
+        with pytest.raises(RuntimeError, match="linear_attention: .*forward mode"):
+            linear_attention(*prompt(), out=dual(prompt()[2]))
+        for args in ((dual(x), x, torch.arange(5), f), (x, dual(x), torch.arange(5), f), (x, None, torch.arange(5), dual(f))):
+            with pytest.raises(RuntimeError, match="apply_rotary: .*forward mode"):
+                apply_rotary(*args)
+        with pytest.raises(RuntimeError, match="CUDA tensors"):  # other tensors' tangents do not matter
+            linear_attention(*prompt())

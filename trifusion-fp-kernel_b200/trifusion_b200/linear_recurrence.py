@@ -131,6 +131,8 @@ def linear_attention(q, k, v, decay, state=None, *, slots=None, lengths=None, sc
     vb, vt, h, p = v.shape
     if vb != b or vt != t:
         raise ValueError(f"{op}: q and k must be [B,T,Hq,N] and v [B,T,H,P]")
+    if _lib.has_tangent(q, k, v, decay, state, out):
+        raise RuntimeError(f"{op}: {_lib.NO_TANGENT}")
     dtype, index = _operands(op, q.dtype, q, k, v, decay, hq, h, n, p), q.get_device()
     sg, shape = decay.stride(), decay.shape
     if shape == (h,) and sg:
@@ -209,6 +211,8 @@ def linear_attention_step(q, k, v, decay, state, *, slots=None, scale=None, out=
     vb, h, p = v.shape
     if vb != b:
         raise ValueError(f"{op}: q and k must be [B,Hq,N] and v [B,H,P]")
+    if _lib.has_tangent(q, k, v, decay, state, out):
+        raise RuntimeError(f"{op}: {_lib.NO_TANGENT}")
     dtype, index = _operands(op, q.dtype, q, k, v, decay, hq, h, n, p), q.get_device()
     sg, shape = decay.stride(), decay.shape
     if shape == (h,) and sg:

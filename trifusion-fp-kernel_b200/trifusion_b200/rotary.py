@@ -102,6 +102,8 @@ def apply_rotary(q, k, positions, inv_freq, *, layout="half", amplitude=1.0, inp
             raise ValueError("apply_rotary: in place needs q and k apart from each other")
     if grad and torch.is_grad_enabled():
         raise RuntimeError("apply_rotary: " + _lib.NO_GRADIENT)
+    if _lib.has_tangent(q, k, inv_freq):
+        raise RuntimeError("apply_rotary: " + _lib.NO_TANGENT)
     if index < 0 or not same or positions.get_device() != index or inv_freq.get_device() != index:
         raise RuntimeError("apply_rotary: all tensors must be CUDA tensors on one device")
     if not inv_freq.is_contiguous():
