@@ -104,3 +104,13 @@ def test_tangents_are_refused(grad):
                 apply_rotary(*args)
         with pytest.raises(RuntimeError, match="CUDA tensors"):  # other tensors' tangents do not matter
             linear_attention(*prompt())
+
+
+def test_a_gradient_of_the_frequencies_is_refused():
+    f, _ = rotary_frequencies(32, device="cpu")
+    f.requires_grad_()
+    x = torch.zeros(1, 5, 2, 64)
+    with pytest.raises(RuntimeError, match="apply_rotary: .*backward"):
+        apply_rotary(x, x, torch.arange(5), f)
+    with torch.no_grad(), pytest.raises(RuntimeError, match="CUDA tensors"):
+        apply_rotary(x, x, torch.arange(5), f)

@@ -100,7 +100,7 @@ def apply_rotary(q, k, positions, inv_freq, *, layout="half", amplitude=1.0, inp
                 raise ValueError("apply_rotary: in place needs tensors that do not overlap themselves")
         if k is not None and q.data_ptr() == k.data_ptr() and q.numel() and k.numel():
             raise ValueError("apply_rotary: in place needs q and k apart from each other")
-    if grad and torch.is_grad_enabled():
+    if (grad or inv_freq.requires_grad) and torch.is_grad_enabled():
         raise RuntimeError("apply_rotary: " + _lib.NO_GRADIENT)
     if _lib.has_tangent(q, k, inv_freq):
         raise RuntimeError("apply_rotary: " + _lib.NO_TANGENT)
