@@ -56,7 +56,8 @@ const char* tf_last_cuda_error(void);
 /* Device-side error word of the current device: non-zero after one of a
  * recurrence or chunked linear-attention kernel's bounded waits gave up (on the tensor core, on the other
  * warps of its CTA, or on another CTA's chunk flag); the kernel then finishes
- * instead of hanging, and the outputs of that launch are invalid. Synchronous;
+ * instead of hanging, and the outputs of that launch are invalid. 1: a recurrence
+ * kernel, 3: a chunked linear-attention kernel (also the host-mapped word). Synchronous;
  * `reset` != 0 clears it (and the host-mapped word below). */
 int tf_device_error(int reset);
 

@@ -5,7 +5,7 @@ import itertools
 import pytest
 import torch
 
-from trifusion_b200 import apply_rotary, linear_attention, linear_attention_step, rotary_frequencies
+from trifusion_b200 import _lib, apply_rotary, linear_attention, linear_attention_step, rotary_frequencies
 
 
 def prompt(b=2, t=5, h=4, hq=2, n=64, p=64):
@@ -114,3 +114,23 @@ def test_a_gradient_of_the_frequencies_is_refused():
         apply_rotary(x, x, torch.arange(5), f)
     with torch.no_grad(), pytest.raises(RuntimeError, match="CUDA tensors"):
         apply_rotary(x, x, torch.arange(5), f)
+
+
+@pytest.mark.parametrize("error,text", [(1, "a recurrence kernel"), (2, "a recurrence kernel"), (3, "a linear attention kernel")])
+def test_the_error_names_the_operator_that_gave_up(monkeypatch, error, text):
+    class Fake:
+        cleared = 0
+
+        def tf_device_error_pending(self):
+            return 0 if self.cleared else error
+
+        def tf_device_error(self, reset):
+            self.cleared += reset
+            return error
+
+    fake = Fake()
+    monkeypatch.setattr(_lib, "lib", lambda: fake)
+    monkeypatch.setitem(_lib._watch, "ready", True)
+    with pytest.raises(RuntimeError, match=f"{text} gave up one of its bounded waits"):
+        _lib.check_device_error()
+    _lib.check_device_error()  # once

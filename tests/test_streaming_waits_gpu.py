@@ -47,7 +47,7 @@ def test_waits_that_run_out_raise_on_the_next_call(shape, limit):
     assert gave_up == (_lib.lib().tf_device_error(0) != 0)
     assert gave_up or limit > 1 or t == 17  # (with the longer limits, or where nothing is polled, all waits may end in time)
     if gave_up:
-        with pytest.raises(RuntimeError, match="bounded waits"):
+        with pytest.raises(RuntimeError, match="linear attention kernel gave up one of its bounded waits"):
             linear_attention(*args, state.clone())
     assert _lib.lib().tf_device_error(0) == 0 and _lib.lib().tf_device_error_pending() == 0
     again = linear_attention(*args, state.clone())

@@ -83,7 +83,8 @@ struct Regs {
   static_assert(4 * state + 8 * (prep + score + out) + 4 * single == 2048, "what was launched");
 };
 
-__device__ int g_linear_error = 0;    // 1: a bounded wait gave up
+constexpr int kLinearGaveUp = 3;      // (1 and 2 are the recurrence kernels')
+__device__ int g_linear_error = 0;    // kLinearGaveUp: a bounded wait gave up
 
 struct ChunkParams {
   CUtensorMap tm_q, tm_k, tm_v, tm_o;
@@ -1094,9 +1095,9 @@ __global__ void __launch_bounds__(kThreads, 1) linear_chunk_kernel(const __grid_
   tc_fence_before();
   const bool any = __syncthreads_or(bad);
   if (any && tid == 0) {
-    atomicExch(&g_linear_error, 1);
+    atomicExch(&g_linear_error, kLinearGaveUp);
     if (p.err_host) {
-      *reinterpret_cast<volatile int*>(p.err_host) = 1;
+      *reinterpret_cast<volatile int*>(p.err_host) = kLinearGaveUp;
       __threadfence_system();
     }
   }

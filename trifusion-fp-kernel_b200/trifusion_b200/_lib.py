@@ -143,6 +143,9 @@ def check(status):
 
 DEVICE_ERROR_MESSAGE = ("trifusion_b200: a recurrence kernel gave up one of its bounded waits "
                         "(outputs of that launch are invalid)")
+LINEAR_ERROR_MESSAGE = ("trifusion_b200: a linear attention kernel gave up one of its bounded waits "
+                        "(outputs and states of that launch are invalid)")
+_LINEAR_ERROR = 3  # tf_device_error_pending() then
 _watch = {"ready": False}
 
 
@@ -162,9 +165,11 @@ def check_device_error():
     """Raise ``RuntimeError`` if an earlier launch recorded a device-side timeout
     (read from the host-mapped word: no synchronisation). The word is cleared, so
     the error is raised once."""
-    if _watch["ready"] and lib().tf_device_error_pending():
-        lib().tf_device_error(1)
-        raise RuntimeError(DEVICE_ERROR_MESSAGE)
+    if _watch["ready"]:
+        error = lib().tf_device_error_pending()
+        if error:
+            lib().tf_device_error(1)
+            raise RuntimeError(LINEAR_ERROR_MESSAGE if error == _LINEAR_ERROR else DEVICE_ERROR_MESSAGE)
 
 
 def set_flag_wait_ns(ns):
