@@ -221,16 +221,6 @@ NO_GRADIENT = "no backward pass; detach the operands or call it under torch.no_g
 NO_TANGENT = "no derivatives in forward mode; pass the operands' primal values"
 
 
-def has_tangent(*tensors):
-    """Whether one of the tensors (None among them) carries a tangent of forward-mode differentiation.
-    (Also under ``torch.no_grad()``, which leaves that mode on.)"""
-    from torch.autograd import forward_ad
-
-    if getattr(forward_ad, "_current_level", 0) < 0:  # outside any dual level, as nearly always
-        return False
-    return any(x is not None and forward_ad.unpack_dual(x).tangent is not None for x in tensors)
-
-
 def launch(fn, device, *args):
     """Call a C-ABI entry point on `device`'s current stream and check its status."""
     import torch

@@ -17,6 +17,7 @@ import functools
 import torch
 
 from . import _lib
+from ._autograd import has_tangent, written
 
 _launch = _lib.launcher("tf_linear_attention_fwd", "9Q2q17qd8i")  # tf_linear_attention_io
 _DTYPES = {torch.float32: _lib.TF_F32, torch.bfloat16: _lib.TF_BF16}
@@ -131,7 +132,7 @@ def linear_attention(q, k, v, decay, state=None, *, slots=None, lengths=None, sc
     vb, vt, h, p = v.shape
     if vb != b or vt != t:
         raise ValueError(f"{op}: q and k must be [B,T,Hq,N] and v [B,T,H,P]")
-    if _lib.has_tangent(q, k, v, decay, state, out):
+    if has_tangent(q, k, v, decay, state, out):
         raise RuntimeError(f"{op}: {_lib.NO_TANGENT}")
     dtype, index = _operands(op, q.dtype, q, k, v, decay, hq, h, n, p), q.get_device()
     sg, shape = decay.stride(), decay.shape
@@ -157,7 +158,8 @@ def linear_attention(q, k, v, decay, state=None, *, slots=None, lengths=None, sc
     if q3 != 1 or k3 != 1 or v3 != 1:
         q, k, v = [x if x.stride(3) == 1 else x.contiguous() for x in (q, k, v)]
         (q0, q1, q2, _), (k0, k1, k2, _), (v0, v1, v2, _) = q.stride(), k.stride(), v.stride()
-    if out is None:
+    given = out is not None
+    if not given:
         out, o0, o1, o2 = torch.empty_like(v, memory_format=torch.contiguous_format), t * h * p, h * p, p
     else:
         o0, o1, o2, _ = out.stride()
@@ -193,6 +195,10 @@ def linear_attention(q, k, v, decay, state=None, *, slots=None, lengths=None, sc
             dtype, fresh, b, t, h, hq, n, p)
     if into is not out:
         out.copy_(into)
+    if not fresh:
+        written(state)
+    if given:
+        written(out)
     return out, state
 
 
@@ -211,7 +217,7 @@ def linear_attention_step(q, k, v, decay, state, *, slots=None, scale=None, out=
     vb, h, p = v.shape
     if vb != b:
         raise ValueError(f"{op}: q and k must be [B,Hq,N] and v [B,H,P]")
-    if _lib.has_tangent(q, k, v, decay, state, out):
+    if has_tangent(q, k, v, decay, state, out):
         raise RuntimeError(f"{op}: {_lib.NO_TANGENT}")
     dtype, index = _operands(op, q.dtype, q, k, v, decay, hq, h, n, p), q.get_device()
     sg, shape = decay.stride(), decay.shape
@@ -241,11 +247,15 @@ def linear_attention_step(q, k, v, decay, state, *, slots=None, scale=None, out=
     if slots is not None:
         slots = slots.contiguous()
         slot = slots.data_ptr()
-    if out is None:
+    given = out is not None
+    if not given:
         out, ob, oh = torch.empty_like(v, memory_format=torch.contiguous_format), h * p, p
     else:
         ob, oh, _ = out.stride()
     _launch(index, q.data_ptr(), k.data_ptr(), v.data_ptr(), out.data_ptr(), decay.data_ptr(), state.data_ptr(), slot, 0,
             0, 0, state.shape[0], qb, 0, qh, kb, 0, kh, vb, 0, vh, *sg, 0, ob, 0, oh, *ss,
             n ** -0.5 if scale is None else scale, dtype, 0, b, 1, h, hq, n, p)
+    written(state)
+    if given:
+        written(out)
     return out

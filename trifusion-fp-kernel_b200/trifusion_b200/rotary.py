@@ -15,6 +15,7 @@ import math
 import torch
 
 from . import _lib
+from ._autograd import has_tangent, written
 
 _DTYPES = {torch.float32: _lib.TF_F32, torch.bfloat16: _lib.TF_BF16}
 _LAYOUTS = {"half": 0, "interleaved": 1}
@@ -102,7 +103,7 @@ def apply_rotary(q, k, positions, inv_freq, *, layout="half", amplitude=1.0, inp
             raise ValueError("apply_rotary: in place needs q and k apart from each other")
     if (grad or inv_freq.requires_grad) and torch.is_grad_enabled():
         raise RuntimeError("apply_rotary: " + _lib.NO_GRADIENT)
-    if _lib.has_tangent(q, k, inv_freq):
+    if has_tangent(q, k, inv_freq):
         raise RuntimeError("apply_rotary: " + _lib.NO_TANGENT)
     if index < 0 or not same or positions.get_device() != index or inv_freq.get_device() != index:
         raise RuntimeError("apply_rotary: all tensors must be CUDA tensors on one device")
@@ -133,4 +134,8 @@ def apply_rotary(q, k, positions, inv_freq, *, layout="half", amplitude=1.0, inp
     _launch(index, q.data_ptr(), kp, qo.data_ptr(), kop, positions.data_ptr(), inv_freq.data_ptr(), q0, q1, q2, k0, k1, k2,
             p0, p1, p2, o0, o1, o2, 0 if len(s) == 1 else s[0], s[-1], amplitude, dtype, interleaved, b, t, h, hk, d,
             2 * half)
+    if inplace:
+        written(q)
+        if k is not None:
+            written(k)
     return qo if k is None else (qo, ko)
