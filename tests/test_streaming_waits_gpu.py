@@ -20,7 +20,7 @@ from trifusion_b200 import linear_attention  # noqa: E402
 DEV = "cuda"
 SHAPES = [  # rows, tokens, heads, key heads, N, P
     (1, 17, 1, 1, 64, 64),       # one partial chunk
-    (2, 600, 3, 1, 128, 64),     # segments, a pair and a single head
+    (2, 1200, 3, 1, 128, 64),    # segments, a pair and a single head
     (1, 2000, 2, 2, 128, 128),   # segments of one wide head
     (80, 300, 2, 1, 64, 128),    # many rows
 ]
