@@ -72,8 +72,9 @@ int tf_error_watch_init(void);
 int tf_device_error_pending(void);
 
 /* Limit, in nanoseconds, of a recurrence kernel's waits on other CTAs' chunk
- * flags, and of the waits in a chunked linear-attention kernel (4.2 s at most), in
- * later launches (0 restores the default of 2 s). A diagnostic
+ * flags, and of the waits in a chunked linear-attention kernel (counted in tries of
+ * 4 us; below 4000 its loads do not wait at all, so that every row that has to wait
+ * gives up), in later launches (0 restores the default of 2 s). A diagnostic
  * control: a launch whose wait runs out records the error above and completes
  * with invalid outputs. Waits inside a recurrence kernel's CTA, and those for copies
  * and products in flight before a CTA ends, keep their fixed 2 s limit. */

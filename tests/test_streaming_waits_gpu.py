@@ -1,8 +1,8 @@
 """Waits of the chunked linear attention that run out reach the caller as exceptions (GPU only).
 
-The limit of the kernel's waits is lowered until ordinary ones, for tiles on their way or for
-the step before, run out. The launch must end by itself, the next call must raise, and the one after
-it must give what it gave before. Nothing is faulted and the context stays usable.
+With a limit of less than one try of 4 us, loads do not wait for room, so that all that wait for
+their tiles give up. The launch must end by itself, the next call must raise, and the one after it
+must give what it gave before. Nothing is faulted and the context stays usable.
 """
 
 import pytest
@@ -26,7 +26,7 @@ SHAPES = [  # rows, tokens, heads, key heads, N, P
 ]
 
 
-@pytest.mark.parametrize("limit", [1, 500, 2000, 5000])
+@pytest.mark.parametrize("limit", [1, 3999, 1000000])
 @pytest.mark.parametrize("shape", SHAPES)
 def test_waits_that_run_out_raise_on_the_next_call(shape, limit):
     b, t, h, hq, n, p = shape
@@ -45,7 +45,7 @@ def test_waits_that_run_out_raise_on_the_next_call(shape, limit):
         _lib.set_flag_wait_ns(0)
     gave_up = _lib.lib().tf_device_error_pending() != 0
     assert gave_up == (_lib.lib().tf_device_error(0) != 0)
-    assert gave_up or limit > 1 or t == 17  # (with the longer limits, or where nothing is polled, all waits may end in time)
+    assert gave_up == (limit < 4000 and t > 17)  # (one chunk waits for no room)
     if gave_up:
         with pytest.raises(RuntimeError, match="linear attention kernel gave up one of its bounded waits"):
             linear_attention(*args, state.clone())

@@ -75,11 +75,14 @@ constexpr int kPrepWarp = 4, kScoreWarp = 12, kOutWarp = 20;  // (state: 0)
 constexpr int kSumWarp = 28, kStateMmaWarp = 29, kOutMmaWarp = 30, kLoadWarp = 31;
 constexpr int kThreads = 32 * 32;
 // Registers of a thread: 32 warps have 64 at launch, 2048 together, and share them out again.
-// The state's four warps hold 64 or 128 values a thread.
-template <int NK>
+// The state's four warps hold 64 or 128 values a thread. (What the compiler spills hangs on these
+// numbers in no simple way: with 168 for the state of N > 64 it is 200 to 300 bytes a thread of other
+// warps.) A wide segment's own state has no scores, and spills nothing with their registers.
+template <int NK, bool WIDE, bool FULL>
 struct Regs {
-  static constexpr int state = NK == 1 ? 120 : 152, prep = NK == 1 ? 56 : 48, score = NK == 1 ? 56 : 48,
-                       out = 56, single = 56;
+  static constexpr bool own = NK == 2 && WIDE && !FULL;
+  static constexpr int state = NK == 1 ? 120 : own ? 200 : 152, prep = NK == 1 ? 56 : 48,
+                       score = NK == 1 ? 56 : own ? 24 : 48, out = 56, single = 56;
   static_assert(4 * state + 8 * (prep + score + out) + 4 * single == 2048, "what was launched");
 };
 
@@ -96,7 +99,7 @@ struct ChunkParams {
   float* seg_state;   // [B*H][segs][N][P]: the state before each segment
   float* seg_decay;   // [B*H][segs]: log2 decay over the segment
   int* err_host;
-  uint32_t wait_ns;   // limit of the kernel's waits
+  uint32_t tries;     // limit of the kernel's waits
 };
 
 // What a CTA works on. Its warps read it from shared memory where they start: few of them
@@ -203,24 +206,13 @@ __device__ __forceinline__ bool bar_or(int id, int n, bool x) {
       : "memory");
   return r != 0;
 }
-// Waits for the phase with `parity` to complete; false after `limit` ns. Its first try suspends the
-// thread for longer than an ordinary wait takes, so that the limit is looked at only in a wait for
-// something that does not come.
-__device__ __forceinline__ bool wait_within(uint64_t* bar, uint32_t parity, uint32_t limit) {
-  if (mbar_try_wait(bar, parity)) return true;
-  const uint64_t t0 = global_timer_ns();
-  for (;;) {
-    if (mbar_try_wait(bar, parity)) return true;
-    if (global_timer_ns() - t0 > limit) return false;
-  }
-}
-// With a limit below a millisecond the thread is not suspended: the limit is kept from the first
-// moment on, and ordinary waits can run out. (Polling always cost 8 x 4097 tokens 3 %.)
-__device__ __forceinline__ bool wait_or_poll(uint64_t* bar, uint32_t parity, uint32_t limit) {
-  if (limit >= 1000000u) return wait_within(bar, parity, limit);
-  const uint64_t t0 = global_timer_ns();
-  while (!mbar_test_wait(bar, parity))
-    if (global_timer_ns() - t0 > limit) return false;
+// Waits for the phase with `parity` to complete; false after `tries` tries and one. A try suspends the
+// thread for up to 4 us (kTryNs, measured). Counted, not timed: the waits are a part of the code that
+// every warp fetches, and with a clock in each of them 24 x 3600 tokens of 12 heads took 5 % longer.
+constexpr uint32_t kTryNs = 4000, kTries = 2000000000u / kTryNs;
+__device__ __forceinline__ bool wait_tries(uint64_t* bar, uint32_t parity, uint32_t tries = kTries) {
+  for (uint32_t i = 0; !mbar_try_wait(bar, parity); ++i)
+    if (i >= tries) return false;
   return true;
 }
 __device__ __forceinline__ void mbar_arrive(uint64_t* bar) {
@@ -370,6 +362,7 @@ __global__ void __launch_bounds__(kThreads, 1) linear_chunk_kernel(const __grid_
   using L = Layout<NK, WIDE, FULL>;
   constexpr int kStages = L::stages;
   using C = Tmem<NK, FULL>;
+  using R = Regs<NK, WIDE, FULL>;
   extern __shared__ unsigned char smem_raw[];
   const uint32_t sb = (smem_u32(smem_raw) + 1023u) & ~1023u;
   Misc<kStages>& m = *reinterpret_cast<Misc<kStages>*>(smem_raw + (sb - smem_u32(smem_raw)) + L::misc);
@@ -377,9 +370,9 @@ __global__ void __launch_bounds__(kThreads, 1) linear_chunk_kernel(const __grid_
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
 
   // Waits of the kernel's steps for one another. One that gives up ends its warp's work: the warps
-  // behind it give up too, the copies and products already issued are waited for (mbar_wait, whose
-  // limit is fixed), TMEM is freed, and the launch leaves an error and invalid outputs and states.
-  auto wait_for = [&](uint64_t* bar, uint32_t parity) { return wait_within(bar, parity, p.wait_ns); };
+  // behind it give up too, the copies and products already issued are waited for (with a limit that
+  // is fixed), TMEM is freed, and the launch leaves an error and invalid outputs and states.
+  auto wait_for = [&](uint64_t* bar, uint32_t parity) { return wait_tries(bar, parity, p.tries); };
   // The states of this CTA's heads lie in pieces of neighbouring values: 64 rows at a time of
   // one wide head, or the heads of a pair.
   auto pieces = [&](const Unit& u) { return WIDE ? NK : u.nheads; };
@@ -482,7 +475,7 @@ __global__ void __launch_bounds__(kThreads, 1) linear_chunk_kernel(const __grid_
   bool bad = false;  // a bounded wait gave up
 
   if (warp >= kSumWarp) {
-    fewer_registers<Regs<NK>::single>();
+    fewer_registers<R::single>();
     const Unit u = m.unit;
     const int n_chunks = u.last - u.first;
     // A product warp ends when its products and their arrivals at barriers are done: none may still
@@ -490,7 +483,7 @@ __global__ void __launch_bounds__(kThreads, 1) linear_chunk_kernel(const __grid_
     auto drain = [&](int x) {
       if (elect_one()) umma_commit(&m.drained[x]);
       __syncwarp();
-      return __all_sync(0xffffffffu, mbar_wait(&m.drained[x], 0)) != 0;
+      return __all_sync(0xffffffffu, wait_tries(&m.drained[x], 0)) != 0;
     };
     if (warp == kLoadWarp && lane == 0) {
       // ---- loads ----------------------------------------------------------------
@@ -498,8 +491,10 @@ __global__ void __launch_bounds__(kThreads, 1) linear_chunk_kernel(const __grid_
       Ring<kStages> ring;
       for (int it = 0; it < n_chunks; ++it, ring.next()) {
         // The stages after the first are free once the state has been taken out of them.
-        if ((it == 1 && has_init && !wait_or_poll(&m.init_read, 0, p.wait_ns)) ||
-            (it >= kStages && !wait_or_poll(&m.empty[ring.st], ring.ph ^ 1, p.wait_ns))) {
+        // (A limit of less than one try: the first wait gives up, and all that wait for its tiles do.)
+        const bool first = it == 1 && has_init, later = it >= kStages;
+        if ((first || later) && p.tries == 0 || first && !wait_for(&m.init_read, 0) ||
+            later && !wait_for(&m.empty[ring.st], ring.ph ^ 1)) {
           bad = true;
           break;
         }
@@ -515,8 +510,8 @@ __global__ void __launch_bounds__(kThreads, 1) linear_chunk_kernel(const __grid_
         }
       }
       // No copy of this CTA may be in flight when it ends (also after a wait that gave up).
-      for (int i = max(0, issued - kStages); i < issued; ++i) bad |= !mbar_wait(&m.full[i % kStages], (i / kStages) & 1);
-      if (has_init) bad |= !mbar_wait(&m.init_full, 0);
+      for (int i = max(0, issued - kStages); i < issued; ++i) bad |= !wait_tries(&m.full[i % kStages], (i / kStages) & 1);
+      if (has_init) bad |= !wait_tries(&m.init_full, 0);
     } else if (warp == kStateMmaWarp) {
       // ---- products that need nothing of the state before --------------------------
       // The whole warp runs this, one lane issues: addresses stay in uniform registers.
@@ -718,7 +713,7 @@ __global__ void __launch_bounds__(kThreads, 1) linear_chunk_kernel(const __grid_
     __syncwarp();
   } else if (warp >= kOutWarp) {
     // ---- outputs ------------------------------------------------------------------------
-    fewer_registers<Regs<NK>::out>();
+    fewer_registers<R::out>();
     if (FULL) {
       const Unit u = m.unit;
       const int n_chunks = u.last - u.first;
@@ -798,7 +793,7 @@ __global__ void __launch_bounds__(kThreads, 1) linear_chunk_kernel(const __grid_
     }
   } else if (warp >= kScoreWarp) {
     // ---- scores to weights: P = D e^{c_i - c_j} for j <= i ------------------------------
-    fewer_registers<Regs<NK>::score>();
+    fewer_registers<R::score>();
     if (FULL) {
       const Unit u = m.unit;
       const int n_chunks = u.last - u.first;
@@ -884,7 +879,7 @@ __global__ void __launch_bounds__(kThreads, 1) linear_chunk_kernel(const __grid_
     }
   } else if (warp >= kPrepWarp) {
     // ---- weighted values, transposed into TMEM -------------------------------------------
-    fewer_registers<Regs<NK>::prep>();
+    fewer_registers<R::prep>();
     const Unit u = m.unit;
     const int n_chunks = u.last - u.first;
     const bool two = WIDE || u.nheads == 2;
@@ -957,7 +952,7 @@ __global__ void __launch_bounds__(kThreads, 1) linear_chunk_kernel(const __grid_
     if (!met) bar_or(2, 256, true);
   } else {
     // ---- state ------------------------------------------------------------------------------
-    more_registers<Regs<NK>::state>();
+    more_registers<R::state>();
     const Unit u = m.unit;
     const int n_chunks = u.last - u.first;
     const int row = 32 * q4 + lane;              // accumulator lane
@@ -1018,16 +1013,19 @@ __global__ void __launch_bounds__(kThreads, 1) linear_chunk_kernel(const __grid_
       const int sl = it % kSums, db = it % C::ds_bufs;
       // S = e^{c_C} S + dS.
       bad |= !wait_for(&m.sums[sl], (it / kSums) & 1);
-      const float a = m.total[sl][hd < u.nheads ? hd : 0];
+      float a = m.total[sl][hd < u.nheads ? hd : 0];
       bad |= !wait_for(&m.ds_full[db], (it / C::ds_bufs) & 1);
       tc_fence_after();
       if (__any_sync(0xffffffffu, bad)) {
         bad = true;
         break;
       }
-      if (__builtin_expect(a < 0.f, 0)) {
+      if (__builtin_expect(a < 0.f, 0)) {  // a decay of -inf: nothing of S, also where it is not finite
 #pragma unroll
-        for (int i = 0; i < kNS; ++i) s[i] = 0.f;  // a decay of -inf: nothing of S, also where it is not finite
+        for (int i = 0; i < kNS; i += 16)  // (in its place something finite, in few instructions)
+          tmem_ld16(tm + C::ds + 64 * NK * db + i + tl, *reinterpret_cast<float(*)[16]>(s + i));
+        tmem_wait_ld();
+        a = 0.f;
       }
       constexpr int kBatch = NK == 1 ? 32 : 16;  // columns on their way at a time, as registers allow
 #pragma unroll
@@ -1264,7 +1262,7 @@ int launch_linear_chunks(const LinearParams& l, int dtype, void* workspace, int6
   p.seg_state = static_cast<float*>(workspace);
   p.seg_decay = reinterpret_cast<float*>(static_cast<char*>(workspace) + x.state_bytes);
   p.err_host = host_error_word();
-  p.wait_ns = static_cast<uint32_t>(std::min(flag_wait_limit_ns(), 0xffffffffull));
+  p.tries = static_cast<uint32_t>(std::min(flag_wait_limit_ns() / kTryNs, 0xffffffffull));
   const unsigned grid = static_cast<unsigned>(x.rows * x.segs);
   if (x.segs > 1) {
     launch_any<false>(p, grid, stream);
