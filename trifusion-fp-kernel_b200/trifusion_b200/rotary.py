@@ -35,7 +35,8 @@ def rotary_frequencies(rotary_dim, base=10000.0, *, scaling=None, factor=1.0, tr
       frequency and divides the lowest by ``factor``;
     * ``"parts"``: frequencies that make fewer than ``turns[0]`` turns within
       ``trained_length`` positions are divided by ``factor``, those with more than
-      ``turns[1]`` kept, the ones between blended linearly; amplitude ``0.1 ln(factor) + 1``.
+      ``turns[1]`` kept, the ones between blended linearly in their turns (a model whose blend
+      is linear in the index of the frequency has others there); amplitude ``0.1 ln(factor) + 1``.
     """
     if rotary_dim < 2 or rotary_dim % 2:
         raise ValueError("rotary_frequencies: rotary_dim must be even and positive")
@@ -62,7 +63,8 @@ def rotary_frequencies(rotary_dim, base=10000.0, *, scaling=None, factor=1.0, tr
 def apply_rotary(q, k, positions, inv_freq, *, layout="half", amplitude=1.0, inplace=False):
     """Rotate ``q`` ([B, T, H, D]) and ``k`` ([B, T, Hk, D], or None) by ``positions * inv_freq``.
 
-    ``positions`` is int64 [B, T] or [T], any values (angles at 2^31 are within 1e-7 turns);
+    ``positions`` is int64 [B, T] or [T], any values (angles at 2^31 are within 1e-7 turns, and
+    the error grows with the position);
     ``inv_freq`` FP64 [R/2] with ``R <= D``: elements R.. of each head are copied. Pairs are
     ``(i, i + R/2)`` (``layout "half"``) or ``(2 i, 2 i + 1)`` (``"interleaved"``); a pair becomes ``amplitude * (x1 cos -
     x2 sin, x2 cos + x1 sin)``. q and k are FP32 or BF16 with any strides; R is at most 1024 and
