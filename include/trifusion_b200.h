@@ -547,7 +547,8 @@ int tf_rotary_positions_fwd(const tf_rotary_io* io, void* stream);
  *   S_t = e^decay[b,h,t] S_(t-1) + k_t v_t^T (key_dim x value_dim, FP32),
  *   out_t = scale * q_t S_t,
  * q, k [B,T,Hq,N], v and out [B,T,H,P] (FP32 or BF16), decay [B,H,T] FP32, N and P
- * multiples of 8 up to 256. `state` (nullable) [state_slots,H,N,P] FP32, 16-byte
+ * multiples of 8 up to 256. A decay of -inf forgets the state before it, also where that is
+ * not finite. `state` (nullable) [state_slots,H,N,P] FP32, 16-byte
  * aligned: row b starts from entry slots[b] (or b) and leaves its last state there;
  * with `fresh` it starts from zero instead. A negative slot: zero outputs, no state
  * changes; a slot >= state_slots or one that an earlier row has: NaN outputs, no

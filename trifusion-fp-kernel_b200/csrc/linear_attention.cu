@@ -58,15 +58,15 @@ __device__ __forceinline__ float far_factor(float g) {
 // behind which every warp sums up the output of some of its tokens. Bound by issue and, with few
 // blocks, by the latency of a token's chain. Up to two blocks an SM, eight warps with a whole batch
 // unrolled are faster, else four warps with half of it (fewer instructions for a token). FP32, us:
-//   1 x 7 tokens, 12 heads, N 128, P 64        24 blocks     eight 4.4   four  4.7
-//   2 x 3600, 12 heads, N 128, P 64            48 blocks     eight 510   four  639
-//   12 x 200, 12 heads, N 128, P 64           288 blocks     eight 49.4  four 54.7
-//   16 x 200, 12 heads, N 128, P 64           384 blocks     eight 74.1  four 72.0
-//   8 x 4097, 32 heads, N 64, P 64            512 blocks     eight 1356  four 1091
-//   32 x 7, 32 heads, N 128, P 64            2048 blocks     eight 30.1  four 22.2
-// (All with the rounded factor e^g; decay_factor's two forms take these to 4.6, 604 and, the larger
-// ones with four warps, 1137 and 23.1. 2 x 3600 with a barrier for every token: 1058 us; with a column
-// a lane: 800 us; the next batch loaded while one is worked on, not two: 694 us.)
+//   1 x 7 tokens, 12 heads, N 128, P 64        24 blocks     eight 4.5   four  4.9
+//   2 x 3600, 12 heads, N 128, P 64            48 blocks     eight 590   four  758
+//   12 x 200, 12 heads, N 128, P 64           288 blocks     eight 52.1  four 61.0
+//   16 x 200, 12 heads, N 128, P 64           384 blocks     eight 83.0  four 78.4
+//   8 x 4097, 32 heads, N 64, P 64            512 blocks     eight 1494  four 1190
+//   32 x 7, 32 heads, N 128, P 64            2048 blocks     eight 33.0  four 24.1
+// (2 x 3600, each against the kernel of its time: a barrier for every token 1058 against 510 us; a
+// column a lane 800 against 510; the next batch loaded while one is worked on, not two, 694 against
+// 604; both parts of a factor applied to each token 625 against 607.)
 template <typename T, int NR, int WARPS>
 __global__ void __launch_bounds__(32 * WARPS, NR == 8 ? 4 : 2) linear_scan_kernel(const __grid_constant__ LinearParams p) {
   constexpr int kThreads = 32 * WARPS, kRows = 4 * WARPS * NR;
@@ -248,7 +248,7 @@ constexpr int kStepThreads = 256;
 // shuffles and eight partial sums in shared memory. Bound by HBM: the states are
 // read and written once. They are streamed (evict-first): larger pools than the L2 would only
 // push each other out, smaller ones stay in it all the same. 64 rows of 32 heads, 128 x 128:
-// 43.4 us (268 MB, 94 % of the measured copy rate); 48.0 us with ordinary accesses, 45.1 and
+// 43.5 us (268 MB, 94 % of the measured copy rate); 48.0 us with ordinary accesses, 45.1 and
 // 46.6 us with four and six blocks an SM instead of five.
 template <typename T, int NR, int CS>
 __global__ void __launch_bounds__(kStepThreads, NR > 4 ? 3 : NR == 4 ? 5 : CS == 1 ? 6 : 4)

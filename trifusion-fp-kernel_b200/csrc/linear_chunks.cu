@@ -36,12 +36,13 @@
 // that do not. What decides: 64 registers a thread (shared out again by setmaxnreg) and code that
 // stays in the instruction cache - loops are kept rolled where unrolling them cost a fetch a pass.
 // Measured on a B200 (device time; copy rate 6552 GB/s):
-//   2 x 26 tokens, 4 heads, N 128, P 64        8.7 us   launch, set-up and two memory latencies
+//   2 x 26 tokens, 4 heads, N 128, P 64        9.0 us   launch, set-up and two memory latencies
 //   16 x 200 ragged, 12 heads, N 128, P 64    14.3 us   four chunks in a row of about 2400 cycles
-//   2 x 3600 ragged, 12 heads, N 128, P 64    34 us     5 chunks a segment, twice, and a join
-//   1 x 32768, 16 + 16 heads, 128 x 128      168 us     102 us at 5.2 TB/s, 58 us for the
-//                                                       segments' states (4.2 TB/s), join 8 us
-//   8 x 4097 ragged, 32 + 8 heads, 64 x 64    88 us     issue: 71 % of the slots of 128 SMs
+//   2 x 3600 ragged, 12 heads, N 128, P 64    34.9 us   5 chunks a segment, twice, and a join
+//   1 x 32768, 16 + 16 heads, 128 x 128      168 us     102 us at 5.1 TB/s, 58 us for the
+//                                                       segments' states (4.1 TB/s), join 8 us
+//   8 x 4097 ragged, 32 + 8 heads, 64 x 64    91 us     issue: 73 % of the slots of 128 SMs
+//   24 x 3600, 12 heads, N 128, P 64         100 us     144 CTAs, 57 chunks each
 #include <cuda.h>
 #include <cudaTypedefs.h>
 
@@ -93,7 +94,6 @@ struct ChunkParams {
   CUtensorMap tm_q, tm_k, tm_v, tm_o;
   LinearParams l;
   int pairs;       // CTAs of a k head: pairs of its heads (P <= 64), or its heads
-  int chunks;      // of T
   int segs;        // segments of the time axis
   int seg_chunks;  // chunks of a segment
   float* seg_state;   // [B*H][segs][N][P]: the state before each segment
@@ -735,7 +735,7 @@ __global__ void __launch_bounds__(kThreads, 1) linear_chunk_kernel(const __grid_
             break;
           }
           // From a decay of -inf on, tokens have nothing of the state: their columns of OI are zero, also
-          // where the state is not finite. (One branch for the two rare cases: of its own it cost 2 %.)
+          // where the state is not finite.
 #pragma unroll 1
           for (int t = max(m.reset[sl][hd < u.nheads ? hd : 0] - 32 * half, 0); t < 32; ++t)
             tmem_st1(tm + C::oi + 32 * half + t + tl, 0u);
@@ -1185,9 +1185,15 @@ struct Plan {
   int64_t rows, state_bytes, bytes;
 };
 
-// A prompt shorter than this runs token by token: 6.2, 10.8 and 38 us for 16 tokens (1, 16 and 32
-// rows of 12, 12 and 32 heads, N = 128, P = 64) against 9.5, 9.9 and 37 us in a chunk; 17 tokens take
-// 7, 12 and 44 us.
+// A prompt shorter than this runs token by token, in batches of eight tokens. With a carried state, us
+// token by token / in a chunk:
+//   N 128, P 64, 1 row of 12 heads, 16 of 12, 32 of 32
+//     12 tokens    6.8 / 9.6    11.3 / 10.1   41.0 / 37.8
+//     16           6.8 / 9.6    11.5 / 10.1   41.7 / 37.5
+//     17           8.2 / 9.6    14.5 / 10.0   53.9 / 37.5
+//   N 64, P 64, 1, 16 and 80 rows of 8 heads
+//     16           5.3 / 7.9     6.7 / 8.1    19.2 / 22.8
+//     17           6.4 / 7.8     8.1 / 8.1    24.4 / 22.8
 constexpr int kMinTokens = 17;
 
 bool plan_of(int B, int T, int H, int Hq, int N, int P, int dtype, Plan& x) {
@@ -1199,10 +1205,10 @@ bool plan_of(int B, int T, int H, int Hq, int N, int P, int dtype, Plan& x) {
   // As many segments as there are SMs for, of four chunks or more. Each is worked on twice, and the join
   // and the further launches take as long as six chunks; where that is no gain, rows stay whole.
   // 12 heads, N 128, P 64 (six CTAs a row), us cut / whole:
-  //   1 x 512, 1024, 3600 tokens     25.4 / 19.2   26.7 / 30.4   29.5 / 88.8
-  //   6 x 512, 1024, 3600            27.7 / 19.9   31.8 / 31.2   61.2 / 91.7
-  //   10 x 512, 1024, 3600           31.0 / 20.1   40.9 / 31.8   97.0 / 94.5
-  //   12 x 512, 1024, 3600           32.1 / 20.4   42.8 / 32.6   102.5 / 96.8
+  //   1 x 512, 1024, 3600 tokens     25.9 / 19.1   27.0 / 30.4   29.6 / 87.8
+  //   6 x 512, 1024, 3600            28.1 / 19.5   30.9 / 30.8   55.4 / 89.1
+  //   10 x 512, 1024, 3600           30.4 / 19.9   39.6 / 31.0   88.8 / 89.3
+  //   12 x 512, 1024, 3600           31.3 / 20.2   40.6 / 31.3   91.1 / 89.6
   const int64_t most = std::min<int64_t>(sm_count() / x.rows, (x.chunks + 3) / 4);
   x.seg_chunks = x.chunks;
   if (most > 1) {
@@ -1258,7 +1264,7 @@ int launch_linear_chunks(const LinearParams& l, int dtype, void* workspace, int6
   if (x.bytes > 0 && (!workspace || reinterpret_cast<uintptr_t>(workspace) % 256)) return TF_ERR_ARG;
   if (workspace_bytes < x.bytes) return TF_ERR_SIZE;
   p.l = l;
-  p.pairs = x.pairs, p.chunks = x.chunks, p.segs = x.segs, p.seg_chunks = x.seg_chunks;
+  p.pairs = x.pairs, p.segs = x.segs, p.seg_chunks = x.seg_chunks;
   p.seg_state = static_cast<float*>(workspace);
   p.seg_decay = reinterpret_cast<float*>(static_cast<char*>(workspace) + x.state_bytes);
   p.err_host = host_error_word();
