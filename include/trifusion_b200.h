@@ -53,12 +53,12 @@ int tf_version(void);
 /* Last CUDA error string recorded by this thread (static storage). */
 const char* tf_last_cuda_error(void);
 
-/* Device-side error word of the current device: non-zero after one of a
- * recurrence or chunked linear-attention kernel's bounded waits gave up (on the tensor core, on the other
- * warps of its CTA, or on another CTA's chunk flag); the kernel then finishes
- * instead of hanging, and the outputs of that launch are invalid. 1: a recurrence
- * kernel, 3: a chunked linear-attention kernel (also the host-mapped word). Synchronous;
- * `reset` != 0 clears it (and the host-mapped word below). */
+/* Device-side error word of the current device: non-zero after one of the bounded
+ * waits of a recurrence kernel (1) or a chunked linear-attention kernel (3) gave up
+ * (on the tensor core, on the other warps of its CTA, or on another CTA's chunk
+ * flag); the kernel then finishes instead of hanging, and the outputs of that launch
+ * are invalid. The host-mapped word below has the same values. Synchronous;
+ * `reset` != 0 clears it (and the host-mapped word). */
 int tf_device_error(int reset);
 
 /* Sets up a pinned, device-mapped host word that the kernels also set when a
